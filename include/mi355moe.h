@@ -387,6 +387,109 @@ int mi355moe_silu_and_mul_mxfp4_quant(uint8_t* out, const void* input, int in_dt
                                       int64_t hidden, int64_t group_size, float eps,
                                       void* stream);
 
+/* -------------------------------------------------------------------- norm */
+
+/* Root-mean-square norm of rows, with the residual's addition before it and
+ * its result in 16 / 32 bits, in e4m3 with a scale per group of columns, or
+ * both (no counterpart among the reference's MoE ops: it makes the layer's
+ * input, 16-bit for the router and pre-quantised for
+ * mi355moe_fused_moe_args::hidden_scale).  In fp32, with one rounding for
+ * each output:
+ *   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight
+ *   residual_out = T(h);  out = T(y)
+ *   per group of columns: a = max(max |y|, 1e-10),
+ *   s = max(a / 448, 1 / (448 * 512)), rounded up to a power of two for
+ *   scale_ue8m0 and for e8m0 scales; q = e4m3(clamp(y * (1 / s), +-448)).
+ * The norm and the quantiser take h and y before their rounding to T.  A NaN
+ * of y stays NaN in q and does not count in its group's maximum; a group
+ * with an infinite y has an infinite scale, zeros, and NaN at that y.
+ * Squares that overflow fp32 (|h| > 1.8e19) give y = 0, as the formula does
+ * in fp32.
+ *
+ * Rows: row r of x, residual, residual_out and out starts at element
+ * (r / inner) * outer_stride + (r % inner) * inner_stride of its pointer
+ * (heads inside a packed projection: inner = heads); columns are contiguous.
+ * inner = 1: plain rows with outer_stride.  q is [rows, cols] contiguous; the
+ * scale of (row r, group g) is at element r * scale_row + g * scale_group.
+ * out and residual_out may each be x or residual (same pointer and strides)
+ * but not the same of them; otherwise no output may overlap an input or
+ * another output. */
+typedef struct {
+  int dtype;          /* F32, BF16 or F16: x, residual, residual_out, out     */
+  int weight_dtype;   /* dtype, or F32                                        */
+  int64_t rows, cols, inner;
+  const void* x;
+  int64_t x_outer, x_inner;
+  const void* residual;      /* optional                                      */
+  int64_t residual_outer, residual_inner;
+  void* residual_out;        /* given exactly when residual is                */
+  int64_t residual_out_outer, residual_out_inner;
+  const void* weight;        /* [cols]                                        */
+  float eps;
+  void* out;                 /* optional when q is given                      */
+  int64_t out_outer, out_inner;
+  void* q;                   /* optional: e4m3 [rows, cols]                   */
+  void* scales;
+  int scale_dtype;           /* F32, or U8 for e8m0 codes                     */
+  int scale_ue8m0;           /* F32 scales rounded up to powers of two        */
+  int64_t group;             /* columns per scale: 32, 64 or 128              */
+  int64_t scale_row, scale_group;
+} mi355moe_rms_norm_args;
+int mi355moe_rms_norm(const mi355moe_rms_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------------ linear */
+
+typedef enum {
+  MI355MOE_LINEAR_NONE = 0,
+  MI355MOE_LINEAR_SILU = 1,
+  MI355MOE_LINEAR_GELU = 2,       /* erf form                                 */
+  MI355MOE_LINEAR_GELU_TANH = 3,
+  MI355MOE_LINEAR_RELU2 = 4,      /* max(z, 0)^2                              */
+  /* gated: weight has 2N rows, the gate's 0..N-1 and the factor's N..2N-1    */
+  MI355MOE_LINEAR_SILU_AND_MUL = 5,
+  MI355MOE_LINEAR_GELU_AND_MUL = 6,
+  MI355MOE_LINEAR_GELU_TANH_AND_MUL = 7
+} mi355moe_linear_activation;
+
+/* Matrix product with bias, activation and residual in its epilogue (no
+ * counterpart among the reference's MoE ops: the router's logits and the
+ * dense products beside the experts).  fp32 accumulation, one rounding:
+ *   z[m, n] = sum_k x[m, k] weight[n, k] + bias[n]
+ *   out[m, n] = T(act(z)[m, n] + residual[m, n]),  0 <= n < N;
+ * gated activations: act(z)[m, n] = f(z[m, n]) * z[m, N + n].
+ * x_dtype BF16 or F16: weight of the same type.  x_dtype FP8E4M3: weight
+ * e4m3, K % 128 == 0, z[m, n] = sum over 128-blocks b of K of
+ * x_scale[m, b] * weight_scale[n / 128, b] * sum_{k in b} x[m, k] weight[n, k].
+ * Row strides ld* and scale strides are in elements; columns of x, weight,
+ * bias, residual and out are contiguous.  M may be 0; N and K are positive.
+ * out may be residual with the same stride and type; otherwise it may overlap
+ * no input.  Products of few rows or few tiles split K and need the
+ * workspace of mi355moe_linear_workspace_size (0 for many sizes). */
+typedef struct {
+  int x_dtype;          /* BF16, F16 or FP8E4M3                               */
+  int out_dtype;        /* F32, BF16 or F16                                   */
+  int bias_dtype;       /* F32, BF16 or F16                                   */
+  int residual_dtype;   /* F32, BF16 or F16                                   */
+  int activation;       /* mi355moe_linear_activation                         */
+  int64_t M, N, K;
+  const void* x;
+  int64_t ldx;
+  const float* x_scale;             /* FP8E4M3                                */
+  int64_t x_scale_row, x_scale_blk;
+  const void* weight;               /* [N or 2N, K]                           */
+  int64_t ldw;
+  const float* weight_scale;        /* FP8E4M3: [ceil(rows / 128), K / 128]   */
+  int64_t weight_scale_row, weight_scale_blk;
+  const void* bias;                 /* optional [N or 2N]                     */
+  const void* residual;             /* optional [M, N]                        */
+  int64_t ldr;
+  void* out;                        /* [M, N]                                 */
+  int64_t ldo;
+} mi355moe_linear_args;
+size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* args);
+int mi355moe_linear(const mi355moe_linear_args* args, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------ grouped GEMM */
 
 /* Replaces torch.ops._xpu_C.cutlass_grouped_gemm_interface

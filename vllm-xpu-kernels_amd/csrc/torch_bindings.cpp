@@ -12,6 +12,9 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "../../include/mi355moe.h"
 
 namespace {
@@ -702,6 +705,295 @@ void silu_and_mul_mxfp4_quant(at::Tensor& out, const at::Tensor& input, at::Tens
            "silu_and_mul_mxfp4_quant");
 }
 
+// ------------------------------------------------------------ norm, linear
+// [first, last) bytes that a tensor's elements lie in (empty: first == last)
+std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {p, p};
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {p, p + static_cast<uintptr_t>(last + 1) * t.element_size()};
+}
+// rows of one stride whose columns lie apart: both tensors step through memory
+// by the same row stride, and within it their rows' bytes do not meet (a head
+// range of a packed projection beside another)
+bool interleaved_apart(const at::Tensor& a, const at::Tensor& b) {
+  if (a.dim() < 2 || b.dim() < 2) return false;
+  const int64_t row = a.stride(0) * static_cast<int64_t>(a.element_size());
+  if (row <= 0 || row != b.stride(0) * static_cast<int64_t>(b.element_size())) return false;
+  const auto x = extent(a.select(0, 0)), y = extent(b.select(0, 0));
+  const int64_t wa = static_cast<int64_t>(x.second - x.first);
+  const int64_t wb = static_cast<int64_t>(y.second - y.first);
+  int64_t d = static_cast<int64_t>(y.first) - static_cast<int64_t>(x.first);
+  d = ((d % row) + row) % row;
+  return d >= wa && d + wb <= row;
+}
+// an output shares no memory with another tensor, or (same_ok) is that tensor:
+// same start, type and strides
+void check_apart(const at::Tensor& out, const char* oname, const at::Tensor& t, const char* tname,
+                 bool same_ok) {
+  const auto a = extent(out), b = extent(t);
+  if (a.first >= b.second || b.first >= a.second) return;
+  const bool same = a.first == b.first && out.scalar_type() == t.scalar_type() &&
+                    out.sizes() == t.sizes() && out.strides() == t.strides();
+  TORCH_CHECK((same && same_ok) || interleaved_apart(out, t), oname, " must not overlap ", tname);
+}
+void check_here(const at::Tensor& t, const char* name, const at::Tensor& x) {
+  TORCH_CHECK(t.is_cuda(), name, " must be on a GPU device");
+  TORCH_CHECK(t.device() == x.device(), name, " must be on the device of the input");
+}
+bool float16or32(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 ||
+         t.scalar_type() == at::kHalf;
+}
+
+// Row strides of [.., cols] with contiguous columns: 1-D to 3-D as they are,
+// more leading dimensions where they fold into one stride.
+struct Rows {
+  int64_t outer = 0, inner = 0;
+};
+Rows rows_of(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
+  Rows r;
+  const int64_t d = t.dim();
+  for (int64_t i = 0; i + 1 < d; ++i) TORCH_CHECK(t.stride(i) >= 0, name, " has a negative stride");
+  if (d >= 2) r.inner = t.stride(d - 2);
+  if (d == 2) r = {t.stride(0), 0};
+  if (d >= 3) {
+    r.outer = t.stride(d - 3);
+    for (int64_t i = d - 4; i >= 0; --i)
+      TORCH_CHECK(t.size(i) <= 1 || t.stride(i) == t.stride(i + 1) * t.size(i + 1), name,
+                  " has leading dimensions that do not fold into one");
+  }
+  return r;
+}
+// written elements lie apart: strides, smallest first, step over what the
+// dimensions below cover
+void check_rows_apart(const at::Tensor& t, const char* name) {
+  if (t.numel() == 0 || t.is_contiguous()) return;
+  std::vector<std::pair<int64_t, int64_t>> s;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) s.emplace_back(t.stride(i), t.size(i));
+  std::sort(s.begin(), s.end());
+  int64_t cover = 1;
+  for (const auto& [st, n] : s) {
+    TORCH_CHECK(st >= cover, name, " must not overlap itself");
+    cover += st * (n - 1);
+  }
+}
+
+void rms_norm(const std::optional<at::Tensor>& out, const std::optional<at::Tensor>& q,
+              const std::optional<at::Tensor>& scales,
+              const std::optional<at::Tensor>& residual_out, const at::Tensor& input,
+              const at::Tensor& weight, const std::optional<at::Tensor>& residual,
+              double epsilon, int64_t group_size, bool scale_ue8m0) {
+  TORCH_CHECK(input.is_cuda(), "input must be on a GPU device");
+  TORCH_CHECK(input.dim() >= 1, "input must have at least one dimension");
+  TORCH_CHECK(float16or32(input), "input must be float32, bfloat16 or float16");
+  const int64_t cols = input.size(-1);
+  TORCH_CHECK(cols > 0, "input must have columns");
+  check_here(weight, "weight", input);
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == cols && weight.is_contiguous(),
+              "weight must be contiguous [hidden_size]");
+  TORCH_CHECK(weight.scalar_type() == input.scalar_type() || weight.scalar_type() == at::kFloat,
+              "weight must have the input's type or be float32");
+  TORCH_CHECK(residual.has_value() == residual_out.has_value(),
+              "residual and residual_out go together");
+  TORCH_CHECK(out.has_value() || q.has_value(), "out or q must be given");
+  TORCH_CHECK(q.has_value() == scales.has_value(), "q and scales go together");
+  mi355moe_rms_norm_args a{};
+  a.dtype = dtype_code(input.scalar_type());
+  a.weight_dtype = dtype_code(weight.scalar_type());
+  a.cols = cols;
+  a.rows = input.numel() / cols;
+  a.inner = input.dim() >= 3 ? input.size(-2) : 1;
+  if (a.inner == 0) a.inner = 1;
+  a.eps = static_cast<float>(epsilon);
+  auto like_input = [&](const at::Tensor& t, const char* name) {
+    check_here(t, name, input);
+    TORCH_CHECK(t.scalar_type() == input.scalar_type(), name, " must have the input's type");
+    TORCH_CHECK(t.sizes() == input.sizes(), name, " must have the input's shape");
+    return rows_of(t, name);
+  };
+  const Rows x = rows_of(input, "input");
+  a.x = input.data_ptr();
+  a.x_outer = x.outer;
+  a.x_inner = x.inner;
+  a.weight = weight.data_ptr();
+  if (residual) {
+    const Rows r = like_input(*residual, "residual"), ro = like_input(*residual_out, "residual_out");
+    a.residual = residual->data_ptr();
+    a.residual_outer = r.outer;
+    a.residual_inner = r.inner;
+    a.residual_out = residual_out->data_ptr();
+    a.residual_out_outer = ro.outer;
+    a.residual_out_inner = ro.inner;
+    check_rows_apart(*residual_out, "residual_out");
+    check_apart(*residual_out, "residual_out", *residual, "residual", true);
+    check_apart(*residual_out, "residual_out", input, "input", true);
+    check_apart(*residual_out, "residual_out", weight, "weight", false);
+  }
+  if (out) {
+    const Rows o = like_input(*out, "out");
+    a.out = out->data_ptr();
+    a.out_outer = o.outer;
+    a.out_inner = o.inner;
+    check_rows_apart(*out, "out");
+    check_apart(*out, "out", input, "input", true);
+    check_apart(*out, "out", weight, "weight", false);
+    if (residual) {
+      check_apart(*out, "out", *residual, "residual", true);
+      check_apart(*out, "out", *residual_out, "residual_out", false);
+    }
+  }
+  if (q) {
+    check_gpu(*q, "q");
+    check_here(*q, "q", input);
+    check_here(*scales, "scales", input);
+    TORCH_CHECK(q->scalar_type() == at::kFloat8_e4m3fn, "q must be float8_e4m3fn");
+    TORCH_CHECK(q->sizes() == input.sizes(), "q must have the input's shape");
+    TORCH_CHECK(group_size == 32 || group_size == 64 || group_size == 128,
+                "group_size must be 32, 64, or 128, got ", group_size);
+    TORCH_CHECK(cols % group_size == 0, "hidden_size must be divisible by group_size");
+    const auto sd = scales->scalar_type();
+    TORCH_CHECK(sd == at::kFloat || sd == at::kFloat8_e8m0fnu || sd == at::kByte,
+                "scales must be float32, float8_e8m0fnu or uint8 (e8m0 codes)");
+    TORCH_CHECK(scales->dim() == 2 && scales->size(0) == a.rows &&
+                    scales->size(1) == cols / group_size,
+                "scales must have logical shape [num_rows, num_groups]");
+    check_rows_apart(*scales, "scales");
+    a.q = q->data_ptr();
+    a.scales = scales->data_ptr();
+    a.scale_dtype = sd == at::kFloat ? MI355MOE_F32 : MI355MOE_U8;
+    a.scale_ue8m0 = scale_ue8m0;
+    a.group = group_size;
+    a.scale_row = scales->stride(0);
+    a.scale_group = scales->stride(1);
+    for (const auto* t : {&*q, &*scales}) {
+      const char* n = t == &*q ? "q" : "scales";
+      check_apart(*t, n, input, "input", false);
+      check_apart(*t, n, weight, "weight", false);
+      if (residual) check_apart(*t, n, *residual, "residual", false);
+      if (residual) check_apart(*t, n, *residual_out, "residual_out", false);
+      if (out) check_apart(*t, n, *out, "out", false);
+    }
+    check_apart(*q, "q", *scales, "scales", false);
+  }
+  if (a.rows == 0) return;
+  DevGuard g(input.device());
+  check_rc(mi355moe_rms_norm(&a, cur_stream(input)), "rms_norm");
+}
+
+// [.., cols] as [rows, cols] with one row stride
+int64_t row_stride(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
+  int64_t ld = t.size(-1);
+  bool set = false;
+  int64_t want = 0;
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) <= 1) continue;
+    if (!set) ld = t.stride(i);
+    else
+      TORCH_CHECK(t.stride(i) == want, name, " has leading dimensions that do not fold into one");
+    TORCH_CHECK(t.stride(i) >= 0, name, " has a negative stride");
+    want = t.stride(i) * t.size(i);
+    set = true;
+  }
+  return ld;
+}
+
+void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
+            const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
+            const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual,
+            int64_t activation) {
+  TORCH_CHECK(input.is_cuda(), "input must be on a GPU device");
+  TORCH_CHECK(input.dim() >= 1, "input must have at least one dimension");
+  const bool fp8 = input.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(fp8 || input.scalar_type() == at::kBFloat16 || input.scalar_type() == at::kHalf,
+              "input must be bfloat16, float16 or float8_e4m3fn");
+  check_here(weight, "weight", input);
+  TORCH_CHECK(weight.scalar_type() == input.scalar_type(), "weight must have the input's type");
+  TORCH_CHECK(weight.dim() == 2, "weight must be 2-dimensional");
+  TORCH_CHECK(weight.size(1) == input.size(-1), "weight must be [out_features, in_features] with "
+              "the input's last dimension as in_features");
+  TORCH_CHECK(activation >= MI355MOE_LINEAR_NONE && activation <= MI355MOE_LINEAR_GELU_TANH_AND_MUL,
+              "unknown activation");
+  const bool gated = activation >= MI355MOE_LINEAR_SILU_AND_MUL;
+  const int64_t K = weight.size(1), rows = weight.size(0);
+  TORCH_CHECK(K > 0 && rows > 0, "in_features and out_features must be positive");
+  TORCH_CHECK(!gated || rows % 2 == 0, "a gated activation needs an even number of weight rows");
+  mi355moe_linear_args a{};
+  a.N = gated ? rows / 2 : rows;
+  a.K = K;
+  a.M = input.numel() / K;
+  a.activation = static_cast<int>(activation);
+  a.x_dtype = dtype_code(input.scalar_type());
+  a.x = input.data_ptr();
+  a.ldx = row_stride(input, "input");
+  a.weight = weight.data_ptr();
+  a.ldw = row_stride(weight, "weight");
+  TORCH_CHECK(fp8 == input_scale.has_value() && fp8 == weight_scale.has_value(),
+              "scales belong to float8_e4m3fn operands");
+  if (fp8) {
+    TORCH_CHECK(K % 128 == 0, "in_features must be divisible by 128");
+    check_here(*input_scale, "input_scale", input);
+    check_here(*weight_scale, "weight_scale", input);
+    TORCH_CHECK(input_scale->scalar_type() == at::kFloat && weight_scale->scalar_type() == at::kFloat,
+                "scales must be float32");
+    TORCH_CHECK(input_scale->dim() == 2 && input_scale->size(0) == a.M &&
+                    input_scale->size(1) == K / 128,
+                "input_scale must be [num_rows, in_features / 128]");
+    TORCH_CHECK(weight_scale->dim() == 2 && weight_scale->size(0) == (rows + 127) / 128 &&
+                    weight_scale->size(1) == K / 128,
+                "weight_scale must be [ceil(out_features / 128), in_features / 128]");
+    a.x_scale = input_scale->data_ptr<float>();
+    a.x_scale_row = input_scale->stride(0);
+    a.x_scale_blk = input_scale->stride(1);
+    a.weight_scale = weight_scale->data_ptr<float>();
+    a.weight_scale_row = weight_scale->stride(0);
+    a.weight_scale_blk = weight_scale->stride(1);
+  }
+  auto out_shape = [&](const at::Tensor& t, const char* name) {
+    check_here(t, name, input);
+    TORCH_CHECK(float16or32(t), name, " must be float32, bfloat16 or float16");
+    TORCH_CHECK(t.dim() == input.dim() && t.size(-1) == a.N &&
+                    t.sizes().slice(0, t.dim() - 1) == input.sizes().slice(0, input.dim() - 1),
+                name, " must have the input's shape with out_features columns");
+    return row_stride(t, name);
+  };
+  a.ldo = out_shape(out, "out");
+  a.out = out.data_ptr();
+  a.out_dtype = dtype_code(out.scalar_type());
+  check_rows_apart(out, "out");
+  check_apart(out, "out", input, "input", false);
+  check_apart(out, "out", weight, "weight", false);
+  if (fp8) {
+    check_apart(out, "out", *input_scale, "input_scale", false);
+    check_apart(out, "out", *weight_scale, "weight_scale", false);
+  }
+  if (bias) {
+    check_here(*bias, "bias", input);
+    TORCH_CHECK(float16or32(*bias), "bias must be float32, bfloat16 or float16");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == rows && bias->is_contiguous(),
+                "bias must be contiguous [out_features]");
+    check_apart(out, "out", *bias, "bias", false);
+    a.bias = bias->data_ptr();
+    a.bias_dtype = dtype_code(bias->scalar_type());
+  }
+  if (residual) {
+    a.ldr = out_shape(*residual, "residual");
+    a.residual = residual->data_ptr();
+    a.residual_dtype = dtype_code(residual->scalar_type());
+    check_apart(out, "out", *residual, "residual", true);
+  }
+  if (a.M == 0) return;
+  DevGuard g(input.device());
+  const size_t need = mi355moe_linear_workspace_size(&a);
+  at::Tensor ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, input.options().dtype(at::kByte));
+  check_rc(mi355moe_linear(&a, need ? ws.data_ptr() : nullptr, need, cur_stream(input)), "linear");
+}
+
 // ------------------------------------------------------------- grouped GEMM
 at::Tensor grouped_gemm_meta(at::Tensor&, const std::optional<at::Tensor>&, at::Tensor&,
                              const std::optional<at::Tensor>&,
@@ -1128,4 +1420,24 @@ TORCH_LIBRARY_IMPL(_xpu_C, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(_xpu_C, Meta, m) {
   m.impl("cutlass_grouped_gemm_interface", &grouped_gemm_meta);
+}
+
+// Operators beside the experts: no counterpart in the reference's namespaces,
+// so they have one of their own.
+TORCH_LIBRARY(_mi355_C, m) {
+  m.def("rms_norm(Tensor(a!)? out, Tensor(b!)? q, Tensor(c!)? scales, Tensor(d!)? residual_out, "
+        "Tensor input, Tensor weight, Tensor? residual, float epsilon, int group_size=128, "
+        "bool scale_ue8m0=False) -> ()");
+  m.def("linear(Tensor! out, Tensor input, Tensor? input_scale, Tensor weight, "
+        "Tensor? weight_scale, Tensor? bias, Tensor? residual, int activation) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(_mi355_C, CUDA, m) {
+  m.impl("rms_norm", &rms_norm);
+  m.impl("linear", &linear);
+}
+
+TORCH_LIBRARY_IMPL(_mi355_C, Meta, m) {
+  for (const char* op : {"rms_norm", "linear"})
+    m.impl(op, torch::CppFunction::makeFromBoxedFunction<&meta_noop>());
 }

@@ -131,6 +131,43 @@ def fused_args(moe, output, hidden_states, topk_weights, topk_ids,
     return a
 
 
+class RmsNormArgs(ctypes.Structure):
+    """mi355moe_rms_norm_args."""
+    _fields_ = [("dtype", ctypes.c_int), ("weight_dtype", ctypes.c_int),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("inner", ctypes.c_int64),
+                ("x", ctypes.c_void_p), ("x_outer", ctypes.c_int64), ("x_inner", ctypes.c_int64),
+                ("residual", ctypes.c_void_p), ("residual_outer", ctypes.c_int64),
+                ("residual_inner", ctypes.c_int64), ("residual_out", ctypes.c_void_p),
+                ("residual_out_outer", ctypes.c_int64), ("residual_out_inner", ctypes.c_int64),
+                ("weight", ctypes.c_void_p), ("eps", ctypes.c_float), ("out", ctypes.c_void_p),
+                ("out_outer", ctypes.c_int64), ("out_inner", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("scale_dtype", ctypes.c_int), ("scale_ue8m0", ctypes.c_int),
+                ("group", ctypes.c_int64), ("scale_row", ctypes.c_int64),
+                ("scale_group", ctypes.c_int64)]
+
+
+class LinearArgs(ctypes.Structure):
+    """mi355moe_linear_args."""
+    _fields_ = [("x_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int),
+                ("bias_dtype", ctypes.c_int), ("residual_dtype", ctypes.c_int),
+                ("activation", ctypes.c_int), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("K", ctypes.c_int64), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+                ("x_scale", ctypes.c_void_p), ("x_scale_row", ctypes.c_int64),
+                ("x_scale_blk", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("ldw", ctypes.c_int64), ("weight_scale", ctypes.c_void_p),
+                ("weight_scale_row", ctypes.c_int64), ("weight_scale_blk", ctypes.c_int64),
+                ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("ldr", ctypes.c_int64), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64)]
+
+
+lib.mi355moe_rms_norm.argtypes = [ctypes.POINTER(RmsNormArgs), ctypes.c_void_p]
+lib.mi355moe_linear.argtypes = [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_size_t,
+                                ctypes.c_void_p]
+lib.mi355moe_linear_workspace_size.restype = ctypes.c_size_t
+lib.mi355moe_linear_workspace_size.argtypes = [ctypes.POINTER(LinearArgs)]
+
+
 class StageTimer:
     """HIP-event timer of the five fused stages over `steps` calls."""
 

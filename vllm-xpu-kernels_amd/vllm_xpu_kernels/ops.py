@@ -264,6 +264,135 @@ def silu_and_mul_mxfp4_quant(input: torch.Tensor, group_size: int = 32,
     return out, scales
 
 
+def _no_grad_needed(*tensors) -> None:
+    """The operators below have no backward pass: refuse to lose a gradient."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("this operator has no gradient: call it under torch.no_grad() or "
+                           "detach its inputs")
+
+
+_rms_norm = torch.ops._mi355_C.rms_norm.default
+_linear = torch.ops._mi355_C.linear.default
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+             residual: Optional[torch.Tensor] = None,
+             residual_out: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None):
+    """Root-mean-square norm over the last dimension, after the residual's
+    addition:  h = x + residual,  out = h / sqrt(mean(h^2) + eps) * weight,
+    in fp32 with one rounding per output.
+
+    x [.., H] float32, bfloat16 or float16, columns contiguous, rows of any
+    stride (heads inside a packed projection are normed where they lie);
+    weight [H] of x's type or float32.  Returns out, with a residual
+    (out, h).  h is written to residual_out, which may be residual itself
+    (in place); out may be x."""
+    _no_grad_needed(x, weight, residual)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError("residual_out needs a residual")
+        _rms_norm(out, None, None, None, x, weight, None, eps)
+        return out
+    if residual_out is None:
+        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _rms_norm(out, None, None, residual_out, x, weight, residual, eps)
+    return out, residual_out
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                   residual: Optional[torch.Tensor] = None,
+                   residual_out: Optional[torch.Tensor] = None, group_size: int = 128,
+                   scale_dtype: torch.dtype = torch.float32, scale_ue8m0: bool = False,
+                   is_scale_transposed: bool = False, with_norm: bool = False):
+    """rms_norm with its result in float8_e4m3fn and a scale per group_size
+    (32, 64, 128) columns, quantised from the fp32 result: the pre-quantised
+    input of XpuFusedMoe.apply (a1q_scale) and of linear_fp8.
+
+    scale_dtype float32 (rounded up to powers of two with scale_ue8m0) or
+    float8_e8m0fnu (power-of-two codes; mxfp8 with group_size 32).  Returns
+    (q, scales [rows, H / group_size]), then the norm in x's type
+    (with_norm: the router's input), then the new residual (with a residual).
+    The scales are a transposed view when is_scale_transposed."""
+    _no_grad_needed(x, weight, residual)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    H = x.shape[-1]
+    rows, groups = x.numel() // max(H, 1), H // group_size
+    if is_scale_transposed:
+        scales = torch.empty((groups, rows), dtype=scale_dtype, device=x.device).t()
+    else:
+        scales = torch.empty((rows, groups), dtype=scale_dtype, device=x.device)
+    norm = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_norm else None
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError("residual_out needs a residual")
+    elif residual_out is None:
+        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _rms_norm(norm, q, scales, residual_out, x, weight, residual, eps, group_size, scale_ue8m0)
+    got = (q, scales)
+    if with_norm:
+        got += (norm,)
+    return got if residual is None else got + (residual_out,)
+
+
+_LINEAR_ACT = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu2": 4, "silu_and_mul": 5,
+               "gelu_and_mul": 6, "gelu_tanh_and_mul": 7}
+
+
+def _linear_out(x, rows, activation, out_dtype, out):
+    """(activation code, output tensor) of a product with `rows` weight rows."""
+    code = _LINEAR_ACT.get(activation)
+    if code is None:
+        raise ValueError(f"Unsupported activation: {activation}.")
+    if out is None:
+        out = torch.empty(x.shape[:-1] + (rows // 2 if code >= 5 else rows,), dtype=out_dtype,
+                          device=x.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out must have out_dtype")
+    return code, out
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+           out_dtype: Optional[torch.dtype] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x @ weight.T + bias) + residual in one call: fp32 accumulation and
+    epilogue, one rounding to out_dtype (x's type by default, float32 for
+    router logits).
+
+    x [.., K] and weight [N, K] bfloat16 or float16; bias [N] and residual
+    [.., N] float32, bfloat16 or float16.  activation: None, "silu", "gelu",
+    "gelu_tanh", "relu2", or a gated one, "silu_and_mul", "gelu_and_mul",
+    "gelu_tanh_and_mul": f of the first half of the weight rows' results
+    times the second half's, N / 2 columns.  out may be residual (in place)."""
+    _no_grad_needed(x, weight, bias, residual)
+    if out is None and out_dtype is None:
+        out_dtype = x.dtype
+    code, out = _linear_out(x, weight.shape[0], activation, out_dtype, out)
+    _linear(out, x, None, weight, None, bias, residual, code)
+    return out
+
+
+def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
+               weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear on float8_e4m3fn operands with float32 scales: x [.., K] with
+    x_scale [rows, K / 128] (rms_norm_quant, per_token_group_fp8_quant; any
+    strides), weight [N, K] with weight_scale [ceil(N / 128), K / 128] (the
+    layer's block-scaled recipe).  K % 128 == 0.  out_dtype: bfloat16 by
+    default, float16 or float32."""
+    _no_grad_needed(x_scale, weight_scale, bias, residual)
+    if out is None and out_dtype is None:
+        out_dtype = torch.bfloat16
+    code, out = _linear_out(x, weight.shape[0], activation, out_dtype, out)
+    _linear(out, x, x_scale, weight, weight_scale, bias, residual, code)
+    return out
+
+
 def init_expert_map(num_experts: int, ep_rank: int, ep_size: int,
                     device) -> torch.Tensor:
     m = torch.empty(num_experts * ep_size, dtype=torch.int32, device=device)

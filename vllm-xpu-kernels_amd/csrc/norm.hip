@@ -5,8 +5,11 @@
 // and per group of columns of y the scale and codes of the group quantisers
 // (per_token_group_fp8_quant's arithmetic; e8m0 scales as the mxfp8 layer's).
 //
-// One workgroup per row: a pass that sums the squares, a workgroup sum, and a
-// pass that reads the row again (from L2) and writes the outputs.
+// Bound by HBM (each input read once, each output written once) from a few
+// hundred rows on, by latency below.  A row stays in registers between the sum
+// of its squares and the outputs: R chunks of 8 columns per lane, the row's
+// lanes in one wave (rows up to 512 columns, several rows per wave) or in one
+// workgroup.  Rows beyond the registers of 1024 lanes are read twice.
 #include "common.h"
 
 namespace mi355 {
@@ -14,10 +17,11 @@ namespace {
 
 typedef mi355moe_rms_norm_args NormArgs;
 
-// Elements i .. i + 7 of a row (i a multiple of 8): two or one 16-byte loads
-// when VEC, else the elements below `cols` one by one and zeros.
+// Elements i, i + step, .. i + 7 step of a row: two or one 16-byte loads when VEC
+// (step 1, i a multiple of 8), else those below `cols` one by one and zeros.
 template <typename E, bool VEC>
-__device__ __forceinline__ void load8(const void* p, int64_t i, int64_t cols, float (&f)[8]) {
+__device__ __forceinline__ void load8(const void* p, int64_t i, int64_t cols, float (&f)[8],
+                                      int step = 1) {
   const typename E::T* q = static_cast<const typename E::T*>(p) + i;
   if constexpr (VEC && sizeof(typename E::T) == 2) {
     const uint4 u = *reinterpret_cast<const uint4*>(q);
@@ -34,11 +38,21 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, int64_t cols, fl
     for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(w[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = i + k < cols ? E::ld(q[k]) : 0.f;
+    for (int k = 0; k < 8; ++k) f[k] = i + k * step < cols ? E::ld(q[k * step]) : 0.f;
   }
 }
+// 16 bytes; `nt`: past the caches (launch_rows has the rule)
+typedef uint32_t norm_u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t norm_u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void put16(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d,
+                                      bool nt) {
+  const norm_u32x4 v = {a, b, c, d};
+  if (nt) __builtin_nontemporal_store(v, static_cast<norm_u32x4*>(p));
+  else *static_cast<norm_u32x4*>(p) = v;
+}
 template <typename E, bool VEC>
-__device__ __forceinline__ void store8(void* p, int64_t i, int64_t cols, const float (&f)[8]) {
+__device__ __forceinline__ void store8(void* p, int64_t i, int64_t cols, const float (&f)[8],
+                                       bool nt, int step = 1) {
   typename E::T* q = static_cast<typename E::T*>(p) + i;
   if constexpr (VEC && sizeof(typename E::T) == 2) {
     uint32_t w[4];
@@ -46,17 +60,17 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int64_t cols, const f
     for (int k = 0; k < 4; ++k)
       w[k] = static_cast<uint32_t>(E::st(f[2 * k])) |
              (static_cast<uint32_t>(E::st(f[2 * k + 1])) << 16);
-    *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+    put16(q, w[0], w[1], w[2], w[3], nt);
   } else if constexpr (VEC) {
     uint32_t w[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(f[k]);
-    reinterpret_cast<uint4*>(q)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4*>(q)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    put16(q, w[0], w[1], w[2], w[3], nt);
+    put16(q + 4, w[4], w[5], w[6], w[7], nt);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (i + k < cols) q[k] = E::st(f[k]);
+      if (i + k * step < cols) q[k * step] = E::st(f[k]);
   }
 }
 
@@ -79,16 +93,24 @@ __device__ __forceinline__ uint32_t e4m3x4_nan(float v0, float v1, float v2, flo
   return static_cast<uint32_t>(w);
 }
 
-// The group's scale and the lane's 8 codes.  A group is G / 8 consecutive,
-// aligned lanes, all of them active (cols % G == 0).
+// The group's scale and the lane's 8 codes of columns i .. i + 7.  A group is
+// G / 8 consecutive, aligned lanes; every lane of the wave takes part, those
+// without columns (`active` false) with zeros.
 template <bool VEC>
-__device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int64_t i,
-                                       const float (&y)[8]) {
+__device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int i, bool active,
+                                       const float (&y)[8], bool nt) {
   float amax = 1e-10f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(y[k]));
-  const int lanes = static_cast<int>(a.group >> 3);
-  for (int o = 1; o < lanes; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+  const int group = static_cast<int>(a.group);
+  if (group == 128) {
+    amax = row16_max(amax);
+  } else {
+    amax = fmaxf(amax, __shfl_xor(amax, 1, 64));
+    amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
+    if (group == 64) amax = fmaxf(amax, __shfl_xor(amax, 4, 64));
+  }
+  if (!active) return;
   float s = fmaxf(amax / 448.0f, 1.0f / (448.0f * 512.0f));
   const bool e8m0 = a.scale_dtype == MI355MOE_U8;
   int ex = 0;
@@ -96,9 +118,8 @@ __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int64_t i,
     ex = ceil_log2(s);
     s = ex > 127 ? __uint_as_float(0x7F800000u) : pow2i(ex);  // an infinite maximum
   }
-  const int64_t g = i / a.group;
-  if (i % a.group == 0) {
-    const int64_t at = r * a.scale_row + g * a.scale_group;
+  if ((i & (group - 1)) == 0) {
+    const int64_t at = r * a.scale_row + (i / group) * a.scale_group;
     if (e8m0) static_cast<uint8_t*>(a.scales)[at] = static_cast<uint8_t>(ex + 127);
     else static_cast<float*>(a.scales)[at] = s;
   }
@@ -107,16 +128,106 @@ __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int64_t i,
   const uint32_t hi = e4m3x4_nan(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
   uint8_t* q = static_cast<uint8_t*>(a.q) + r * a.cols + i;
   if constexpr (VEC) {
-    *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
+    const norm_u32x2 v = {lo, hi};
+    if (nt) __builtin_nontemporal_store(v, reinterpret_cast<norm_u32x2*>(q));
+    else *reinterpret_cast<norm_u32x2*>(q) = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) q[k] = static_cast<uint8_t>((k < 4 ? lo : hi) >> (8 * (k & 3)));
   }
 }
 
+// LANES: lanes of a row inside a wave (8 to 64, 256 / LANES rows to a
+// workgroup of 256), or 0: the workgroup's blockDim.x lanes are one row's.
+template <typename E, bool VEC, int LANES, int R, bool QUANT>
+__global__ __launch_bounds__(LANES ? 256 : 1024) void rms_norm_kernel(const NormArgs a, int64_t row0, bool nt) {
+  const int lanes = LANES ? LANES : static_cast<int>(blockDim.x);
+  const int t = LANES ? threadIdx.x % LANES : threadIdx.x;
+  const int64_t r = row0 + (LANES ? static_cast<int64_t>(blockIdx.x) * (256 / LANES) +
+                                       threadIdx.x / LANES
+                                 : static_cast<int64_t>(blockIdx.x));
+  const int cols = static_cast<int>(a.cols);
+  const bool row = r < a.rows;
+  const int64_t rr = row ? r : 0;
+  const char* x = static_cast<const char*>(a.x) + row_at<E>(rr, a.inner, a.x_outer, a.x_inner);
+  const char* res = a.residual ? static_cast<const char*>(a.residual) +
+                                     row_at<E>(rr, a.inner, a.residual_outer, a.residual_inner)
+                               : nullptr;
+  // Chunk c of this lane: 8 consecutive columns; where rows start anywhere and
+  // no group binds columns to lanes, 8 columns `lanes` apart, so that a wave's
+  // accesses are runs of 64 columns (8192 x 7167 bf16 314 -> 268 us).
+  const int step = VEC || QUANT ? 1 : lanes;
+  const auto at = [&](int c) { return step == 1 ? (c * lanes + t) * 8 : c * lanes * 8 + t; };
+  float h[R][8], w[R][8];
+  bool on[R];
+#pragma unroll
+  for (int c = 0; c < R; ++c) {
+    const int i = at(c);
+    on[c] = row && i < cols;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) h[c][k] = 0.f;
+    if (on[c]) load8<E, VEC>(x, i, cols, h[c], step);
+  }
+  if (res) {
+#pragma unroll
+    for (int c = 0; c < R; ++c) {
+      float u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (on[c]) load8<E, VEC>(res, at(c), cols, u, step);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) h[c][k] += u[k];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < R; ++c) {
+    const int i = at(c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[c][k] = 0.f;
+    if (on[c]) {
+      if (a.weight_dtype == MI355MOE_F32) load8<F32, VEC>(a.weight, i, cols, w[c], step);
+      else load8<E, VEC>(a.weight, i, cols, w[c], step);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < R; ++c)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss += h[c][k] * h[c][k];
+  if constexpr (LANES != 0) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+  } else {
+    __shared__ float part[16];
+    ss = wave_sum(ss);
+    if ((t & 63) == 0) part[t >> 6] = ss;
+    __syncthreads();
+    const int waves = lanes >> 6;
+    ss = 0.f;
+    for (int v = 0; v < waves; ++v) ss += part[v];
+  }
+  const float rs = 1.0f / sqrtf(ss / static_cast<float>(cols) + a.eps);
+  char* res_out = a.residual_out ? static_cast<char*>(a.residual_out) +
+                                       row_at<E>(rr, a.inner, a.residual_out_outer,
+                                                 a.residual_out_inner)
+                                 : nullptr;
+  char* out = a.out ? static_cast<char*>(a.out) + row_at<E>(rr, a.inner, a.out_outer, a.out_inner)
+                    : nullptr;
+#pragma unroll
+  for (int c = 0; c < R; ++c) {
+    const int i = at(c);
+    if (res_out && on[c]) store8<E, VEC>(res_out, i, cols, h[c], nt, step);
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = h[c][k] * rs * w[c][k];
+    if (out && on[c]) store8<E, VEC>(out, i, cols, y, nt, step);
+    if constexpr (QUANT) quant8<VEC>(a, rr, i, on[c], y, nt);
+  }
+}
+
+// Rows of any length: the row is read again for the outputs (by the same
+// lanes, so an output may be the input).
 template <typename E, bool VEC>
-__global__ __launch_bounds__(256) void rms_norm_kernel(const NormArgs a) {
-  const int64_t r = blockIdx.x;
+__global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a, int64_t row0, bool nt) {
+  const int64_t r = row0 + blockIdx.x;
   const char* x = static_cast<const char*>(a.x) + row_at<E>(r, a.inner, a.x_outer, a.x_inner);
   const char* res = a.residual ? static_cast<const char*>(a.residual) +
                                      row_at<E>(r, a.inner, a.residual_outer, a.residual_inner)
@@ -131,34 +242,80 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(const NormArgs a) {
     }
   };
   float ss = 0.f;
-  for (int64_t i = threadIdx.x * 8; i < a.cols; i += 256 * 8) {
+  for (int64_t i = threadIdx.x * 8; i < a.cols; i += 1024 * 8) {
     float h[8];
     load_h(i, h);
 #pragma unroll
     for (int k = 0; k < 8; ++k) ss += h[k] * h[k];
   }
-  __shared__ float part[4];
+  __shared__ float part[16];
   ss = wave_sum(ss);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
   __syncthreads();
-  ss = (part[0] + part[1]) + (part[2] + part[3]);
+  ss = 0.f;
+  for (int v = 0; v < 16; ++v) ss += part[v];
   const float rs = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
-  for (int64_t i = threadIdx.x * 8; i < a.cols; i += 256 * 8) {
-    float h[8], w[8], y[8];
-    load_h(i, h);
-    if (a.residual_out)
+  for (int64_t i0 = 0; i0 < a.cols; i0 += 1024 * 8) {  // uniform: groups exchange maxima
+    const int64_t i = i0 + threadIdx.x * 8;
+    const bool on = i < a.cols;
+    float h[8] = {}, w[8] = {}, y[8];
+    if (on) load_h(i, h);
+    if (on && a.residual_out)
       store8<E, VEC>(static_cast<char*>(a.residual_out) +
                          row_at<E>(r, a.inner, a.residual_out_outer, a.residual_out_inner),
-                     i, a.cols, h);
-    if (a.weight_dtype == MI355MOE_F32) load8<F32, VEC>(a.weight, i, a.cols, w);
-    else load8<E, VEC>(a.weight, i, a.cols, w);
+                     i, a.cols, h, nt);
+    if (on) {
+      if (a.weight_dtype == MI355MOE_F32) load8<F32, VEC>(a.weight, i, a.cols, w);
+      else load8<E, VEC>(a.weight, i, a.cols, w);
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = h[k] * rs * w[k];
-    if (a.out)
+    if (on && a.out)
       store8<E, VEC>(static_cast<char*>(a.out) + row_at<E>(r, a.inner, a.out_outer, a.out_inner),
-                     i, a.cols, y);
-    if (a.q) quant8<VEC>(a, r, i, y);
+                     i, a.cols, y, nt);
+    if (a.q) quant8<VEC>(a, r, static_cast<int>(on ? i : 0), on, y, nt);
   }
+}
+
+template <typename E, bool VEC, int LANES, int R>
+void launch_one(const NormArgs& a, int64_t row0, int64_t rows, int threads, bool nt,
+                hipStream_t st) {
+  const int64_t per = LANES ? 256 / (LANES ? LANES : 1) : 1;
+  const dim3 grid(static_cast<unsigned>(cdiv(rows, per)));
+  if (a.q) rms_norm_kernel<E, VEC, LANES, R, true><<<grid, dim3(threads), 0, st>>>(a, row0, nt);
+  else rms_norm_kernel<E, VEC, LANES, R, false><<<grid, dim3(threads), 0, st>>>(a, row0, nt);
+}
+
+template <typename E, bool VEC>
+int launch_rows(const NormArgs& a, int64_t row0, int64_t rows, hipStream_t st) {
+  const int64_t chunks = cdiv(a.cols, 8);
+  // Outputs larger than the L2s of the 8 XCDs (32 MiB) cannot stay there for
+  // their reader; stored past them they leave room for the rows still read
+  // (8192 x 7168 with e4m3 107 -> 99 us, 2048 x 7168 34 -> 24).
+  const int64_t size = sizeof(typename E::T);
+  const bool nt = a.rows * a.cols *
+                      ((a.out ? size : 0) + (a.residual ? size : 0) + (a.q ? 1 : 0)) >
+                  (int64_t(32) << 20);
+  if (chunks <= 8) launch_one<E, VEC, 8, 1>(a, row0, rows, 256, nt, st);
+  else if (chunks <= 16) launch_one<E, VEC, 16, 1>(a, row0, rows, 256, nt, st);
+  else if (chunks <= 32) launch_one<E, VEC, 32, 1>(a, row0, rows, 256, nt, st);
+  else if (chunks <= 64) launch_one<E, VEC, 64, 1>(a, row0, rows, 256, nt, st);
+  else {
+    // One chunk per lane is the fastest wherever its many waves are few rounds
+    // of the GPU or one workgroup's barrier is short (bf16 with a residual, 1 / 2 / 4
+    // chunks: 1 x 7168 3.3 / 3.8 / 5.2 us, 512 x 7168 8.4 / 8.7 / 11.0, 8192 x
+    // 4096 46.2 / 49.3 / 54.0); wide rows in numbers want two (1024 x 7168 15.3 /
+    // 12.1 / 13.0, 8192 x 7168 96.1 / 91.4 / 104.9).
+    const int r = chunks <= 512 || (chunks <= 1024 && a.rows < 768) ? 1 : chunks <= 2048 ? 2 : 4;
+    const int threads = static_cast<int>(cdiv(cdiv(chunks, r), 64) * 64);
+    if (threads > 1024)
+      rms_norm_long_kernel<E, VEC><<<dim3(static_cast<unsigned>(rows)), dim3(1024), 0, st>>>(a, row0, nt);
+    else if (r == 1) launch_one<E, VEC, 0, 1>(a, row0, rows, threads, nt, st);
+    else if (r == 2) launch_one<E, VEC, 0, 2>(a, row0, rows, threads, nt, st);
+    else launch_one<E, VEC, 0, 4>(a, row0, rows, threads, nt, st);
+  }
+  MI_LAUNCH_CHECK();
+  return MI355MOE_OK;
 }
 
 bool mul16(const void* p, int64_t outer, int64_t inner, int64_t n_inner, int size) {
@@ -176,10 +333,14 @@ int launch(const NormArgs& a, hipStream_t st) {
         mul16(a.residual_out, a.residual_out_outer, a.residual_out_inner, a.inner, size))) &&
       (!a.out || mul16(a.out, a.out_outer, a.out_inner, a.inner, size)) &&
       mul16(a.weight, 0, 0, 1, 2) && (!a.q || (reinterpret_cast<uintptr_t>(a.q) & 7) == 0);
-  const dim3 grid(static_cast<unsigned>(a.rows));
-  if (vec) rms_norm_kernel<E, true><<<grid, dim3(256), 0, st>>>(a);
-  else rms_norm_kernel<E, false><<<grid, dim3(256), 0, st>>>(a);
-  MI_LAUNCH_CHECK();
+  // a launch's threads stay below 2^32
+  constexpr int64_t kRows = int64_t(1) << 21;
+  for (int64_t row0 = 0; row0 < a.rows; row0 += kRows) {
+    const int64_t rows = a.rows - row0 < kRows ? a.rows - row0 : kRows;
+    const int rc = vec ? launch_rows<E, true>(a, row0, rows, st)
+                       : launch_rows<E, false>(a, row0, rows, st);
+    if (rc) return rc;
+  }
   return MI355MOE_OK;
 }
 
@@ -196,7 +357,7 @@ extern "C" int mi355moe_rms_norm(const mi355moe_rms_norm_args* p, void* stream) 
   MI_ARG(a.weight_dtype == a.dtype || a.weight_dtype == MI355MOE_F32,
          "rms_norm: weight must have the input's type or be float32");
   MI_ARG(a.rows >= 0 && a.cols > 0 && a.inner > 0, "rms_norm: invalid shape");
-  MI_ARG(a.rows <= 0x7FFFFFFF, "rms_norm: too many rows");
+  MI_ARG(a.cols <= (1 << 28), "rms_norm: size too large");
   MI_ARG((a.residual != nullptr) == (a.residual_out != nullptr) || a.rows == 0,
          "rms_norm: residual and residual_out go together");
   MI_ARG(a.out || a.q || a.rows == 0, "rms_norm: no output");

@@ -167,15 +167,21 @@ int check(const LinArgs& a) {
 
 using namespace mi355;
 
+namespace {
+enum Path { SKINNY, TILE, ANY };
+Path path_of(const LinArgs& a) {
+  if (linear_skinny_takes(a)) return SKINNY;
+  return linear_tile_supported(a) ? TILE : ANY;
+}
+}  // namespace
+
 extern "C" size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* p) {
-  (void)p;
-  return 0;
+  if (!p || check(*p) || p->M == 0) return 0;
+  return path_of(*p) == TILE ? linear_tile_workspace(*p) : 0;
 }
 
 extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
                                size_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   MI_ARG(p, "null pointer");
   const LinArgs a = *p;
   if (const int rc = check(a)) return rc;
@@ -184,6 +190,16 @@ extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
   MI_ARG(a.x && a.weight && a.out, "null pointer");
   MI_ARG(!fp8 || (a.x_scale && a.weight_scale), "linear: scales missing");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (path_of(a)) {
+    case SKINNY: return launch_linear_skinny(a, st);
+    case TILE: {
+      const size_t need = linear_tile_workspace(a);
+      MI_CHECK(need == 0 || (workspace && workspace_bytes >= need), MI355MOE_ERR_WORKSPACE,
+               "linear: workspace too small");
+      return launch_linear_tile(a, workspace, st);
+    }
+    default: break;
+  }
   const int eb = fp8 ? 1 : 2;
   auto rows16 = [&](const void* p_, int64_t ld) {
     return ((reinterpret_cast<uintptr_t>(p_) | static_cast<uintptr_t>(ld * eb)) & 15) == 0;

@@ -387,6 +387,9 @@ def test_opcheck(dev):
     op = torch.ops._mi355_C.linear.default
     torch.library.opcheck(op, (torch.empty(5, 16, dtype=x.dtype, device=dev), x, None, w, None, None, None, 0))
     torch.library.opcheck(op, (torch.empty(5, 8, dtype=x.dtype, device=dev), x, None, w, None, b, r, 5))
+    op = torch.ops._mi355_C.linear_new.default
+    torch.library.opcheck(op, (x, None, w, None, None, None, 0, torch.float32))
+    torch.library.opcheck(op, (x.view(1, 5, 256), None, w, None, b, r.view(1, 5, 8), 5, torch.bfloat16))
 
 
 # ------------------------------------------------- a decoder block's MoE part

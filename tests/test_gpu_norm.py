@@ -127,6 +127,13 @@ def test_rms_norm_quant(dev, T, H, dtype, res, group, kind):
     assert torch.equal(got2[0].view(torch.uint8), q.view(torch.uint8))
     assert got2[1].stride(0) == 1 or T == 1
     assert torch.equal(got2[1].double(), s.double())
+    if res:   # the residual updated in place
+        r2 = r.clone()
+        got3 = _ops().rms_norm_quant(x, w, EPS, residual=r2, residual_out=r2, group_size=group,
+                                     scale_dtype=sdt, scale_ue8m0=kind == "ue8m0", with_norm=True)
+        for a, b in zip(got3, got):
+            assert torch.equal(a.double(), b.double())
+        assert got3[3] is r2
 
 
 @pytest.mark.parametrize("T,heads,H,dtype", [(1003, 32, 128, "fp16"), (3, 5, 64, "bf16"),
@@ -274,6 +281,12 @@ def test_opcheck(dev):
     s = torch.zeros(5, 2, device=dev)
     torch.library.opcheck(op, (None, q, s, None, x, w, None, EPS, 128, True),
                           test_utils=("test_autograd_registration", "test_faketensor"))
+    op = torch.ops._mi355_C.rms_norm_new.default
+    torch.library.opcheck(op, (x, w, None, EPS))
+    torch.library.opcheck(op, (x, w, x.clone(), EPS))
+    for more in ((True, 128, None, True, False), (False, 32, torch.float8_e8m0fnu, False, True)):
+        torch.library.opcheck(op, (x, w, x.clone(), EPS) + more,
+                              test_utils=("test_autograd_registration", "test_faketensor"))
 
 
 def test_traced_by_the_compiler_front_end(dev):

@@ -80,7 +80,8 @@ __device__ __forceinline__ void for_each(F&& f) {
 
 enum { K_BF16 = 0, K_F16 = 1, K_FP8 = 2, K_FP8_EXACT = 3 };
 
-template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int SB, int NSTAGE, int D>
+template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int SB, int NSTAGE,
+          int D>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs a, int tiles_m,
                                                                     int tiles_n, int splits,
                                                                     int stages_per_split) {
@@ -376,17 +377,17 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
           if constexpr (UNI) ws[i] = sw[wrow(i)];
           else ws[i] = *reinterpret_cast<const f32x4*>(sw + wrow(i) + 4 * q);
         }
-        // the results of x tile j - 1 are scaled and added while tile j's MFMAs run
-        f32x4 d[2][NT];
-        auto add = [&](int i, int j) __attribute__((always_inline)) {
-          const f32x4 v = d[j & 1][i];
+        // a result is scaled and added while the next MFMA runs
+        f32x4 d[2];
+        auto add = [&](auto ec) __attribute__((always_inline)) {
+          constexpr int e = decltype(ec)::value, i = e % NT, j = e / NT;
           if constexpr (UNI) {
             const float f = xs[j % 3] * ws[i];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] += v[r] * f;
+            for (int r = 0; r < 4; ++r) acc[i][j][r] += d[e & 1][r] * f;
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] += v[r] * (xs[j % 3] * ws[i][r]);
+            for (int r = 0; r < 4; ++r) acc[i][j][r] += d[e & 1][r] * (xs[j % 3] * ws[i][r]);
           }
         };
         for_each<MT>([&](auto jc) __attribute__((always_inline)) {
@@ -399,11 +400,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
           __builtin_amdgcn_sched_barrier(0);
           for_each<NT>([&](auto ic) __attribute__((always_inline)) {
             constexpr int i = decltype(ic)::value;
-            d[j & 1][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            constexpr int Q = j * NT + i;
+            d[Q & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
                 w[i], x[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 127, 0, 127);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (j > 0) add(i, j - 1);
-            constexpr int Q = j * NT + i;
+            if constexpr (Q > 0) add(std::integral_constant<int, Q - 1>{});
             if constexpr (Q < ND) {
               if (dma) {
                 if constexpr (Q < PER) copy(std::integral_constant<int, Q>{}, koff, nslot, false);
@@ -413,8 +414,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
             __builtin_amdgcn_sched_barrier(0);
           });
         });
-#pragma unroll
-        for (int i = 0; i < NT; ++i) add(i, MT - 1);
+        add(std::integral_constant<int, MT * NT - 1>{});
       } else {
         if (dma) issue(kn);
 #pragma unroll
@@ -546,25 +546,30 @@ __global__ __launch_bounds__(256) void linear_finish_kernel(const LinArgs a, con
              ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * osize)) & 15) == 0);
 }
 
-// The tiles that calls choose from.  us: time of one round of a stage on every
-// CU, measured (bf16 4096 x 4096 x 4096, 2048 x 4096 x 4096, 512 x 4096 x 4096; e4m3
-// alike); per_cu: workgroups of it that a CU holds at once.
+// The tiles that calls choose from.  us: time of one stage (128 bytes of K) on
+// every CU at once; per_cu: workgroups of the tile that a CU holds.
 struct Tile {
   int bm, bn, per_cu;
-  float us16, us8;
+  float us;
 };
-constexpr Tile kTiles[] = {
-    {256, 256, 1, 1.80f, 1.80f},  // 8 waves, 2 stages
-    {128, 128, 2, 1.15f, 1.15f},  // 4 waves, 2 stages, two workgroups per CU
-    {128, 128, 1, 0.60f, 0.60f},  // 4 waves, 4 stages
-    {64, 128, 1, 0.48f, 0.48f},   // 4 waves, 4 stages
-};
+// Measured at 8192 x 4096 x 4096 / 2048 x 4096 x 4096 / 1003 x 4096 x 4096 / 400 x
+// 4096 x 4096 (242 / 77 / 46 / 31 us).  256 x 256: 8 waves of 128 x 64 and two
+// stages (four of 64 bytes: 5 % slower; 4 waves of 128 x 128: alike); two
+// workgroups of 128 x 128 per CU hide each other's epilogues, one with four
+// stages hides the latency where tiles are few.
+constexpr Tile kTiles16[] = {
+    {256, 256, 1, 1.78f}, {128, 128, 2, 1.16f}, {128, 128, 1, 0.66f}, {64, 128, 1, 0.43f}};
+// e4m3 at 8192 x / 2048 x / 1003 x / 400 x 4096 x 4096 (210 / 59 / 40 / 25 us): 256 x
+// 256 leaves no registers for the scaled sums (spills, 288 us).
+constexpr Tile kTiles8[] = {
+    {128, 256, 1, 1.45f}, {128, 128, 2, 1.73f}, {128, 128, 1, 1.08f}, {64, 128, 1, 0.68f}};
 constexpr int kMaxSplits = 16;
 
 struct Plan {
   int tile, splits, per;  // stages per split
 };
 
+// 16 weight rows from a multiple of 16 share a scale block
 bool uniform_scales(const LinArgs& a) { return !lin_gated(a.activation) || a.N % 16 == 0; }
 
 // The tile and the split of K with the least estimated time: rounds of the
@@ -579,8 +584,7 @@ Plan plan(const LinArgs& a) {
   Plan best{-1, 1, nk};
   double best_us = 0;
   for (int t = 0; t < 4; ++t) {
-    const Tile& c = kTiles[t];
-    if (t == 0 && fp8 && (exact || !uniform_scales(a))) continue;
+    const Tile& c = fp8 ? kTiles8[t] : kTiles16[t];
     for (int s = 1; s <= kMaxSplits; ++s) {
       const int per = static_cast<int>(cdiv(nk, s));
       if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
@@ -589,7 +593,7 @@ Plan plan(const LinArgs& a) {
                            cdiv(g && s > 1 ? 2 * a.N : a.N, g && s == 1 ? c.bn / 2 : c.bn) * s;
       const double slots = 256.0 * c.per_cu;
       const double rounds = tiles <= 256 && c.per_cu > 1 ? 0.62 : __builtin_ceil(tiles / slots);
-      double us = rounds * ((fp8 ? c.us8 : c.us16) * (exact ? 2 : 1) * per + 3.0);
+      double us = rounds * (c.us * (exact ? 2 : 1) * per + 3.0);
       if (s > 1) us += 4.0 + 2.0 * s * a.M * rows * 4 / 5e6;
       if (best.tile < 0 || us < best_us) {
         best = {t, s, per};
@@ -600,7 +604,8 @@ Plan plan(const LinArgs& a) {
   return best;
 }
 
-template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int SB, int NSTAGE, int D>
+template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int SB, int NSTAGE,
+          int D>
 int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
   const int tm = static_cast<int>(cdiv(a.M, BM)), tn = static_cast<int>(cdiv(a.N, GATED ? BN / 2 : BN));
   const dim3 grid(static_cast<unsigned>(cdiv(static_cast<int64_t>(tm) * tn * p.splits, 8) * 8));
@@ -616,9 +621,9 @@ int launch_tiles(const LinArgs& a, const Plan& p, hipStream_t st) {
   const bool uni = !FP8 || uniform_scales(a);
   switch (p.tile) {
     case 0:
-      if constexpr (KIND != K_FP8_EXACT)
-        return launch<KIND, GATED, true, 256, 256, 2, 4, 128, 2, 1>(a, p, st);
-      return set_error(MI355MOE_ERR_UNSUPPORTED, "linear: no such tile");
+      if constexpr (!FP8) return launch<KIND, GATED, true, 256, 256, 2, 4, 128, 2, 1>(a, p, st);
+      else return uni ? launch<KIND, GATED, true, 128, 256, 2, 4, 128, 3, 1>(a, p, st)
+                      : launch<KIND, GATED, false, 128, 256, 2, 4, 128, 3, 1>(a, p, st);
     case 1:
       return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 128, 2, 1>(a, p, st)
                  : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 128, 2, 1>(a, p, st);

@@ -884,6 +884,43 @@ void rms_norm(const std::optional<at::Tensor>& out, const std::optional<at::Tens
   check_rc(mi355moe_rms_norm(&a, cur_stream(input)), "rms_norm");
 }
 
+// The same with outputs made here (1.2 us a call less than made in Python):
+// [q, scales] with a group size, the norm with `with_norm`, the new residual with
+// a residual, in this order.
+std::vector<at::Tensor> rms_norm_new(const at::Tensor& input, const at::Tensor& weight,
+                                     const std::optional<at::Tensor>& residual, double epsilon,
+                                     bool with_norm, std::optional<int64_t> group_size,
+                                     std::optional<at::ScalarType> scale_dtype, bool scale_ue8m0,
+                                     bool is_scale_transposed) {
+  TORCH_CHECK(input.dim() >= 1 && input.sym_size(-1) > 0, "input must have columns");
+  std::vector<at::Tensor> made;
+  std::optional<at::Tensor> q, scales, out, residual_out;
+  const auto sizes = input.sym_sizes();
+  if (group_size) {
+    TORCH_CHECK(*group_size > 0, "group_size must be 32, 64, or 128, got ", *group_size);
+    const c10::SymInt cols = input.sym_size(-1), rows = input.sym_numel() / cols;
+    const c10::SymInt groups = cols / c10::SymInt(*group_size);
+    q = at::empty_symint(sizes, input.options().dtype(at::kFloat8_e4m3fn));
+    const auto so = input.options().dtype(scale_dtype.value_or(at::kFloat));
+    scales = is_scale_transposed ? at::empty_symint({groups, rows}, so).t()
+                                 : at::empty_symint({rows, groups}, so);
+    made.push_back(*q);
+    made.push_back(*scales);
+  }
+  if (with_norm) {
+    out = at::empty_symint(sizes, input.options());
+    made.push_back(*out);
+  }
+  if (residual) {
+    residual_out = at::empty_symint(sizes, input.options());
+    made.push_back(*residual_out);
+  }
+  if (!input.is_meta())
+    rms_norm(out, q, scales, residual_out, input, weight, residual, epsilon,
+             group_size.value_or(128), scale_ue8m0);
+  return made;
+}
+
 // [.., cols] as [rows, cols] with one row stride
 int64_t row_stride(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
@@ -992,6 +1029,21 @@ void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Te
   at::Tensor ws;
   if (need) ws = at::empty({static_cast<int64_t>(need)}, input.options().dtype(at::kByte));
   check_rc(mi355moe_linear(&a, need ? ws.data_ptr() : nullptr, need, cur_stream(input)), "linear");
+}
+
+at::Tensor linear_new(const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
+                      const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
+                      const std::optional<at::Tensor>& bias,
+                      const std::optional<at::Tensor>& residual, int64_t activation,
+                      at::ScalarType out_dtype) {
+  TORCH_CHECK(input.dim() >= 1, "input must have at least one dimension");
+  TORCH_CHECK(weight.dim() == 2, "weight must be 2-dimensional");
+  std::vector<c10::SymInt> sizes(input.sym_sizes().begin(), input.sym_sizes().end());
+  sizes.back() = activation >= MI355MOE_LINEAR_SILU_AND_MUL ? weight.sym_size(0) / 2 : weight.sym_size(0);
+  at::Tensor out = at::empty_symint(sizes, input.options().dtype(out_dtype));
+  if (!input.is_meta())
+    linear(out, input, input_scale, weight, weight_scale, bias, residual, activation);
+  return out;
 }
 
 // ------------------------------------------------------------- grouped GEMM
@@ -1430,14 +1482,23 @@ TORCH_LIBRARY(_mi355_C, m) {
         "bool scale_ue8m0=False) -> ()");
   m.def("linear(Tensor! out, Tensor input, Tensor? input_scale, Tensor weight, "
         "Tensor? weight_scale, Tensor? bias, Tensor? residual, int activation) -> ()");
+  m.def("rms_norm_new(Tensor input, Tensor weight, Tensor? residual, float epsilon, "
+        "bool with_norm=True, int? group_size=None, ScalarType? scale_dtype=None, "
+        "bool scale_ue8m0=False, bool is_scale_transposed=False) -> Tensor[]");
+  m.def("linear_new(Tensor input, Tensor? input_scale, Tensor weight, Tensor? weight_scale, "
+        "Tensor? bias, Tensor? residual, int activation, ScalarType out_dtype) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(_mi355_C, CUDA, m) {
   m.impl("rms_norm", &rms_norm);
   m.impl("linear", &linear);
+  m.impl("rms_norm_new", &rms_norm_new);
+  m.impl("linear_new", &linear_new);
 }
 
 TORCH_LIBRARY_IMPL(_mi355_C, Meta, m) {
   for (const char* op : {"rms_norm", "linear"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&meta_noop>());
+  m.impl("rms_norm_new", &rms_norm_new);
+  m.impl("linear_new", &linear_new);
 }

@@ -272,7 +272,9 @@ def _no_grad_needed(*tensors) -> None:
 
 
 _rms_norm = torch.ops._mi355_C.rms_norm.default
+_rms_norm_new = torch.ops._mi355_C.rms_norm_new.default
 _linear = torch.ops._mi355_C.linear.default
+_linear_new = torch.ops._mi355_C.linear_new.default
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -289,17 +291,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     (out, h).  h is written to residual_out, which may be residual itself
     (in place); out may be x."""
     _no_grad_needed(x, weight, residual)
+    if out is None and residual_out is None:
+        got = _rms_norm_new(x, weight, residual, eps)
+        return got[0] if residual is None else (got[0], got[1])
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out needs a residual")
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if residual is None:
-        if residual_out is not None:
-            raise ValueError("residual_out needs a residual")
-        _rms_norm(out, None, None, None, x, weight, None, eps)
-        return out
-    if residual_out is None:
+    if residual is not None and residual_out is None:
         residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     _rms_norm(out, None, None, residual_out, x, weight, residual, eps)
-    return out, residual_out
+    return out if residual is None else (out, residual_out)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -317,41 +319,44 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     (with_norm: the router's input), then the new residual (with a residual).
     The scales are a transposed view when is_scale_transposed."""
     _no_grad_needed(x, weight, residual)
+    if residual_out is None:
+        return tuple(_rms_norm_new(x, weight, residual, eps, with_norm, group_size, scale_dtype,
+                                   scale_ue8m0, is_scale_transposed))
+    if residual is None:
+        raise ValueError("residual_out needs a residual")
+    q, scales, *norm = _rms_norm_outputs(x, group_size, scale_dtype, is_scale_transposed, with_norm)
+    _rms_norm(norm[0] if norm else None, q, scales, residual_out, x, weight, residual, eps,
+              group_size, scale_ue8m0)
+    return (q, scales, *norm, residual_out)
+
+
+def _rms_norm_outputs(x, group_size, scale_dtype, transposed, with_norm):
+    rows, groups = x.numel() // max(x.shape[-1], 1), x.shape[-1] // group_size
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    H = x.shape[-1]
-    rows, groups = x.numel() // max(H, 1), H // group_size
-    if is_scale_transposed:
+    if transposed:
         scales = torch.empty((groups, rows), dtype=scale_dtype, device=x.device).t()
     else:
         scales = torch.empty((rows, groups), dtype=scale_dtype, device=x.device)
-    norm = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_norm else None
-    if residual is None:
-        if residual_out is not None:
-            raise ValueError("residual_out needs a residual")
-    elif residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _rms_norm(norm, q, scales, residual_out, x, weight, residual, eps, group_size, scale_ue8m0)
-    got = (q, scales)
-    if with_norm:
-        got += (norm,)
-    return got if residual is None else got + (residual_out,)
+    norm = (torch.empty(x.shape, dtype=x.dtype, device=x.device),) if with_norm else ()
+    return (q, scales, *norm)
 
 
 _LINEAR_ACT = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu2": 4, "silu_and_mul": 5,
                "gelu_and_mul": 6, "gelu_tanh_and_mul": 7}
 
 
-def _linear_out(x, rows, activation, out_dtype, out):
-    """(activation code, output tensor) of a product with `rows` weight rows."""
+def _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
+                default_dtype):
     code = _LINEAR_ACT.get(activation)
     if code is None:
         raise ValueError(f"Unsupported activation: {activation}.")
     if out is None:
-        out = torch.empty(x.shape[:-1] + (rows // 2 if code >= 5 else rows,), dtype=out_dtype,
-                          device=x.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
+        return _linear_new(x, x_scale, weight, weight_scale, bias, residual, code,
+                           default_dtype if out_dtype is None else out_dtype)
+    if out_dtype is not None and out.dtype != out_dtype:
         raise ValueError("out must have out_dtype")
-    return code, out
+    _linear(out, x, x_scale, weight, weight_scale, bias, residual, code)
+    return out
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -368,11 +373,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     "gelu_tanh_and_mul": f of the first half of the weight rows' results
     times the second half's, N / 2 columns.  out may be residual (in place)."""
     _no_grad_needed(x, weight, bias, residual)
-    if out is None and out_dtype is None:
-        out_dtype = x.dtype
-    code, out = _linear_out(x, weight.shape[0], activation, out_dtype, out)
-    _linear(out, x, None, weight, None, bias, residual, code)
-    return out
+    return _run_linear(x, None, weight, None, bias, activation, residual, out_dtype, out, x.dtype)
 
 
 def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
@@ -384,13 +385,11 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     x_scale [rows, K / 128] (rms_norm_quant, per_token_group_fp8_quant; any
     strides), weight [N, K] with weight_scale [ceil(N / 128), K / 128] (the
     layer's block-scaled recipe).  K % 128 == 0.  out_dtype: bfloat16 by
-    default, float16 or float32."""
+    default, float16 or float32 (whose sums have fp32's precision; 16-bit
+    outputs may use the e4m3 matrix instruction, 1.5e-5 coarser)."""
     _no_grad_needed(x_scale, weight_scale, bias, residual)
-    if out is None and out_dtype is None:
-        out_dtype = torch.bfloat16
-    code, out = _linear_out(x, weight.shape[0], activation, out_dtype, out)
-    _linear(out, x, x_scale, weight, weight_scale, bias, residual, code)
-    return out
+    return _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
+                       torch.bfloat16)
 
 
 def init_expert_map(num_experts: int, ep_rank: int, ep_size: int,

@@ -102,7 +102,7 @@ SIZES = [(1, 7168, 256), (1, 64, 1), (2, 2048, 100), (3, 8, 7), (4, 2880, 2880),
          (8, 512, 768), (9, 1024, 129), (16, 2048, 768), (17, 4096, 512), (31, 136, 72), (33, 2880, 256),
          (61, 4096, 4096), (64, 7168, 512), (65, 512, 96), (100, 2056, 200), (127, 64, 300), (129, 256, 257),
          (200, 7168, 256), (256, 2048, 1536), (300, 2880, 640), (513, 1032, 520), (1003, 2880, 2880),
-         (4, 33, 5), (70, 1001, 77), (1, 1, 1), (300, 7, 300), (2000, 96, 24), (1030, 4096, 1030)]
+         (4, 33, 5), (70, 1001, 77), (1, 1, 1), (300, 7, 300), (3, 50000, 20), (2000, 96, 24), (1030, 4096, 1030)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
@@ -176,7 +176,8 @@ def _fp8_case(M, K, N, act=None, bias=None, residual=None, out="bf16", seed=0):
 
 FP8_SIZES = [(1, 7168, 512), (3, 7168, 2048), (1, 128, 1), (2, 256, 130), (5, 384, 99), (8, 2048, 256),
              (9, 1152, 200), (16, 4096, 576), (17, 512, 384), (48, 7168, 320), (64, 256, 100),
-             (65, 1280, 264), (130, 512, 257), (200, 2048, 1000), (513, 896, 640), (1030, 2048, 1030)]
+             (65, 1280, 264), (2, 20480, 24), (3, 33024, 40), (12, 32768, 33),
+             (130, 512, 257), (200, 2048, 1000), (513, 896, 640), (1030, 2048, 1030)]
 
 
 @pytest.mark.parametrize("M,K,N", FP8_SIZES)

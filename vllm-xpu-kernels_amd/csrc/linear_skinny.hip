@@ -32,11 +32,11 @@ __device__ __forceinline__ uint4 as4(u32x4 v) { return make_uint4(v.x, v.y, v.z,
 
 constexpr int kScaleBytes = 48 * 1024;  // LDS for the e4m3 scales
 
-template <bool FP8, bool F16, bool GATED, int R, int MT, int NT, int U>
-__global__ __launch_bounds__(512) void linear_skinny_kernel(const LinArgs a) {
+template <bool FP8, bool F16, bool GATED, int R, int MT, int U>
+__global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   constexpr int C = 16 / R;
   constexpr int STEP = C * 64;                // bytes of a row per K step
-  constexpr int NS = GATED ? 2 * NT : NT;     // strips: gate and factor interleaved
+  constexpr int NS = GATED ? 2 : 1;           // strips: the gate's, the factor's
   constexpr int EB = FP8 ? 1 : 2;
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -44,19 +44,17 @@ __global__ __launch_bounds__(512) void linear_skinny_kernel(const LinArgs a) {
   const int waves = static_cast<int>(blockDim.x) >> 6;
   const int l16 = lane & 15, q = lane >> 4;
   const int ri = l16 % R, ci = l16 / R;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (R * NT);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * R;
   const int64_t mbase = static_cast<int64_t>(blockIdx.y) * (R * MT);
   const int kbytes = static_cast<int>(a.K) * EB, kfull = kbytes & ~15;  // K <= 2^28
 
-  // row n0 + R t + ri of each strip; rows and columns past the edges repeat the
-  // last one and are not stored
+  // row n0 + ri of each strip; rows past the edges repeat the last one and are
+  // not stored
   const uint8_t* wp[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    const int t = GATED ? s >> 1 : s;
-    int64_t n = n0 + R * t + ri;
-    n = n < a.N ? n : a.N - 1;
-    if (GATED && (s & 1)) n += a.N;
+    int64_t n = n0 + ri;
+    n = (n < a.N ? n : a.N - 1) + s * a.N;
     wp[s] = static_cast<const uint8_t*>(a.weight) + n * a.ldw * EB;
   }
   const uint8_t* xp[MT];
@@ -100,10 +98,8 @@ __global__ __launch_bounds__(512) void linear_skinny_kernel(const LinArgs a) {
   if constexpr (FP8) {
     for (int i = tid; i < kblocks * NS * R; i += blockDim.x) {
       const int kb = i / (NS * R), s = (i / R) % NS, r = i % R;
-      const int t = GATED ? s >> 1 : s;
-      int64_t n = n0 + R * t + r;
-      n = n < a.N ? n : a.N - 1;
-      if (GATED && (s & 1)) n += a.N;
+      int64_t n = n0 + r;
+      n = (n < a.N ? n : a.N - 1) + s * a.N;
       s_ws[i] = a.weight_scale[(n / 128) * a.weight_scale_row + kb * a.weight_scale_blk];
     }
     for (int i = tid; i < kblocks * MT * R; i += blockDim.x) {
@@ -208,16 +204,15 @@ __global__ __launch_bounds__(512) void linear_skinny_kernel(const LinArgs a) {
             acc[i][j];
   }
   __syncthreads();
-  for (int o = tid; o < NT * MT * R * R; o += blockDim.x) {
-    const int r = o % R, t = (o / R) % NT, mr = (o / (R * NT)) % R, j = o / (R * NT * R);
-    const int64_t n = n0 + R * t + r, m = mbase + R * j + mr;
+  for (int o = tid; o < MT * R * R; o += blockDim.x) {
+    const int r = o % R, mr = (o / R) % R, j = o / (R * R);
+    const int64_t n = n0 + r, m = mbase + R * j + mr;
     if (n >= a.N || m >= a.M) continue;
     float z = 0.f, u = 0.f;
-    const int sg = GATED ? 2 * t : t;
     for (int w = 0; w < waves; ++w)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float* p = red + ((w * NS + sg) * MT + j) * TILE + (c * R + mr) * R + r;
+        const float* p = red + (w * NS * MT + j) * TILE + (c * R + mr) * R + r;
         z += p[0];
         if constexpr (GATED) u += p[MT * TILE];
       }
@@ -225,36 +220,42 @@ __global__ __launch_bounds__(512) void linear_skinny_kernel(const LinArgs a) {
   }
 }
 
-template <bool FP8, bool F16, bool GATED, int R, int MT, int NT, int U>
+template <bool FP8, bool F16, bool GATED, int R, int MT, int U>
 int launch(const LinArgs& a, int waves, hipStream_t st) {
-  constexpr int NS = GATED ? 2 * NT : NT;
+  constexpr int NS = GATED ? 2 : 1;
   const int64_t kblocks = FP8 ? a.K / 128 : 0;
+  // at most 48 KiB of scales (linear_skinny_takes) and 8 KiB of sums
   const size_t lds = 4 * (kblocks * (NS + MT) * R + static_cast<size_t>(waves) * NS * MT * 16 * R);
-  const dim3 grid(static_cast<unsigned>(cdiv(a.N, R * NT)), static_cast<unsigned>(cdiv(a.M, R * MT)));
-  auto kernel = linear_skinny_kernel<FP8, F16, GATED, R, MT, NT, U>;
-  if (lds > 64 * 1024)
-    MI_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                               hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-  kernel<<<grid, dim3(64 * waves), lds, st>>>(a);
+  const dim3 grid(static_cast<unsigned>(cdiv(a.N, R)), static_cast<unsigned>(cdiv(a.M, R * MT)));
+  linear_skinny_kernel<FP8, F16, GATED, R, MT, U><<<grid, dim3(64 * waves), lds, st>>>(a);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
 
-// Strip height and waves.  A strip of 4 or 8 rows gives more workgroups, one of
-// 16 fewer loads of x and, for e4m3, fewer copies of the scales; the waves of a
-// launch come to 500-1800, at 8 or more K steps each.
+// Strip height and waves, from sweeps over all of them at 1 to 48 rows of the
+// products below.  Strips of 4 or 8 rows win while strips of 16 leave CUs
+// without work (16-bit, 8 rows, 7168 x 4096 gated: 4-row strips 16.0 us, 16-row
+// 24.0); strips of 16 read x a quarter as often (4 x 7168 x 7168 23.8 against
+// 26.0, 16 x 4096 x 4096 12.2 against 15.1) and stage e4m3 scales once per 16 rows
+// (4 x 2048 x 7168 7.6 against 8.5).  More waves per strip shorten the walk over a
+// long K and lengthen the sum at its end (1 x 7168 x 7168 with 1 / 2 / 4 waves 21.0 /
+// 21.9 / 23.4, e4m3 1 x 7168 x 4096 gated 19.1 / 13.9 / 11.7).
 template <bool FP8, bool F16, bool GATED>
 int launch_rows(const LinArgs& a, hipStream_t st) {
-  const int64_t kbytes = a.K * (FP8 ? 1 : 2);
-  const bool few = a.N <= (FP8 ? 2048 : 1024);  // columns
-  auto waves = [&](int r) {
-    const int64_t steps = kbytes / (16 / r * 64), strips = cdiv(a.N, r);
-    return static_cast<int>(steps >= 32 && strips < 2048 ? 4 : 2);
-  };
-  if (a.M <= 4 && (few || !FP8)) return launch<FP8, F16, GATED, 4, 1, 1, 4>(a, waves(4), st);
-  if (a.M <= 8 && few) return launch<FP8, F16, GATED, 4, 2, 1, 4>(a, waves(4), st);
-  if (few && (a.M <= 16 || a.N <= 512)) return launch<FP8, F16, GATED, 8, 2, 1, 4>(a, waves(8), st);
-  return launch<FP8, F16, GATED, 16, 1, 1, 4>(a, waves(16), st);
+  const bool few = a.N <= 2048;  // at most 128 strips of 16
+  if constexpr (FP8) {
+    const bool lng = a.K >= 4096;
+    if (a.M <= 4 && few) return launch<FP8, F16, GATED, 4, 1, 4>(a, lng ? 4 : 2, st);
+    if (a.M <= 8 && few && lng) return launch<FP8, F16, GATED, 4, 2, 4>(a, 4, st);
+    if (few && lng) return launch<FP8, F16, GATED, 8, 2, 4>(a, 4, st);
+    return launch<FP8, F16, GATED, 16, 1, 4>(a, 4, st);
+  } else {
+    if (a.M == 1 || (a.M <= 4 && a.N < 4096))
+      return launch<FP8, F16, GATED, 4, 1, 4>(a, few ? 2 : 1, st);
+    if (a.M <= 8 && few) return launch<FP8, F16, GATED, 4, 2, 4>(a, a.N <= 1024 ? 2 : 1, st);
+    if (few && (a.M <= 16 || a.N <= 512)) return launch<FP8, F16, GATED, 8, 2, 4>(a, 2, st);
+    return launch<FP8, F16, GATED, 16, 1, 4>(a, a.N <= 5120 && a.M <= 16 ? 4 : 2, st);
+  }
 }
 
 }  // namespace
@@ -264,7 +265,7 @@ int launch_rows(const LinArgs& a, hipStream_t st) {
 // against 12.5; 61 x 4096 x 4096 22 against 16.7).
 bool linear_skinny_takes(const LinArgs& a) {
   const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
-  if (fp8 && (a.K / 128) * 4 * 48 * 4 > kScaleBytes) return false;  // scales beyond their LDS
+  if (fp8 && (a.K / 128) * 48 * 4 > kScaleBytes) return false;  // scales beyond their LDS
   const int64_t rows = lin_gated(a.activation) ? 2 * a.N : a.N;
   return a.M <= 16 || (a.M <= 64 && rows * a.K <= (int64_t(4) << 20));
 }

@@ -70,6 +70,9 @@ def _linear_args(capi, **kw):
     ({"M": 1 << 40}, b"size too large"),
     ({"N": 1 << 40}, b"size too large"),
     ({"K": 1 << 40}, b"size too large"),
+    ({"ldx": -256}, b"negative stride"),
+    ({"ldo": -64}, b"negative stride"),
+    ({"x_dtype": E4M3, "x_scale_row": -2}, b"negative stride"),
     ({"x_dtype": E4M3, "K": 192}, b"K must be divisible by 128"),
     ({"x_dtype": E4M3}, b"scales missing"),
     ({"x": None}, b"null pointer"),

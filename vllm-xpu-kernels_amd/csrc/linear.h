@@ -32,6 +32,9 @@ __host__ __device__ constexpr bool lin_gated(int act) {
   return act >= MI355MOE_LINEAR_SILU_AND_MUL;
 }
 
+// rows of the weight
+inline int64_t lin_rows(const LinArgs& a) { return lin_gated(a.activation) ? 2 * a.N : a.N; }
+
 // element i of a float32, bfloat16 or float16 array
 __device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
   if (dtype == MI355MOE_F32) return static_cast<const float*>(p)[i];
@@ -197,9 +200,10 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
 // few rows of x (linear_skinny.hip), any alignment
 bool linear_skinny_takes(const LinArgs& a);
 int launch_linear_skinny(const LinArgs& a, hipStream_t st);
-// more rows (linear_tile.hip); the workspace holds the partial sums of a split K
+// more rows (linear_tile.hip).  a0: the call; a: the same, or with a split K the
+// product of all weight rows into fp32 partial sums [splits][M][rows]
 bool linear_tile_supported(const LinArgs& a);
-size_t linear_tile_workspace(const LinArgs& a);
-int launch_linear_tile(const LinArgs& a, void* workspace, hipStream_t st);
+int linear_tile_splits(const LinArgs& a);
+int launch_linear_tile(const LinArgs& a0, const LinArgs& a, hipStream_t st);
 
 }  // namespace mi355

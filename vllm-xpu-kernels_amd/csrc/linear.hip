@@ -11,32 +11,31 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int GM = 64, GN = 64;
 
-// 16 bytes from column byte c of a row of `bytes` bytes; zeros past its end
-// and for rows that do not exist.
-template <bool VEC>
+// 16 bytes from column byte c of a row of `bytes` bytes, from any address;
+// zeros past its end and for rows that do not exist.
+typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 __device__ __forceinline__ uint4 row16(const uint8_t* row, bool ok, int64_t c, int64_t bytes) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (!ok || c >= bytes) return v;
-  if constexpr (VEC) {
-    v = *reinterpret_cast<const uint4*>(row + c);
-  } else {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (c + k < bytes) w[k >> 2] |= static_cast<uint32_t>(row[c + k]) << (8 * (k & 3));
-    v = make_uint4(w[0], w[1], w[2], w[3]);
+  if (!ok || c >= bytes) return make_uint4(0, 0, 0, 0);
+  if (c + 16 <= bytes) {
+    const any_u32x4 v = *reinterpret_cast<const any_u32x4*>(row + c);
+    return make_uint4(v.x, v.y, v.z, v.w);
   }
-  return v;
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 15; ++k)
+    if (c + k < bytes) w[k >> 2] |= static_cast<uint32_t>(row[c + k]) << (8 * (k & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// VEC: rows of x and weight start at multiples of 16 bytes and are whole
-// multiples of 16 bytes long.
-template <bool FP8, bool F16, bool GATED, bool VEC>
-__global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
-  constexpr int SB = FP8 ? 128 : 64;     // bytes of a K stage per row (128 e4m3 / 32 16-bit)
+// K stages [split * per, ...) of 128 bytes; the next stage's rows are in registers
+// while this one's products run.
+template <bool FP8, bool F16, bool GATED>
+__global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int per) {
+  constexpr int SB = 128;                // bytes of a K stage per row
   constexpr int PITCH = SB + 16;
   constexpr int WR = GATED ? 2 * GN : GN;
   constexpr int NH = GATED ? 2 : 1;
+  constexpr int XC = GM * (SB / 16) / 256, WC = WR * (SB / 16) / 256;  // 16-byte pieces per thread
   __shared__ __attribute__((aligned(16))) uint8_t sx[GM * PITCH];
   __shared__ __attribute__((aligned(16))) uint8_t sw[WR * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -47,6 +46,9 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
   const int64_t kbytes = a.K * EB;
   const uint8_t* x = static_cast<const uint8_t*>(a.x);
   const uint8_t* w = static_cast<const uint8_t*>(a.weight);
+  const int64_t kfirst = static_cast<int64_t>(blockIdx.z) * per * SB;
+  const int64_t kend = kfirst + static_cast<int64_t>(per) * SB < kbytes
+                           ? kfirst + static_cast<int64_t>(per) * SB : kbytes;
 
   f32x4 acc[NH][4];
 #pragma unroll
@@ -54,22 +56,37 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int64_t k0 = 0; k0 < kbytes; k0 += SB) {
-    __syncthreads();  // the previous stage is read
-    for (int i = tid; i < GM * (SB / 16); i += 256) {
-      const int r = i / (SB / 16), c = (i % (SB / 16)) * 16;
-      const int64_t m = m0 + r;
-      *reinterpret_cast<uint4*>(sx + r * PITCH + c) =
-          row16<VEC>(x + m * a.ldx * EB, m < a.M, k0 + c, kbytes);
+  uint4 px[XC], pw[WC];
+  auto fetch = [&](int64_t k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < XC; ++e) {
+      const int i = e * 256 + tid;
+      const int64_t m = m0 + i / (SB / 16);
+      px[e] = row16(x + m * a.ldx * EB, m < a.M, k + (i % (SB / 16)) * 16, kbytes);
     }
-    for (int i = tid; i < WR * (SB / 16); i += 256) {
-      const int r = i / (SB / 16), c = (i % (SB / 16)) * 16;
+#pragma unroll
+    for (int e = 0; e < WC; ++e) {
+      const int i = e * 256 + tid, r = i / (SB / 16);
       const int64_t n = n0 + (GATED ? r % GN : r);
-      const int64_t row = n + (GATED && r >= GN ? a.N : 0);
-      *reinterpret_cast<uint4*>(sw + r * PITCH + c) =
-          row16<VEC>(w + row * a.ldw * EB, n < a.N, k0 + c, kbytes);
+      pw[e] = row16(w + (n + (GATED && r >= GN ? a.N : 0)) * a.ldw * EB, n < a.N,
+                    k + (i % (SB / 16)) * 16, kbytes);
+    }
+  };
+  fetch(kfirst);
+  for (int64_t k0 = kfirst; k0 < kend; k0 += SB) {
+    __syncthreads();  // the previous stage is read
+#pragma unroll
+    for (int e = 0; e < XC; ++e) {
+      const int i = e * 256 + tid;
+      *reinterpret_cast<uint4*>(sx + (i / (SB / 16)) * PITCH + (i % (SB / 16)) * 16) = px[e];
+    }
+#pragma unroll
+    for (int e = 0; e < WC; ++e) {
+      const int i = e * 256 + tid;
+      *reinterpret_cast<uint4*>(sw + (i / (SB / 16)) * PITCH + (i % (SB / 16)) * 16) = pw[e];
     }
     __syncthreads();
+    if (k0 + SB < kend) fetch(k0 + SB);  // uniform
     if constexpr (FP8) {
       const int64_t kb = k0 / 128;
 #pragma unroll
@@ -106,16 +123,22 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
       }
     } else {
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const uint4 av = *reinterpret_cast<const uint4*>(sw + (h * GN + 16 * wave + l16) * PITCH + 16 * q);
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 bv = *reinterpret_cast<const uint4*>(sx + (16 * j + l16) * PITCH + 16 * q);
-          acc[h][j] = mfma16_16x16x32<F16>(av, bv, acc[h][j]);
+        for (int h = 0; h < NH; ++h) {
+          const uint4 av = *reinterpret_cast<const uint4*>(sw + (h * GN + 16 * wave + l16) * PITCH +
+                                                           64 * t + 16 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 bv = *reinterpret_cast<const uint4*>(sx + (16 * j + l16) * PITCH + 64 * t + 16 * q);
+            acc[h][j] = mfma16_16x16x32<F16>(av, bv, acc[h][j]);
+          }
         }
       }
     }
   }
+  // a split writes its partial sums (float32 outputs without an epilogue)
+  const int64_t part = static_cast<int64_t>(blockIdx.z) * a.M * a.ldo;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int64_t m = m0 + 16 * j + l16;
@@ -124,22 +147,77 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
     for (int r = 0; r < 4; ++r) {
       const int64_t n = n0 + 16 * wave + 4 * q + r;
       if (n >= a.N) continue;
-      st_any(a.out, a.out_dtype, m * a.ldo + n,
+      st_any(a.out, a.out_dtype, part + m * a.ldo + n,
              lin_value(a, m, n, acc[0][j][r], acc[NH - 1][j][r]));
     }
   }
 }
 
 template <bool FP8, bool F16>
-int launch_any(const LinArgs& a, bool vec, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(cdiv(a.N, GN)), static_cast<unsigned>(cdiv(a.M, GM)));
-  const bool g = lin_gated(a.activation);
-  if (g && vec) linear_any_kernel<FP8, F16, true, true><<<grid, dim3(256), 0, st>>>(a);
-  else if (g) linear_any_kernel<FP8, F16, true, false><<<grid, dim3(256), 0, st>>>(a);
-  else if (vec) linear_any_kernel<FP8, F16, false, true><<<grid, dim3(256), 0, st>>>(a);
-  else linear_any_kernel<FP8, F16, false, false><<<grid, dim3(256), 0, st>>>(a);
+int launch_any(const LinArgs& a, int splits, int per, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(cdiv(a.N, GN)), static_cast<unsigned>(cdiv(a.M, GM)),
+                  static_cast<unsigned>(splits));
+  if (lin_gated(a.activation)) linear_any_kernel<FP8, F16, true><<<grid, dim3(256), 0, st>>>(a, per);
+  else linear_any_kernel<FP8, F16, false><<<grid, dim3(256), 0, st>>>(a, per);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
+}
+
+// K is split until there are about 1000 workgroups (four per CU), 8 stages each
+// at least.
+int any_stages(const LinArgs& a) {
+  const int64_t nk = cdiv(a.K * (a.x_dtype == MI355MOE_FP8E4M3 ? 1 : 2), 128);
+  const int64_t tiles = cdiv(a.M, GM) * cdiv(lin_rows(a), GN);
+  const int64_t most = nk / 8 > 1 ? nk / 8 : 1, want = cdiv(1000, tiles);
+  return static_cast<int>(cdiv(nk, want < most ? want : most));
+}
+int any_splits(const LinArgs& a) {
+  return static_cast<int>(cdiv(cdiv(a.K * (a.x_dtype == MI355MOE_FP8E4M3 ? 1 : 2), 128), any_stages(a)));
+}
+
+// Split K: the sum of the splits' partial sums, in their order, then the epilogue.
+__global__ __launch_bounds__(256) void linear_finish_kernel(const LinArgs a, const float* part,
+                                                            int splits, int64_t rows) {
+  const int64_t chunks = (a.N + 7) / 8;
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (idx >= a.M * chunks) return;
+  const int64_t m = idx / chunks, n = (idx % chunks) * 8;
+  const bool gated = lin_gated(a.activation);
+  float z[8], u[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) z[k] = u[k] = 0.f;
+  const int64_t step = a.M * rows;
+  const bool vec = (rows & 3) == 0 && (a.N & 3) == 0 && n + 8 <= a.N;
+  for (int s = 0; s < splits; ++s) {
+    const float* p = part + s * step + m * rows + n;
+    if (vec) {
+      const f32x4 p0 = reinterpret_cast<const f32x4*>(p)[0], p1 = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        z[k] += p0[k];
+        z[4 + k] += p1[k];
+      }
+      if (gated) {
+        const f32x4 q0 = reinterpret_cast<const f32x4*>(p + a.N)[0];
+        const f32x4 q1 = reinterpret_cast<const f32x4*>(p + a.N)[1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          u[k] += q0[k];
+          u[4 + k] += q1[k];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (n + k < a.N) {
+          z[k] += p[k];
+          if (gated) u[k] += p[a.N + k];
+        }
+    }
+  }
+  const int osize = a.out_dtype == MI355MOE_F32 ? 4 : 2;
+  lin_store8(a, m, n, z, u,
+             ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * osize)) & 15) == 0);
 }
 
 bool float_dtype(int d) {
@@ -158,6 +236,9 @@ int check(const LinArgs& a) {
          "linear: unknown activation");
   MI_ARG(a.M >= 0 && a.N > 0 && a.K > 0, "linear: invalid shape");
   MI_ARG(a.M <= 64 * 65535 && a.N <= (1 << 28) && a.K <= (1 << 28), "linear: size too large");
+  MI_ARG(a.ldx >= 0 && a.ldw >= 0 && a.ldr >= 0 && a.ldo >= 0 && a.x_scale_row >= 0 &&
+             a.x_scale_blk >= 0 && a.weight_scale_row >= 0 && a.weight_scale_blk >= 0,
+         "linear: negative stride");
   MI_ARG(!fp8 || a.K % 128 == 0, "linear: K must be divisible by 128 for float8 operands");
   return MI355MOE_OK;
 }
@@ -168,6 +249,15 @@ int check(const LinArgs& a) {
 using namespace mi355;
 
 namespace {
+int launch_linear_finish(const LinArgs& a, const float* part, int splits, hipStream_t st) {
+  linear_finish_kernel<<<dim3(static_cast<unsigned>(cdiv(a.M * cdiv(a.N, 8), 256))), dim3(256), 0, st>>>(
+      a, part, splits, lin_rows(a));
+  MI_LAUNCH_CHECK();
+  return MI355MOE_OK;
+}
+size_t lin_partials(const LinArgs& a, int splits) {
+  return splits == 1 ? 0 : static_cast<size_t>(splits) * a.M * lin_rows(a) * sizeof(float);
+}
 enum Path { SKINNY, TILE, ANY };
 Path path_of(const LinArgs& a) {
   if (linear_skinny_takes(a)) return SKINNY;
@@ -177,7 +267,9 @@ Path path_of(const LinArgs& a) {
 
 extern "C" size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* p) {
   if (!p || check(*p) || p->M == 0) return 0;
-  return path_of(*p) == TILE ? linear_tile_workspace(*p) : 0;
+  const Path path = path_of(*p);
+  return path == SKINNY ? 0
+                        : lin_partials(*p, path == TILE ? linear_tile_splits(*p) : any_splits(*p));
 }
 
 extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
@@ -190,22 +282,25 @@ extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
   MI_ARG(a.x && a.weight && a.out, "null pointer");
   MI_ARG(!fp8 || (a.x_scale && a.weight_scale), "linear: scales missing");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (path_of(a)) {
-    case SKINNY: return launch_linear_skinny(a, st);
-    case TILE: {
-      const size_t need = linear_tile_workspace(a);
-      MI_CHECK(need == 0 || (workspace && workspace_bytes >= need), MI355MOE_ERR_WORKSPACE,
-               "linear: workspace too small");
-      return launch_linear_tile(a, workspace, st);
-    }
-    default: break;
+  const Path path = path_of(a);
+  if (path == SKINNY) return launch_linear_skinny(a, st);
+  const int splits = path == TILE ? linear_tile_splits(a) : any_splits(a);
+  MI_CHECK(splits == 1 || (workspace && workspace_bytes >= lin_partials(a, splits)),
+           MI355MOE_ERR_WORKSPACE, "linear: workspace too small");
+  // a split product leaves fp32 partial sums of all weight rows
+  LinArgs b = a;
+  if (splits > 1) {
+    b.N = b.ldo = lin_rows(a);
+    b.activation = MI355MOE_LINEAR_NONE;
+    b.bias = b.residual = nullptr;
+    b.out = workspace;
+    b.out_dtype = MI355MOE_F32;
   }
-  const int eb = fp8 ? 1 : 2;
-  auto rows16 = [&](const void* p_, int64_t ld) {
-    return ((reinterpret_cast<uintptr_t>(p_) | static_cast<uintptr_t>(ld * eb)) & 15) == 0;
-  };
-  const bool vec = rows16(a.x, a.ldx) && rows16(a.weight, a.ldw) && a.K * eb % 16 == 0;
-  if (fp8) return launch_any<true, false>(a, vec, st);
-  return a.x_dtype == MI355MOE_F16 ? launch_any<false, true>(a, vec, st)
-                                   : launch_any<false, false>(a, vec, st);
+  int rc;
+  if (path == TILE) rc = launch_linear_tile(a, b, st);
+  else if (fp8) rc = launch_any<true, false>(b, splits, any_stages(a), st);
+  else if (a.x_dtype == MI355MOE_F16) rc = launch_any<false, true>(b, splits, any_stages(a), st);
+  else rc = launch_any<false, false>(b, splits, any_stages(a), st);
+  if (rc || splits == 1) return rc;
+  return launch_linear_finish(a, static_cast<const float*>(workspace), splits, st);
 }

@@ -266,8 +266,8 @@ int launch_rows(const LinArgs& a, hipStream_t st) {
 bool linear_skinny_takes(const LinArgs& a) {
   const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
   if (fp8 && (a.K / 128) * 48 * 4 > kScaleBytes) return false;  // scales beyond their LDS
-  const int64_t rows = lin_gated(a.activation) ? 2 * a.N : a.N;
-  return a.M <= 16 || (a.M <= 64 && rows * a.K <= (int64_t(4) << 20));
+  const int64_t rows = lin_rows(a);
+  return a.M <= 16 || (a.M <= 64 && (rows * a.K <= (int64_t(4) << 20)));
 }
 
 int launch_linear_skinny(const LinArgs& a, hipStream_t st) {

@@ -501,51 +501,6 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
   }
 }
 
-// ---- split K: the sum of the splits' partial sums, then the epilogue
-__global__ __launch_bounds__(256) void linear_finish_kernel(const LinArgs a, const float* part,
-                                                            int splits, int64_t rows) {
-  const int64_t chunks = (a.N + 7) / 8;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (idx >= a.M * chunks) return;
-  const int64_t m = idx / chunks, n = (idx % chunks) * 8;
-  const bool gated = lin_gated(a.activation);
-  float z[8], u[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) z[k] = u[k] = 0.f;
-  const int64_t step = a.M * rows;
-  const bool vec = (rows & 3) == 0 && (a.N & 3) == 0 && n + 8 <= a.N;
-  for (int s = 0; s < splits; ++s) {
-    const float* p = part + s * step + m * rows + n;
-    if (vec) {
-      const f32x4 p0 = reinterpret_cast<const f32x4*>(p)[0], p1 = reinterpret_cast<const f32x4*>(p)[1];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        z[k] += p0[k];
-        z[4 + k] += p1[k];
-      }
-      if (gated) {
-        const f32x4 q0 = reinterpret_cast<const f32x4*>(p + a.N)[0];
-        const f32x4 q1 = reinterpret_cast<const f32x4*>(p + a.N)[1];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          u[k] += q0[k];
-          u[4 + k] += q1[k];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (n + k < a.N) {
-          z[k] += p[k];
-          if (gated) u[k] += p[a.N + k];
-        }
-    }
-  }
-  const int osize = a.out_dtype == MI355MOE_F32 ? 4 : 2;
-  lin_store8(a, m, n, z, u,
-             ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * osize)) & 15) == 0);
-}
-
 // The tiles that calls choose from.  us: time of one stage (128 bytes of K) on
 // every CU at once; per_cu: workgroups of the tile that a CU holds.
 struct Tile {
@@ -580,7 +535,7 @@ Plan plan(const LinArgs& a) {
   const bool exact = fp8 && a.out_dtype == MI355MOE_F32;
   const int nk = static_cast<int>(cdiv(a.K * (fp8 ? 1 : 2), 128));
   const bool g = lin_gated(a.activation);
-  const double rows = static_cast<double>(g ? 2 * a.N : a.N);
+  const double rows = static_cast<double>(lin_rows(a));
   Plan best{-1, 1, nk};
   double best_us = 0;
   for (int t = 0; t < 4; ++t) {
@@ -590,7 +545,7 @@ Plan plan(const LinArgs& a) {
       if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
       // a split product runs without gates, over all weight rows
       const double tiles = static_cast<double>(cdiv(a.M, c.bm)) *
-                           cdiv(g && s > 1 ? 2 * a.N : a.N, g && s == 1 ? c.bn / 2 : c.bn) * s;
+                           cdiv(s > 1 ? lin_rows(a) : a.N, g && s == 1 ? c.bn / 2 : c.bn) * s;
       const double slots = 256.0 * c.per_cu;
       const double rounds = tiles <= 256 && c.per_cu > 1 ? 0.62 : __builtin_ceil(tiles / slots);
       double us = rounds * (c.us * (exact ? 2 : 1) * per + 3.0);
@@ -649,51 +604,28 @@ bool linear_tile_supported(const LinArgs& a) {
   };
   if (!rows16(a.x, a.ldx) || !rows16(a.weight, a.ldw) || a.K * eb % 16) return false;
   if (fp8) {
-    const int64_t blocks = cdiv(lin_gated(a.activation) ? 2 * a.N : a.N, 128);
+    const int64_t blocks = cdiv(lin_rows(a), 128);
     // (block strides step a scalar base by 32 bits)
     if (256 * a.x_scale_row * 4 >= lim || a.x_scale_blk * 4 >= lim ||
         blocks * a.weight_scale_row * 4 >= lim || a.weight_scale_blk * 4 >= lim)
       return false;
   }
   // tiles and splits are counted in 32 bits
-  return cdiv(a.M, 64) * cdiv(lin_gated(a.activation) ? 2 * a.N : a.N, 64) * kMaxSplits < (int64_t(1) << 22);
+  return cdiv(a.M, 64) * cdiv(lin_rows(a), 64) * kMaxSplits < (int64_t(1) << 22);
 }
 
-size_t linear_tile_workspace(const LinArgs& a) {
-  const Plan p = plan(a);
-  return p.splits == 1 ? 0
-                       : static_cast<size_t>(p.splits) * a.M *
-                             (lin_gated(a.activation) ? 2 * a.N : a.N) * sizeof(float);
-}
+int linear_tile_splits(const LinArgs& a) { return plan(a).splits; }
 
-int launch_linear_tile(const LinArgs& a0, void* workspace, hipStream_t st) {
+int launch_linear_tile(const LinArgs& a0, const LinArgs& a, hipStream_t st) {
   const Plan p = plan(a0);
-  const bool fp8 = a0.x_dtype == MI355MOE_FP8E4M3;
-  LinArgs a = a0;
-  bool g = lin_gated(a.activation);
-  if (p.splits > 1) {  // fp32 partial sums of all weight rows
-    a.N = g ? 2 * a.N : a.N;
-    a.activation = MI355MOE_LINEAR_NONE;
-    a.bias = a.residual = nullptr;
-    a.out = workspace;
-    a.out_dtype = MI355MOE_F32;
-    a.ldo = a.N;
-    g = false;
-  }
-  int rc;
-  if (fp8 && a0.out_dtype == MI355MOE_F32)
-    rc = g ? launch_tiles<K_FP8_EXACT, true>(a, p, st) : launch_tiles<K_FP8_EXACT, false>(a, p, st);
-  else if (fp8)
-    rc = g ? launch_tiles<K_FP8, true>(a, p, st) : launch_tiles<K_FP8, false>(a, p, st);
-  else if (a.x_dtype == MI355MOE_F16)
-    rc = g ? launch_tiles<K_F16, true>(a, p, st) : launch_tiles<K_F16, false>(a, p, st);
-  else
-    rc = g ? launch_tiles<K_BF16, true>(a, p, st) : launch_tiles<K_BF16, false>(a, p, st);
-  if (rc || p.splits == 1) return rc;
-  linear_finish_kernel<<<dim3(static_cast<unsigned>(cdiv(a0.M * cdiv(a0.N, 8), 256))), dim3(256), 0, st>>>(
-      a0, static_cast<const float*>(workspace), p.splits, a.N);
-  MI_LAUNCH_CHECK();
-  return MI355MOE_OK;
+  const bool g = lin_gated(a.activation);
+  if (a.x_dtype == MI355MOE_FP8E4M3 && a0.out_dtype == MI355MOE_F32)
+    return g ? launch_tiles<K_FP8_EXACT, true>(a, p, st) : launch_tiles<K_FP8_EXACT, false>(a, p, st);
+  if (a.x_dtype == MI355MOE_FP8E4M3)
+    return g ? launch_tiles<K_FP8, true>(a, p, st) : launch_tiles<K_FP8, false>(a, p, st);
+  if (a.x_dtype == MI355MOE_F16)
+    return g ? launch_tiles<K_F16, true>(a, p, st) : launch_tiles<K_F16, false>(a, p, st);
+  return g ? launch_tiles<K_BF16, true>(a, p, st) : launch_tiles<K_BF16, false>(a, p, st);
 }
 
 }  // namespace mi355

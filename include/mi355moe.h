@@ -403,8 +403,8 @@ int mi355moe_silu_and_mul_mxfp4_quant(uint8_t* out, const void* input, int in_dt
  * The norm and the quantiser take h and y before their rounding to T.  A NaN
  * of y stays NaN in q and does not count in its group's maximum; a group
  * with an infinite y has an infinite scale, zeros, and NaN at that y.
- * Squares that overflow fp32 (|h| > 1.8e19) give y = 0, as the formula does
- * in fp32.
+ * Squares that overflow fp32 (|h| > 1.8e19) may give y = 0, as the formula
+ * does in fp32; power-of-two scales are decided in 64 bits.
  *
  * Rows: row r of x, residual, residual_out and out starts at element
  * (r / inner) * outer_stride + (r % inner) * inner_stride of its pointer

@@ -93,12 +93,20 @@ __device__ __forceinline__ uint32_t e4m3x4_nan(float v0, float v1, float v2, flo
   return static_cast<uint32_t>(w);
 }
 
+__device__ __forceinline__ bool pow2_scales(const NormArgs& a) {
+  return a.scale_dtype == MI355MOE_U8 || a.scale_ue8m0;
+}
+
 // The group's scale and the lane's 8 codes of columns i .. i + 7.  A group is
 // G / 8 consecutive, aligned lanes; every lane of the wave takes part, those
 // without columns (`active` false) with zeros.
+// Power-of-two scales double where the maximum passes 448 2^e: a maximum within
+// 2^-20 of that (fp32's error is below) is formed again in 64 bits from h, the
+// weight and rsd, the root's reciprocal in 64 bits.
 template <bool VEC>
 __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int i, bool active,
-                                       const float (&y)[8], bool nt) {
+                                       const float (&y)[8], const float (&h)[8],
+                                       const float (&w)[8], double rsd, bool nt) {
   float amax = 1e-10f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(y[k]));
@@ -114,8 +122,16 @@ __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int i, bool
   float s = fmaxf(amax / 448.0f, 1.0f / (448.0f * 512.0f));
   const bool e8m0 = a.scale_dtype == MI355MOE_U8;
   int ex = 0;
-  if (e8m0 || a.scale_ue8m0) {
+  if (pow2_scales(a)) {
     ex = ceil_log2(s);
+    const int low = ceil_log2(s * (1.0f - 0x1p-20f)), high = ceil_log2(s * (1.0f + 0x1p-20f));
+    if (low != high) {  // the same in all lanes of a group
+      double m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmax(m, fabs(static_cast<double>(h[k]) * w[k] * rsd));
+      for (int o = 1; o < (group >> 3); o <<= 1) m = fmax(m, __shfl_xor(m, o, 64));
+      ex = m / 448.0 <= ldexp(1.0, low) ? low : high;
+    }
     s = ex > 127 ? __uint_as_float(0x7F800000u) : pow2i(ex);  // an infinite maximum
   }
   if ((i & (group - 1)) == 0) {
@@ -135,6 +151,52 @@ __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int i, bool
 #pragma unroll
     for (int k = 0; k < 8; ++k) q[k] = static_cast<uint8_t>((k < 4 ? lo : hi) >> (8 * (k & 3)));
   }
+}
+
+// The row's sum of squares in T, in every lane of the row.
+template <typename T>
+__device__ __forceinline__ T wave_sum_of(T v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T workgroup_sum(T v, int waves) {
+  __shared__ T part[16];
+  v = wave_sum_of(v);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  T s = 0;
+  for (int w = 0; w < waves; ++w) s += part[w];
+  return s;
+}
+template <typename T, int LANES, int R>
+__device__ __forceinline__ T row_sum(const float (&h)[R][8], int lanes) {
+  T ss = 0;
+#pragma unroll
+  for (int c = 0; c < R; ++c)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss += static_cast<T>(h[c][k]) * h[c][k];
+  if constexpr (LANES != 0) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    return ss;
+  } else {
+    return workgroup_sum(ss, lanes >> 6);
+  }
+}
+
+// 1 / sqrt(ss / cols + eps): fp32's values with one Newton step each in 64 bits
+// (about 2^-46; the 64-bit division and root take 0.5 us of a small call)
+__device__ __forceinline__ double rsqrt64(double ss, int cols, float eps) {
+  const double r0 = 1.0f / static_cast<float>(cols);  // cols < 2^24 is exact, above off by 2^-24
+  const double inv = r0 * (2.0 - static_cast<double>(cols) * r0);
+  const double v = ss * inv + eps;
+  const float s0 = 1.0f / sqrtf(static_cast<float>(v));
+  // zero, infinite and NaN roots, and those whose square leaves fp32, stand
+  if (!(v > 1e-30 && v < 1e30)) return s0;
+  const double s = s0;
+  return s * (1.5 - 0.5 * v * s * s);
 }
 
 // LANES: lanes of a row inside a wave (8 to 64, 256 / LANES rows to a
@@ -187,24 +249,14 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void rms_norm_kernel(const Norm
       else load8<E, VEC>(a.weight, i, cols, w[c], step);
     }
   }
-  float ss = 0.f;
-#pragma unroll
-  for (int c = 0; c < R; ++c)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) ss += h[c][k] * h[c][k];
-  if constexpr (LANES != 0) {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+  float rs;
+  double rsd = 0;
+  if (QUANT && pow2_scales(a)) {  // uniform
+    rsd = rsqrt64(row_sum<double, LANES, R>(h, lanes), cols, a.eps);
+    rs = static_cast<float>(rsd);
   } else {
-    __shared__ float part[16];
-    ss = wave_sum(ss);
-    if ((t & 63) == 0) part[t >> 6] = ss;
-    __syncthreads();
-    const int waves = lanes >> 6;
-    ss = 0.f;
-    for (int v = 0; v < waves; ++v) ss += part[v];
+    rs = 1.0f / sqrtf(row_sum<float, LANES, R>(h, lanes) / static_cast<float>(cols) + a.eps);
   }
-  const float rs = 1.0f / sqrtf(ss / static_cast<float>(cols) + a.eps);
   char* res_out = a.residual_out ? static_cast<char*>(a.residual_out) +
                                        row_at<E>(rr, a.inner, a.residual_out_outer,
                                                  a.residual_out_inner)
@@ -219,7 +271,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void rms_norm_kernel(const Norm
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = h[c][k] * rs * w[c][k];
     if (out && on[c]) store8<E, VEC>(out, i, cols, y, nt, step);
-    if constexpr (QUANT) quant8<VEC>(a, rr, i, on[c], y, nt);
+    if constexpr (QUANT) quant8<VEC>(a, rr, i, on[c], y, h[c], w[c], rsd, nt);
   }
 }
 
@@ -241,20 +293,16 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a, i
       for (int k = 0; k < 8; ++k) h[k] += t[k];
     }
   };
-  float ss = 0.f;
+  // (in 64 bits: rows this long leave fp32 sums of some hundred terms per lane)
+  double ss = 0;
   for (int64_t i = threadIdx.x * 8; i < a.cols; i += 1024 * 8) {
     float h[8];
     load_h(i, h);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss += h[k] * h[k];
+    for (int k = 0; k < 8; ++k) ss += static_cast<double>(h[k]) * h[k];
   }
-  __shared__ float part[16];
-  ss = wave_sum(ss);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
-  __syncthreads();
-  ss = 0.f;
-  for (int v = 0; v < 16; ++v) ss += part[v];
-  const float rs = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  const double rsd = rsqrt64(workgroup_sum(ss, 16), static_cast<int>(a.cols), a.eps);
+  const float rs = static_cast<float>(rsd);
   for (int64_t i0 = 0; i0 < a.cols; i0 += 1024 * 8) {  // uniform: groups exchange maxima
     const int64_t i = i0 + threadIdx.x * 8;
     const bool on = i < a.cols;
@@ -273,7 +321,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a, i
     if (on && a.out)
       store8<E, VEC>(static_cast<char*>(a.out) + row_at<E>(r, a.inner, a.out_outer, a.out_inner),
                      i, a.cols, y, nt);
-    if (a.q) quant8<VEC>(a, r, static_cast<int>(on ? i : 0), on, y, nt);
+    if (a.q) quant8<VEC>(a, r, static_cast<int>(on ? i : 0), on, y, h, w, rsd, nt);
   }
 }
 

@@ -2,13 +2,13 @@
 // (rows of x, rows of the weight) whose K stages reach LDS by direct
 // global->LDS copies.
 //
-// LDS.  A stage holds SB bytes of each row of the tile, rows one after the
+// LDS.  A stage holds 128 bytes of each row of the tile, rows one after the
 // other; 16-byte chunk c of row r sits at slot c ^ swz(r), so that the 16 rows
 // that a quarter of a fragment read covers hit all 64 banks once.  A ring of
 // NSTAGE stages; stage kt + NSTAGE is requested as soon as every wave has read
 // stage kt, so NSTAGE - 1 stages are in flight.
 //
-// 16-bit operands: 32x32x16 MFMAs, SB / 32 K steps per stage, the next step's
+// 16-bit operands: 32x32x16 MFMAs, four K steps per stage, the next step's
 // fragments read while this one's MFMAs run; the barrier that publishes stage
 // kt + 1 sits before the last step of stage kt, so that the matrix cores do not
 // start a stage behind its reads.
@@ -34,6 +34,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void_t;
+
+constexpr int SB = 128;  // bytes of a row in a K stage: one e4m3 scale block, 64 16-bit values
+// slot of 16-byte chunk c of row r: c ^ swz(r)
+__device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 
 __device__ __forceinline__ uint32_t lds_off(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)p));
@@ -80,14 +84,12 @@ __device__ __forceinline__ void for_each(F&& f) {
 
 enum { K_BF16 = 0, K_F16 = 1, K_FP8 = 2, K_FP8_EXACT = 3 };
 
-template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int SB, int NSTAGE,
-          int D>
+template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int NSTAGE>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs a, int tiles_m,
                                                                     int tiles_n, int splits,
                                                                     int stages_per_split) {
   constexpr bool FP8 = KIND >= K_FP8;
   static_assert(FP8 || UNI, "scale blocks");
-  static_assert(!FP8 || SB == 128, "an e4m3 stage is one scale block");
   constexpr int EB = FP8 ? 1 : 2;
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   constexpr int TS = FP8 ? 16 : 32;              // MFMA tile side
@@ -148,14 +150,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
   const uint64_t ubase = GATED ? uniform64(wbase + a.N * a.ldw * EB) : wbase;
   uint32_t voff[PER];
   const int cslot = lane % CH, rsub = lane / CH;
-  auto swz_of = [](int r) __attribute__((always_inline)) {
-    return SB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
-  };
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
     // (the regions start at multiples of 16 rows, so a row's swizzle is its own)
     const int r = (q < XQ ? wave * XQ + q : wave * WQ + (q - XQ) % WQ) * RPB + rsub;
-    const int cb = (cslot ^ swz_of(r)) << 4;
+    const int cb = (cslot ^ swz(r)) << 4;
     const int64_t last = q < XQ ? a.M - 1 - m0 : a.N - 1 - n0;
     voff[q] = static_cast<uint32_t>((r < last ? r : last) * (q < XQ ? a.ldx : a.ldw) * EB + cb);
   }
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
     uint32_t v = voff[Q];
     if (past) {  // uniform
       const int r = (X ? wave * XQ + Q : wave * WQ + (Q - XQ) % WQ) * RPB + rsub;
-      const int cb = (cslot ^ swz_of(r)) << 4;
+      const int cb = (cslot ^ swz(r)) << 4;
       if (cb >= tail) v -= cb;
     }
     if constexpr (X) dma16<Q * 1024>(v, xbase + koff, slot + wave * (XQ * 1024));
@@ -225,9 +224,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
     uint8_t* S = lds + (kt % NSTAGE) * STAGE;
     for (int i = tid; i < (BM + BN) * CH; i += THREADS) {
       const int r = i / CH, c = i % CH;
-      const int swz = SB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
       if ((c << 4) >= tail)
-        *reinterpret_cast<uint4*>(S + r * SB + ((c ^ swz) << 4)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(S + r * SB + ((c ^ swz(r)) << 4)) = make_uint4(0, 0, 0, 0);
     }
     lds_barrier();
   };
@@ -270,19 +268,16 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
 
   if constexpr (!FP8) {
     constexpr int KS = SB / 32;  // K steps of 16 per stage
-    // fragments are read D steps ahead into NB buffers
-    constexpr int NB = D == 1 ? 2 : 4;
-    static_assert(D <= KS && KS % NB == 0, "buffer indices repeat every stage");
     const int l32 = lane & 31, h = lane >> 5;
     struct Frag {
       uint4 x[MT], w[NT];
     };
-    Frag f[NB];
-    const int swz = SB == 128 ? (l32 >> 1) & 7 : (l32 >> 2) & 3;  // rows l32 + 32 i share it
+    Frag f[2];
+    const int sw = swz(l32);  // rows l32 + 32 i share it
     // fragment e of a K step, in the order that the MFMAs want them
     constexpr int NF = MT + NT;
     auto read = [&](Frag& g, const uint8_t* S, int ks, int e) __attribute__((always_inline)) {
-      const int c = ((2 * ks + h) ^ swz) << 4;
+      const int c = ((2 * ks + h) ^ sw) << 4;
       if (e == 0 || e > MT) {
         const int i = e == 0 ? 0 : e - MT;
         g.w[i] = lds16(S + (BM + wrow(i) + l32) * SB + c);
@@ -294,9 +289,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
     // (kn of stage Sn) and, with `dma`, the copies of a stage; the order is kept.
     // (`dma`, uniform, guards the copies alone: two versions of the step would
     // have the compiler copy every accumulator where they join.)
-    constexpr int NM = NT * MT, RPM = (NF + NM - 1) / NM, CPM = (PER + D * NM - 1) / (D * NM);
-    // D steps share a stage's copies: step `d` of them takes CPM per MFMA.
-    auto step = [&](auto dma_c, bool dma, const Frag& g, Frag& next, const uint8_t* Sn, int kn,
+    constexpr int NM = NT * MT, RPM = (NF + NM - 1) / NM, CPM = (PER + NM - 1) / NM;
+    auto step = [&](auto last_c, bool dma, const Frag& g, Frag& next, const uint8_t* Sn, int kn,
                     uint64_t koff, uint32_t slot) __attribute__((always_inline)) {
       for_each<NM>([&](auto tc) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::value, i = t / MT, j = t % MT;
@@ -304,11 +298,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = t * RPM; e < (t + 1) * RPM && e < NF; ++e) read(next, Sn, kn, e);
-        constexpr int q0 = (decltype(dma_c)::value * NM + t) * CPM;
-        if constexpr (decltype(dma_c)::value >= 0 && q0 < PER) {
+        if constexpr (decltype(last_c)::value && t * CPM < PER) {
           if (dma) {
             for_each<CPM>([&](auto c) __attribute__((always_inline)) {
-              constexpr int Q = q0 + decltype(c)::value;
+              constexpr int Q = t * CPM + decltype(c)::value;
               if constexpr (Q < PER) copy(std::integral_constant<int, Q>{}, koff, slot, false);
             });
           }
@@ -317,9 +310,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
       });
     };
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-#pragma unroll
-      for (int e = 0; e < NF; ++e) read(f[d], lds, d, e);
+    for (int e = 0; e < NF; ++e) read(f[0], lds, 0, e);
     // stages [NSTAGE, nfull) are requested between MFMAs, a partial last one at once
     const int nfull = tail ? nk - 1 : nk;
     uint64_t koff = static_cast<uint64_t>(k0 + NSTAGE) * SB;
@@ -329,25 +320,22 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
       const int nslot = slot + 1 == NSTAGE ? 0 : slot + 1;
       const uint8_t* Sn = lds + nslot * STAGE;
 #pragma unroll
-      for (int ks = 0; ks + D < KS; ++ks)
-        step(std::integral_constant<int, -1>{}, false, f[ks % NB], f[(ks + D) % NB], S, ks + D, 0, 0);
+      for (int ks = 0; ks + 1 < KS; ++ks)
+        step(std::false_type{}, false, f[ks & 1], f[(ks + 1) & 1], S, ks + 1, 0, 0);
       advance(kt);
       if (tail && kt + NSTAGE == nk - 1) issue(kt + NSTAGE);
-      // after the last stage these read a stale slot, unused
-      for_each<D>([&](auto d) __attribute__((always_inline)) {
-        constexpr int ks = KS - D + decltype(d)::value;
-        step(d, kt + NSTAGE < nfull, f[ks % NB], f[(ks + D) % NB], Sn, ks + D - KS, koff,
-             ring + slot * STAGE);
-      });
+      // after the last stage this reads a stale slot, unused
+      step(std::true_type{}, kt + NSTAGE < nfull, f[(KS - 1) & 1], f[0], Sn, 0, koff,
+           ring + slot * STAGE);
       koff += SB;
       slot = nslot;
     }
   } else {
     const int l16 = lane & 15, q = lane >> 4;
-    const int swz = (l16 >> 1) & 7;
+    const int sw16 = swz(l16);
     // operand bytes 0-15 from chunk q, 16-31 from chunk 4 + q: both operands the
     // same, so the order within the block does not matter
-    const int c0 = (q ^ swz) << 4, c1 = ((4 + q) ^ swz) << 4;
+    const int c0 = (q ^ sw16) << 4, c1 = ((4 + q) ^ sw16) << 4;
     for (int kt = 0; kt < nk; ++kt) {
       const uint8_t* S = lds + (kt % NSTAGE) * STAGE;
       const float* sx = reinterpret_cast<const float*>(S + (BM + BN) * SB);
@@ -559,12 +547,11 @@ Plan plan(const LinArgs& a) {
   return best;
 }
 
-template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int SB, int NSTAGE,
-          int D>
+template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int NSTAGE>
 int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
   const int tm = static_cast<int>(cdiv(a.M, BM)), tn = static_cast<int>(cdiv(a.N, GATED ? BN / 2 : BN));
   const dim3 grid(static_cast<unsigned>(cdiv(static_cast<int64_t>(tm) * tn * p.splits, 8) * 8));
-  linear_tile_kernel<KIND, GATED, UNI, BM, BN, WM, WN, SB, NSTAGE, D>
+  linear_tile_kernel<KIND, GATED, UNI, BM, BN, WM, WN, NSTAGE>
       <<<grid, dim3(64 * WM * WN), 0, st>>>(a, tm, tn, p.splits, p.per);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
@@ -576,18 +563,18 @@ int launch_tiles(const LinArgs& a, const Plan& p, hipStream_t st) {
   const bool uni = !FP8 || uniform_scales(a);
   switch (p.tile) {
     case 0:
-      if constexpr (!FP8) return launch<KIND, GATED, true, 256, 256, 2, 4, 128, 2, 1>(a, p, st);
-      else return uni ? launch<KIND, GATED, true, 128, 256, 2, 4, 128, 3, 1>(a, p, st)
-                      : launch<KIND, GATED, false, 128, 256, 2, 4, 128, 3, 1>(a, p, st);
+      if constexpr (!FP8) return launch<KIND, GATED, true, 256, 256, 2, 4, 2>(a, p, st);
+      else return uni ? launch<KIND, GATED, true, 128, 256, 2, 4, 3>(a, p, st)
+                      : launch<KIND, GATED, false, 128, 256, 2, 4, 3>(a, p, st);
     case 1:
-      return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 128, 2, 1>(a, p, st)
-                 : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 128, 2, 1>(a, p, st);
+      return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 2>(a, p, st)
+                 : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 2>(a, p, st);
     case 2:
-      return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 128, 4, 1>(a, p, st)
-                 : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 128, 4, 1>(a, p, st);
+      return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 4>(a, p, st)
+                 : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 4>(a, p, st);
     default:
-      return uni ? launch<KIND, GATED, true, 64, 128, 2, 2, 128, 4, 1>(a, p, st)
-                 : launch<KIND, GATED, !FP8, 64, 128, 2, 2, 128, 4, 1>(a, p, st);
+      return uni ? launch<KIND, GATED, true, 64, 128, 2, 2, 4>(a, p, st)
+                 : launch<KIND, GATED, !FP8, 64, 128, 2, 2, 4>(a, p, st);
   }
 }
 

@@ -402,7 +402,7 @@ int mi355moe_silu_and_mul_mxfp4_quant(uint8_t* out, const void* input, int in_dt
  *   scale_ue8m0 and for e8m0 scales; q = e4m3(clamp(y * (1 / s), +-448)).
  * The norm and the quantiser take h and y before their rounding to T.  A NaN
  * of y stays NaN in q and does not count in its group's maximum; a group
- * with an infinite y has an infinite scale, zeros, and NaN at that y.
+ * with an infinite y has an infinite scale (e8m0: NaN), zeros, and NaN there.
  * Squares that overflow fp32 (|h| > 1.8e19) may give y = 0, as the formula
  * does in fp32; power-of-two scales are decided in 64 bits.
  *
@@ -463,8 +463,11 @@ typedef enum {
  * Row strides ld* and scale strides are in elements; columns of x, weight,
  * bias, residual and out are contiguous.  M may be 0; N and K are positive.
  * out may be residual with the same stride and type; otherwise it may overlap
- * no input.  Products of few rows or few tiles split K and need the
- * workspace of mi355moe_linear_workspace_size (0 for many sizes). */
+ * no input, nor one of its rows another.  M <= 4194240, N <= 2^24, K <= 2^28.
+ * Products of few rows or few tiles split K and need a workspace, 16-byte
+ * aligned, of mi355moe_linear_workspace_size bytes (0 for many sizes).  That is
+ * asked with the call's own arguments, pointers and strides included: the
+ * operands' alignment takes part in the choice. */
 typedef struct {
   int x_dtype;          /* BF16, F16 or FP8E4M3                               */
   int out_dtype;        /* F32, BF16 or F16                                   */

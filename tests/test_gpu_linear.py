@@ -448,3 +448,15 @@ def test_moe_block_of_these_operators(dev, T):
 
 
 EPS_ = 1e-6
+
+
+@pytest.mark.parametrize("act", [None, "silu_and_mul"])
+def test_linear_many_tiles(dev, act):
+    """Outputs whose elements pass 2^31, some hundred thousand tiles."""
+    M, K, N = 262144, 64, 8448
+    x = _rand((M, K), torch.bfloat16, 71)
+    w = _rand((2 * N if act else N, K), torch.bfloat16, 72, 0.125)
+    out = _ops().linear(x, w, activation=act)
+    for m in (0, 131001, M - 70):
+        r = slice(m, m + 70)
+        _close(out[r], *_want(x[r].double(), w.double(), None, act, None))

@@ -296,3 +296,19 @@ def test_traced_by_the_compiler_front_end(dev):
     f = torch.compile(lambda a, b: o.rms_norm(a, b, EPS), backend="aot_eager", fullgraph=True)
     assert torch.equal(f(x, w), o.rms_norm(x, w, EPS))
     assert math.isfinite(float(x.float().sum()))
+
+
+def test_rms_norm_leading_dimensions_of_one(dev):
+    """Slices that leave a dimension of one element between others: its stride
+    does not count."""
+    w = _rand((64,), torch.bfloat16, 61) + 1
+    buf = _rand((6, 5, 3, 64), torch.bfloat16, 62)
+    for x in (buf[:, 2:3], buf[:, 4:, 1:], buf[3:4, :, :2], buf[:, :, 1:2][:, 1:2], buf[2:3, 1:2, 2:]):
+        _close(_ops().rms_norm(x, w, EPS), _exact(x, w)[1])
+        y = x.contiguous()
+        want, wr = _ops().rms_norm(y, w, EPS, residual=y)
+        out = torch.full_like(buf, 7.0).as_strided(x.shape, x.stride(), x.storage_offset())
+        got, r = _ops().rms_norm(x, w, EPS, residual=x, out=out)
+        assert torch.equal(got, want) and torch.equal(r, wr)
+    with pytest.raises(RuntimeError, match="do not fold"):
+        _ops().rms_norm(buf[:, :2].unsqueeze(2).expand(6, 2, 2, 3, 64), w, EPS)

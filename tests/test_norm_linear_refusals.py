@@ -136,3 +136,36 @@ def test_meta_kernels_trace():
     assert q.shape == n.shape == r.shape == (3, 128) and s.shape == (3, 1)
     w = torch.zeros(16, 128, dtype=torch.bfloat16, device="meta")
     assert ops.linear(x, w, activation="silu_and_mul").shape == (3, 8)
+
+
+def test_linear_workspace_is_checked(capi):
+    """A product that splits K refuses a workspace that is missing, too small or
+    not aligned, and rows of out that meet, before any device work."""
+    a = _linear_args(capi, M=61, N=4096, K=4096, ldx=4096, ldw=4096, ldo=4096, x=1 << 20,
+                     weight=1 << 20, out=1 << 20)
+    a.x += 2                               # unaligned rows: 64 x 64 tiles, too few without splits
+    need = capi.lib.mi355moe_linear_workspace_size(ctypes.byref(a))
+    assert need > 0 and need % (61 * 4096 * 4) == 0
+    for ws, size in ((None, 0), (None, need), (1 << 20, need - 1)):
+        assert capi.lib.mi355moe_linear(ctypes.byref(a), ws, size, None) == -4
+        assert b"workspace too small" in capi.lib.mi355moe_last_error()
+    assert capi.lib.mi355moe_linear(ctypes.byref(a), (1 << 20) + 4, need, None) == -1
+    assert b"workspace must be 16-byte aligned" in capi.lib.mi355moe_last_error()
+
+
+@pytest.mark.parametrize("kw,msg", [({"N": (1 << 24) + 1, "ldo": 1 << 25}, b"size too large"),
+                                    ({"M": 64 * 65535 + 1}, b"size too large"),
+                                    ({"ldo": 63}, b"rows of out overlap"),
+                                    ({"ldo": 0}, b"rows of out overlap")])
+def test_linear_refuses_sizes_beyond_its_grids(capi, kw, msg):
+    a = _linear_args(capi, **kw)
+    assert capi.lib.mi355moe_linear(ctypes.byref(a), None, 0, None) == -1
+    assert msg in capi.lib.mi355moe_last_error()
+
+
+@pytest.mark.parametrize("group", [0, -128, 48])
+def test_rms_norm_quant_refuses_groups(group):
+    from vllm_xpu_kernels import ops
+    x = torch.zeros(2, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="group_size must be 32, 64, or 128"):
+        ops.rms_norm_quant(x, x[0], residual=x, residual_out=x, group_size=group)

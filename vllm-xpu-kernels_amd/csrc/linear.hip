@@ -235,10 +235,12 @@ int check(const LinArgs& a) {
   MI_ARG(a.activation >= MI355MOE_LINEAR_NONE && a.activation <= MI355MOE_LINEAR_GELU_TANH_AND_MUL,
          "linear: unknown activation");
   MI_ARG(a.M >= 0 && a.N > 0 && a.K > 0, "linear: invalid shape");
-  MI_ARG(a.M <= 64 * 65535 && a.N <= (1 << 28) && a.K <= (1 << 28), "linear: size too large");
+  // grids and their threads are counted in 32 bits (4 weight rows to a workgroup)
+  MI_ARG(a.M <= 64 * 65535 && a.N <= (1 << 24) && a.K <= (1 << 28), "linear: size too large");
   MI_ARG(a.ldx >= 0 && a.ldw >= 0 && a.ldr >= 0 && a.ldo >= 0 && a.x_scale_row >= 0 &&
              a.x_scale_blk >= 0 && a.weight_scale_row >= 0 && a.weight_scale_blk >= 0,
          "linear: negative stride");
+  MI_ARG(a.M <= 1 || a.ldo >= a.N, "linear: rows of out overlap");
   MI_ARG(!fp8 || a.K % 128 == 0, "linear: K must be divisible by 128 for float8 operands");
   return MI355MOE_OK;
 }
@@ -287,6 +289,8 @@ extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
   const int splits = path == TILE ? linear_tile_splits(a) : any_splits(a);
   MI_CHECK(splits == 1 || (workspace && workspace_bytes >= lin_partials(a, splits)),
            MI355MOE_ERR_WORKSPACE, "linear: workspace too small");
+  MI_ARG(splits == 1 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+         "linear: workspace must be 16-byte aligned");
   // a split product leaves fp32 partial sums of all weight rows
   LinArgs b = a;
   if (splits > 1) {

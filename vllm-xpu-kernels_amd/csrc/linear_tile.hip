@@ -507,6 +507,7 @@ constexpr Tile kTiles16[] = {
 constexpr Tile kTiles8[] = {
     {128, 256, 1, 1.45f}, {128, 128, 2, 1.73f}, {128, 128, 1, 1.08f}, {64, 128, 1, 0.68f}};
 constexpr int kMaxSplits = 16;
+constexpr int kMaxSplitTiles = 1 << 16;  // workgroups of a split product: far more than fill the CUs
 
 struct Plan {
   int tile, splits, per;  // stages per split
@@ -534,6 +535,7 @@ Plan plan(const LinArgs& a) {
       // a split product runs without gates, over all weight rows
       const double tiles = static_cast<double>(cdiv(a.M, c.bm)) *
                            cdiv(s > 1 ? lin_rows(a) : a.N, g && s == 1 ? c.bn / 2 : c.bn) * s;
+      if (s > 1 && tiles > kMaxSplitTiles) continue;
       const double slots = 256.0 * c.per_cu;
       const double rounds = tiles <= 256 && c.per_cu > 1 ? 0.62 : __builtin_ceil(tiles / slots);
       double us = rounds * (c.us * (exact ? 2 : 1) * per + 3.0);
@@ -597,8 +599,8 @@ bool linear_tile_supported(const LinArgs& a) {
         blocks * a.weight_scale_row * 4 >= lim || a.weight_scale_blk * 4 >= lim)
       return false;
   }
-  // tiles and splits are counted in 32 bits
-  return cdiv(a.M, 64) * cdiv(lin_rows(a), 64) * kMaxSplits < (int64_t(1) << 22);
+  // a grid's threads (256 to a tile of 64 rows of x) stay below 2^32
+  return cdiv(a.M, 64) * cdiv(lin_rows(a), 64) < (int64_t(1) << 24);
 }
 
 int linear_tile_splits(const LinArgs& a) { return plan(a).splits; }

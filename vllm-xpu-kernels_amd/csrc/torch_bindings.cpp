@@ -747,23 +747,28 @@ bool float16or32(const at::Tensor& t) {
          t.scalar_type() == at::kHalf;
 }
 
-// Row strides of [.., cols] with contiguous columns: 1-D to 3-D as they are,
-// more leading dimensions where they fold into one stride.
+// Row strides of [.., cols] with contiguous columns: the last leading dimension
+// is the inner one, those before it fold into one stride (dimensions of one
+// element have none).
 struct Rows {
   int64_t outer = 0, inner = 0;
 };
 Rows rows_of(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
-  Rows r;
   const int64_t d = t.dim();
   for (int64_t i = 0; i + 1 < d; ++i) TORCH_CHECK(t.stride(i) >= 0, name, " has a negative stride");
-  if (d >= 2) r.inner = t.stride(d - 2);
-  if (d == 2) r = {t.stride(0), 0};
-  if (d >= 3) {
-    r.outer = t.stride(d - 3);
-    for (int64_t i = d - 4; i >= 0; --i)
-      TORCH_CHECK(t.size(i) <= 1 || t.stride(i) == t.stride(i + 1) * t.size(i + 1), name,
-                  " has leading dimensions that do not fold into one");
+  if (d == 2) return {t.stride(0), 0};
+  Rows r;
+  if (d >= 3) r.inner = t.stride(d - 2);
+  bool set = false;
+  int64_t want = 0;
+  for (int64_t i = d - 3; i >= 0; --i) {
+    if (t.size(i) <= 1) continue;
+    if (!set) r.outer = t.stride(i);
+    else
+      TORCH_CHECK(t.stride(i) == want, name, " has leading dimensions that do not fold into one");
+    want = t.stride(i) * t.size(i);
+    set = true;
   }
   return r;
 }

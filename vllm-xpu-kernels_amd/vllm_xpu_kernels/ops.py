@@ -324,6 +324,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                                    scale_ue8m0, is_scale_transposed))
     if residual is None:
         raise ValueError("residual_out needs a residual")
+    if group_size not in (32, 64, 128):
+        raise ValueError(f"group_size must be 32, 64, or 128, got {group_size}")
     q, scales, *norm = _rms_norm_outputs(x, group_size, scale_dtype, is_scale_transposed, with_norm)
     _rms_norm(norm[0] if norm else None, q, scales, residual_out, x, weight, residual, eps,
               group_size, scale_ue8m0)

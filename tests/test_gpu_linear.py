@@ -460,3 +460,27 @@ def test_linear_many_tiles(dev, act):
     for m in (0, 131001, M - 70):
         r = slice(m, m + 70)
         _close(out[r], *_want(x[r].double(), w.double(), None, act, None))
+
+
+# sizes whose tiles differ: few or many rows against the same weight, K of one step,
+# a few, an odd end, and long enough to be split; ragged edges
+TILES = [(250, 40, 4090), (250, 72, 4090), (250, 1032, 4090), (61, 4104, 4096), (700, 40, 4090),
+         (700, 72, 4096), (700, 1032, 4090), (1003, 520, 2881), (1500, 72, 4090), (1500, 1032, 4096),
+         (2047, 264, 2050), (1003, 1032, 4095)]
+
+
+@pytest.mark.parametrize("M,K,N", TILES)
+def test_linear_tiles(dev, M, K, N):
+    _case(M, K, N, "bf16", bias="bf16", residual="bf16", seed=40)
+    _case(M, K, N, "fp16", "silu_and_mul", bias="fp16", seed=50)
+    if K < 100:
+        test_values_that_do_not_count_stay_out(dev, M, K, N)
+
+
+@pytest.mark.parametrize("M,K,N", [(250, 128, 4090), (250, 1152, 4090), (120, 1024, 7170), (61, 4096, 4096),
+                                   (250, 1152, 2049), (700, 1152, 4090), (700, 384, 4090), (1500, 256, 4090),
+                                   (1500, 1152, 4090), (2047, 384, 2050), (300, 2048, 776)])
+def test_linear_fp8_tiles(dev, M, K, N):
+    _fp8_case(M, K, N, bias="bf16", residual="bf16", seed=40)
+    _fp8_case(M, K, N, "silu_and_mul", seed=50)
+    _fp8_case(M, K, N, "gelu_and_mul", out="fp32", seed=60)

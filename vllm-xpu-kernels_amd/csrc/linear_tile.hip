@@ -107,7 +107,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
   constexpr int SC = FP8 ? (BM + BN) / 64 : 0;   // scale copies of a stage
   constexpr int SPER = (SC + WAVES - 1) / WAVES;
   constexpr int ND = PER + SPER;
-  constexpr int EM = 64;                         // rows of x per pass of the epilogue
+  constexpr int EM = BM % 64 ? 32 : 64;          // rows of x per pass of the epilogue
   constexpr int EP = BN + 4;                     // its pitch in floats
   constexpr int LDS = NSTAGE * STAGE > EM * EP * 4 ? NSTAGE * STAGE : EM * EP * 4;
   static_assert(LDS <= 160 * 1024, "LDS");
@@ -378,6 +378,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
             for (int r = 0; r < 4; ++r) acc[i][j][r] += d[e & 1][r] * (xs[j % 3] * ws[i][r]);
           }
         };
+        constexpr int CPM = (ND + MT * NT - 1) / (MT * NT);  // copies behind an MFMA
         for_each<MT>([&](auto jc) __attribute__((always_inline)) {
           constexpr int j = decltype(jc)::value;
           if constexpr (j + 1 < MT) {
@@ -393,10 +394,13 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
                 w[i], x[j & 1], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 127, 0, 127);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (Q > 0) add(std::integral_constant<int, Q - 1>{});
-            if constexpr (Q < ND) {
+            if constexpr (Q * CPM < ND) {
               if (dma) {
-                if constexpr (Q < PER) copy(std::integral_constant<int, Q>{}, koff, nslot, false);
-                else copy_scale(Q - PER, kn, nslot);
+                for_each<CPM>([&](auto cc) __attribute__((always_inline)) {
+                  constexpr int C = Q * CPM + decltype(cc)::value;
+                  if constexpr (C < PER) copy(std::integral_constant<int, C>{}, koff, nslot, false);
+                  else if constexpr (C < ND) copy_scale(C - PER, kn, nslot);
+                });
               }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -490,27 +494,43 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
 }
 
 // The tiles that calls choose from.  us: time of one stage (128 bytes of K) on
-// every CU at once; per_cu: workgroups of the tile that a CU holds.
+// every CU at once; per_cu: workgroups of the tile that a CU holds; gated: takes
+// both halves of a gated weight (a split product needs no gates; 16-bit 64 x 64
+// with two waves of 32 x 64 gained nothing there, 200 x 2048 x 768 13.4 -> 14.9).
+enum Shape { T256X256, T128X256, T128X128X2, T128X128, T96X128, T64X128, T64X64 };
 struct Tile {
+  Shape shape;
   int bm, bn, per_cu;
+  bool gated;
   float us;
 };
-// Measured at 8192 x 4096 x 4096 / 2048 x 4096 x 4096 / 1003 x 4096 x 4096 / 400 x
-// 4096 x 4096 (242 / 77 / 46 / 31 us).  256 x 256: 8 waves of 128 x 64 and two
-// stages (four of 64 bytes: 5 % slower; 4 waves of 128 x 128: alike); two
-// workgroups of 128 x 128 per CU hide each other's epilogues, one with four
-// stages hides the latency where tiles are few.
+// 16-bit.  256 x 256: 8 waves of 128 x 64 and two stages (four of 64 bytes: 5 %
+// slower; 4 waves of 128 x 128: alike).  Two workgroups of 128 x 128 per CU hide
+// each other's epilogues, one with four stages hides the latency where tiles are
+// few.  The others fill the CUs where these leave some idle (us, K = 4096 unless
+// said, best of the others after it): 128 x 256 1500 x 4096 65 / 69, 2048 x 2048
+// gated 71 / 77; 96 x 128 1003 x 2880 x 2880 30.6 / 34.9, 700 x 4096 39.6 / 41.8;
+// 64 x 64, eight stages, 250 x 4096 24.4 / 31.5 (64 x 128), 61 x 4096 split by 4
+// 16.5 / 17.1 (64 x 128 by 8).
 constexpr Tile kTiles16[] = {
-    {256, 256, 1, 1.78f}, {128, 128, 2, 1.16f}, {128, 128, 1, 0.66f}, {64, 128, 1, 0.43f}};
-// e4m3 at 8192 x / 2048 x / 1003 x / 400 x 4096 x 4096 (210 / 59 / 40 / 25 us): 256 x
-// 256 leaves no registers for the scaled sums (spills, 288 us).
+    {T256X256, 256, 256, 1, true, 1.85f}, {T128X256, 128, 256, 1, true, 1.14f},
+    {T128X128X2, 128, 128, 2, true, 1.16f}, {T128X128, 128, 128, 1, true, 0.66f},
+    {T96X128, 96, 128, 1, false, 0.555f}, {T64X128, 64, 128, 1, true, 0.42f},
+    {T64X64, 64, 64, 1, false, 0.31f}};
+// e4m3.  256 x 256 leaves no registers for the scaled sums (spills: 8192 x 4096 x
+// 4096 288 us, 128 x 256 210); 96 rows are no whole copies of scales.  64 x 64: 250 x
+// 4096 x 4096 18.8 us (64 x 128 24.9), 61 x 2048 x 7168 12.4 (16.1), 250 x 4096 x 2048
+// gated 18.2 (24.6).
 constexpr Tile kTiles8[] = {
-    {128, 256, 1, 1.45f}, {128, 128, 2, 1.73f}, {128, 128, 1, 1.08f}, {64, 128, 1, 0.68f}};
+    {T128X256, 128, 256, 1, true, 1.45f}, {T128X128X2, 128, 128, 2, true, 1.73f},
+    {T128X128, 128, 128, 1, true, 1.08f}, {T64X128, 64, 128, 1, true, 0.70f},
+    {T64X64, 64, 64, 1, true, 0.44f}};
 constexpr int kMaxSplits = 16;
 constexpr int kMaxSplitTiles = 1 << 16;  // workgroups of a split product: far more than fill the CUs
 
 struct Plan {
-  int tile, splits, per;  // stages per split
+  Shape shape;
+  int splits, per;  // stages per split
 };
 
 // 16 weight rows from a multiple of 16 share a scale block
@@ -518,34 +538,37 @@ bool uniform_scales(const LinArgs& a) { return !lin_gated(a.activation) || a.N %
 
 // The tile and the split of K with the least estimated time: rounds of the
 // grid over the CUs, each its stages and 3 us around them, and for a split the
-// partial sums written and read at 5 TB/s and a second launch.
+// partial sums written and read at 3.5 TB/s and a second launch.
 Plan plan(const LinArgs& a) {
   const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
   const bool exact = fp8 && a.out_dtype == MI355MOE_F32;
   const int nk = static_cast<int>(cdiv(a.K * (fp8 ? 1 : 2), 128));
   const bool g = lin_gated(a.activation);
   const double rows = static_cast<double>(lin_rows(a));
-  Plan best{-1, 1, nk};
-  double best_us = 0;
-  for (int t = 0; t < 4; ++t) {
-    const Tile& c = fp8 ? kTiles8[t] : kTiles16[t];
+  Plan best{};
+  double best_us = -1;
+  auto look = [&](const Tile& c) {
     for (int s = 1; s <= kMaxSplits; ++s) {
       const int per = static_cast<int>(cdiv(nk, s));
       if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
-      // a split product runs without gates, over all weight rows
+      const bool gates = g && s == 1;  // a split product: all weight rows, no gates
+      if (gates && !c.gated) continue;
       const double tiles = static_cast<double>(cdiv(a.M, c.bm)) *
-                           cdiv(s > 1 ? lin_rows(a) : a.N, g && s == 1 ? c.bn / 2 : c.bn) * s;
+                           cdiv(gates ? a.N : lin_rows(a), gates ? c.bn / 2 : c.bn) * s;
       if (s > 1 && tiles > kMaxSplitTiles) continue;
-      const double slots = 256.0 * c.per_cu;
-      const double rounds = tiles <= 256 && c.per_cu > 1 ? 0.62 : __builtin_ceil(tiles / slots);
+      const double rounds = __builtin_ceil(tiles / (256.0 * c.per_cu));
       double us = rounds * (c.us * (exact ? 2 : 1) * per + 3.0);
-      if (s > 1) us += 4.0 + 2.0 * s * a.M * rows * 4 / 5e6;
-      if (best.tile < 0 || us < best_us) {
-        best = {t, s, per};
+      if (s > 1) us += 4.0 + 2.0 * s * a.M * rows * 4 / 3.5e6;
+      if (best_us < 0 || us < best_us) {
+        best = {c.shape, s, per};
         best_us = us;
       }
     }
-  }
+  };
+  if (fp8)
+    for (const Tile& c : kTiles8) look(c);
+  else
+    for (const Tile& c : kTiles16) look(c);
   return best;
 }
 
@@ -559,24 +582,27 @@ int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
   return MI355MOE_OK;
 }
 
+template <int KIND, bool GATED, int BM, int BN, int WM, int WN, int NSTAGE>
+int launch_uni(const LinArgs& a, const Plan& p, hipStream_t st) {
+  if constexpr (KIND >= K_FP8)
+    if (!uniform_scales(a)) return launch<KIND, GATED, false, BM, BN, WM, WN, NSTAGE>(a, p, st);
+  return launch<KIND, GATED, true, BM, BN, WM, WN, NSTAGE>(a, p, st);
+}
+
 template <int KIND, bool GATED>
 int launch_tiles(const LinArgs& a, const Plan& p, hipStream_t st) {
-  constexpr bool FP8 = KIND >= K_FP8;
-  const bool uni = !FP8 || uniform_scales(a);
-  switch (p.tile) {
-    case 0:
-      if constexpr (!FP8) return launch<KIND, GATED, true, 256, 256, 2, 4, 2>(a, p, st);
-      else return uni ? launch<KIND, GATED, true, 128, 256, 2, 4, 3>(a, p, st)
-                      : launch<KIND, GATED, false, 128, 256, 2, 4, 3>(a, p, st);
-    case 1:
-      return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 2>(a, p, st)
-                 : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 2>(a, p, st);
-    case 2:
-      return uni ? launch<KIND, GATED, true, 128, 128, 2, 2, 4>(a, p, st)
-                 : launch<KIND, GATED, !FP8, 128, 128, 2, 2, 4>(a, p, st);
-    default:
-      return uni ? launch<KIND, GATED, true, 64, 128, 2, 2, 4>(a, p, st)
-                 : launch<KIND, GATED, !FP8, 64, 128, 2, 2, 4>(a, p, st);
+  if constexpr (KIND < K_FP8) {
+    if (p.shape == T256X256) return launch_uni<KIND, GATED, 256, 256, 2, 4, 2>(a, p, st);
+    if constexpr (!GATED)
+      if (p.shape == T96X128) return launch_uni<KIND, GATED, 96, 128, 1, 4, 4>(a, p, st);
+  }
+  if constexpr (KIND >= K_FP8 || !GATED)
+    if (p.shape == T64X64) return launch_uni<KIND, GATED, 64, 64, 2, 2, 8>(a, p, st);
+  switch (p.shape) {
+    case T128X256: return launch_uni<KIND, GATED, 128, 256, 2, 4, 3>(a, p, st);
+    case T128X128X2: return launch_uni<KIND, GATED, 128, 128, 2, 2, 2>(a, p, st);
+    case T128X128: return launch_uni<KIND, GATED, 128, 128, 2, 2, 4>(a, p, st);
+    default: return launch_uni<KIND, GATED, 64, 128, 2, 2, 4>(a, p, st);
   }
 }
 

@@ -484,3 +484,21 @@ def test_linear_fp8_tiles(dev, M, K, N):
     _fp8_case(M, K, N, bias="bf16", residual="bf16", seed=40)
     _fp8_case(M, K, N, "silu_and_mul", seed=50)
     _fp8_case(M, K, N, "gelu_and_mul", out="fp32", seed=60)
+
+
+@pytest.mark.parametrize("M,K,N", [(8, 4160, 1030), (9, 4160, 1030), (16, 7168, 264), (16, 4096, 1030),
+                                   (17, 2048, 1540), (32, 2048, 3070), (33, 2048, 1540), (64, 2048, 1536)])
+def test_linear_between_few_rows_and_tiles(dev, M, K, N):
+    """Sizes on both sides of the rule that leaves rows to the streaming kernels."""
+    _case(M, K, N, "bf16", "silu_and_mul", residual="fp16", seed=80)
+    _case(M, K, N, "fp16", bias="fp32", out="fp32", seed=90)
+    # rows that start anywhere
+    x, w = _rand((M, K + 3), torch.bfloat16, 81), _rand((N, K + 1), torch.bfloat16, 82, 1 / math.sqrt(K))
+    _close(_ops().linear(x[:, 1:K + 1], w[:, 1:]), *_want(x[:, 1:K + 1].double(), w[:, 1:].double(), None, None, None))
+
+
+@pytest.mark.parametrize("M,K,N", [(4, 7168, 2400), (5, 7168, 2400), (8, 4224, 1030), (9, 4224, 1030),
+                                   (16, 4096, 1030), (32, 2048, 3070), (33, 2048, 1540)])
+def test_linear_fp8_between_few_rows_and_tiles(dev, M, K, N):
+    _fp8_case(M, K, N, "gelu_tanh_and_mul", residual="bf16", seed=80)
+    _fp8_case(M, K, N, bias="bf16", out="fp32", seed=90)

@@ -197,8 +197,8 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
   }
 }
 
-// few rows of x (linear_skinny.hip), any alignment
-bool linear_skinny_takes(const LinArgs& a);
+// few rows of x (linear_skinny.hip), any alignment; tile: the tiles can take them too
+bool linear_skinny_takes(const LinArgs& a, bool tile);
 int launch_linear_skinny(const LinArgs& a, hipStream_t st);
 // more rows (linear_tile.hip).  a0: the call; a: the same, or with a split K the
 // product of all weight rows into fp32 partial sums [splits][M][rows]

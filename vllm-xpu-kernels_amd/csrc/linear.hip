@@ -274,8 +274,9 @@ size_t lin_partials(const LinArgs& a, int splits) {
 }
 enum Path { SKINNY, TILE, ANY };
 Path path_of(const LinArgs& a) {
-  if (linear_skinny_takes(a)) return SKINNY;
-  return linear_tile_supported(a) ? TILE : ANY;
+  const bool tile = linear_tile_supported(a);
+  if (linear_skinny_takes(a, tile)) return SKINNY;
+  return tile ? TILE : ANY;
 }
 }  // namespace
 

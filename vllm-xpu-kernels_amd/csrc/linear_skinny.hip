@@ -260,14 +260,22 @@ int launch_rows(const LinArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// Up to 16 rows of x; up to 64 where the weight is small (its tiles would leave
-// most CUs idle: 61 x 7168 x 256 12.6 us against 14.2, 61 x 2048 x 1536 8.8
-// against 12.5; 61 x 4096 x 4096 22 against 16.7).
-bool linear_skinny_takes(const LinArgs& a) {
+// Rows of x that the stream takes.  Its waves walk K, so a long K and many rows
+// go to the tiles, which split it (skinny / tile us: 8 x 7168 x 2048 11.9 / 12.1 e4m3,
+// 13.6 / 13.4 bf16; 16 x 7168 x 256 11.9 / 9.5, 12.1 / 10.3; 16 x 7168 x 7168 22.9 / 18.0,
+// 33.4 / 24.4; 16 x 4096 x 4096 9.2 / 12.1, 12.2 / 13.5); e4m3 products of large
+// weights from 5 rows on (8 x 7168 x 4096 gated 16.5 / 13.7, 4 rows 12.5 / 13.6).  Past 16
+// rows it streams the weight once per 16: for weights that leave the tiles
+// short of work (32 x 2048 x 1536 gated 7.0 / 9.6 and 9.7 / 12.0, 61 x 2048 x
+// 1536 8.1 / 9.8 and 10.8 / 10.4; 32 x 2816 x 2816 11.9 / 9.9 and 15.2 / 12.4).
+// Rows that the tiles cannot fetch (`tile` false): any K, and small weights.
+bool linear_skinny_takes(const LinArgs& a, bool tile) {
   const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
   if (fp8 && (a.K / 128) * 48 * 4 > kScaleBytes) return false;  // scales beyond their LDS
-  const int64_t rows = lin_rows(a);
-  return a.M <= 16 || (a.M <= 64 && (rows * a.K <= (int64_t(4) << 20)));
+  const int64_t weight = lin_rows(a) * a.K;
+  if (!tile) return a.M <= 16 || (a.M <= 64 && weight <= (int64_t(4) << 20));
+  if (a.K > 4096) return a.M <= (fp8 && weight > (int64_t(16) << 20) ? 4 : 8);
+  return a.M <= 16 || (a.M <= 64 && cdiv(a.M, 16) * weight <= (int64_t(12) << 20));
 }
 
 int launch_linear_skinny(const LinArgs& a, hipStream_t st) {

@@ -245,7 +245,7 @@ int launch(const LinArgs& a, int waves, hipStream_t st) {
 // 26.0, 16 x 4096 x 4096 12.2 against 15.1) and stage e4m3 scales once per 16 rows
 // (4 x 2048 x 7168 7.6 against 8.5).  More waves per strip shorten the walk over a
 // long K and lengthen the sum at its end (1 x 7168 x 7168 with 1 / 2 / 4 waves 21.0 /
-// 21.9 / 23.4, e4m3 1 x 7168 x 4096 gated 19.1 / 13.9 / 11.7).
+// 21.9 / 23.4, e4m3 1 x 7168 x 4096 gated 19.1 / 13.9 / 11.7, before GUARD).
 template <bool FP8, bool F16, bool GATED>
 int launch_rows(const LinArgs& a, hipStream_t st) {
   const bool few = a.N <= 2048;  // at most 128 strips of 16
@@ -270,7 +270,7 @@ int launch_rows(const LinArgs& a, hipStream_t st) {
 // go to the tiles, which split it (skinny / tile us: 8 x 7168 x 2048 11.9 / 12.1 e4m3,
 // 13.6 / 13.4 bf16; 16 x 7168 x 256 11.9 / 9.5, 12.1 / 10.3; 16 x 7168 x 7168 22.9 / 18.0,
 // 33.4 / 24.4; 16 x 4096 x 4096 9.2 / 12.1, 12.2 / 13.5); e4m3 products of large
-// weights from 5 rows on (8 x 7168 x 4096 gated 16.5 / 13.7, 4 rows 12.5 / 13.6).  Past 16
+// weights from 5 rows on (8 x 7168 x 4096 gated 16.5 / 13.7, 4 rows 10.9 / 13.6).  Past 16
 // rows it streams the weight once per 16: for weights that leave the tiles
 // short of work (32 x 2048 x 1536 gated 7.0 / 9.6 and 9.7 / 12.0, 61 x 2048 x
 // 1536 8.1 / 9.8 and 10.8 / 10.4; 32 x 2816 x 2816 11.9 / 9.9 and 15.2 / 12.4).

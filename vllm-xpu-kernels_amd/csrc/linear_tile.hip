@@ -44,13 +44,14 @@ __device__ __forceinline__ uint32_t lds_off(const void* p) {
 }
 // 16 / 4 bytes per lane from sbase + voff (scalar base, 32-bit lane offset) into
 // LDS at lds_base + OFF + 16 (4) lane
+// (s_nop: M0 takes one wait state from its write to the copy that reads it)
 template <int OFF>
 __device__ __forceinline__ void dma16(uint32_t voff, uint64_t sbase, uint32_t lds_base) {
-  asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :: "v"(voff), "s"(sbase), "s"(lds_base), "n"(OFF) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void dma4(uint32_t voff, uint64_t sbase, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                :: "v"(voff), "s"(sbase), "s"(lds_base) : "memory", "m0");
 }
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) {

@@ -69,12 +69,13 @@ __device__ __forceinline__ uint32_t lds_off(const void* p) {
 }
 // 16 (dma16) or 4 (dma4) bytes per lane from sbase + voff (scalar base,
 // 32-bit lane offset) into LDS at lds_base + 16 lane (4 lane).
+// (s_nop: M0 takes one wait state from its write to the copy that reads it)
 __device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :: "v"(voff), "s"(reinterpret_cast<uint64_t>(sbase)), "s"(lds_base) : "memory", "m0");
 }
 __device__ __forceinline__ void dma4(uint32_t voff, const void* sbase, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                :: "v"(voff), "s"(reinterpret_cast<uint64_t>(sbase)), "s"(lds_base) : "memory", "m0");
 }
 // readfirstlane returns int: each half goes through uint32_t so that the low

@@ -404,7 +404,9 @@ int mi355moe_silu_and_mul_mxfp4_quant(uint8_t* out, const void* input, int in_dt
  * of y stays NaN in q and does not count in its group's maximum; a group
  * with an infinite y has an infinite scale (e8m0: NaN), zeros, and NaN there.
  * Squares that overflow fp32 (|h| > 1.8e19) may give y = 0, as the formula
- * does in fp32; power-of-two scales are decided in 64 bits.
+ * does in fp32.  A power-of-two scale is the least that is no less than a / 448
+ * in 64 bits, where a / 448 up to 1 + 2^-40 times a power of two counts as
+ * that power.
  *
  * Rows: row r of x, residual, residual_out and out starts at element
  * (r / inner) * outer_stride + (r % inner) * inner_stride of its pointer

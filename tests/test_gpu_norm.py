@@ -312,3 +312,49 @@ def test_rms_norm_leading_dimensions_of_one(dev):
         assert torch.equal(got, want) and torch.equal(r, wr)
     with pytest.raises(RuntimeError, match="do not fold"):
         _ops().rms_norm(buf[:, :2].unsqueeze(2).expand(6, 2, 2, 3, 64), w, EPS)
+
+
+def _border_case(T, H, dtype, c, group, seed):
+    """Rows of +-c under eps 0, so that y = +-weight exactly; the groups' largest weights at
+    448 * 2^e, one float32 step (2^-23.8 of it) below and above it, or 1.5 times it.  -> x, weight,
+    power-of-two scales"""
+    g = torch.Generator().manual_seed(seed)
+    n = H // group
+    e = torch.randint(-6, 4, (n,), generator=g).double()
+    off = torch.tensor([0.0, -2.0 ** -21, 2.0 ** -21, 3.5])[torch.randint(0, 4, (n,), generator=g)].double()
+    top = 64.0 * torch.exp2(e) * (7 + off)
+    w = top.unsqueeze(1) * (0.25 + 0.5 * torch.rand(n, group, generator=g).double())
+    w[torch.arange(n), torch.randint(0, group, (n,), generator=g)] = top
+    sign = torch.randint(0, 2, (T, H), generator=g) * 2.0 - 1
+    x = (sign * c).to(DT[dtype])
+    assert bool((x.double().abs() == c).all()) and bool((w.float().double().amax(1) == top).all())
+    return x.cuda(), w.view(H).float().cuda(), torch.exp2(e + (off > 0)).cuda()
+
+
+@pytest.mark.parametrize("group,kind", [(32, "e8m0"), (64, "ue8m0"), (128, "e8m0"), (128, "ue8m0")])
+@pytest.mark.parametrize("H", [96, 384, 512, 768, 896, 2816, 2880, 4096, 6144, 7168, 33280, 40000])
+def test_rms_norm_scales_at_powers_of_two(dev, H, group, kind):
+    """A power-of-two scale is the least that is no less than max / 448, on the border and one step
+    to either side of it, where fp32 cannot tell: not one group may double or halve.  Squares far from
+    1 (their fp32 root is coarser than the border) among them."""
+    H = max(H // group, 1) * group
+    for i, (dtype, c) in enumerate([("bf16", 1.0), ("fp16", 1.5703125), ("fp32", 0.8515625),
+                                    ("bf16", 1.5703125 * 2.0 ** 54), ("fp32", 1.2265625 * 2.0 ** -54)]):
+        x, w, want = _border_case(7, H, dtype, c, group, 100 * i + H)
+        sdt = torch.float8_e8m0fnu if kind == "e8m0" else torch.float32
+        for res in (None, torch.zeros_like(x)):
+            got = _ops().rms_norm_quant(x, w, 0.0, residual=res, group_size=group, scale_dtype=sdt,
+                                        scale_ue8m0=kind == "ue8m0")
+            s = got[1].double()
+            assert torch.equal(s, want.expand_as(s)), (dtype, c, int((s != want).sum()))
+
+
+def test_rms_norm_scales_at_powers_of_two_any_alignment(dev):
+    """The same where rows start anywhere."""
+    for H, group in ((384, 32), (2880, 64), (4096, 128)):
+        x, w, want = _border_case(9, H, "bf16", 1.5703125, group, H)
+        buf = torch.zeros(9, H + 5, dtype=x.dtype, device=dev)
+        buf[:, 3:H + 3] = x
+        s = _ops().rms_norm_quant(buf[:, 3:H + 3], w, 0.0, group_size=group,
+                                  scale_dtype=torch.float8_e8m0fnu)[1].double()
+        assert torch.equal(s, want.expand_as(s))

@@ -101,12 +101,15 @@ __device__ __forceinline__ bool pow2_scales(const NormArgs& a) {
 // G / 8 consecutive, aligned lanes; every lane of the wave takes part, those
 // without columns (`active` false) with zeros.
 // Power-of-two scales double where the maximum passes 448 2^e: a maximum within
-// 2^-20 of that (fp32's error is below) is formed again in 64 bits from h, the
-// weight and rsd, the root's reciprocal in 64 bits.
+// 2^-20 of that (fp32's error is below) is compared in 64 bits, as squares and
+// without a root or division:  |h w| / sqrt(ss / cols + eps) <= 448 2^e  where
+// (h w)^2 cols <= (448 2^e)^2 (ss + eps cols).  The sides are off by a few 2^-53
+// each; 2^-39 of slack (2^-40 of the maximum, which the clamp takes off its
+// code) leaves a maximum that the formula puts on the border below it.
 template <bool VEC>
 __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int i, bool active,
                                        const float (&y)[8], const float (&h)[8],
-                                       const float (&w)[8], double rsd, bool nt) {
+                                       const float (&w)[8], double ss, bool nt) {
   float amax = 1e-10f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(y[k]));
@@ -128,9 +131,10 @@ __device__ __forceinline__ void quant8(const NormArgs& a, int64_t r, int i, bool
     if (low != high) {  // the same in all lanes of a group
       double m = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmax(m, fabs(static_cast<double>(h[k]) * w[k] * rsd));
+      for (int k = 0; k < 8; ++k) m = fmax(m, fabs(static_cast<double>(h[k]) * w[k]));
       for (int o = 1; o < (group >> 3); o <<= 1) m = fmax(m, __shfl_xor(m, o, 64));
-      ex = m / 448.0 <= ldexp(1.0, low) ? low : high;
+      const double n = static_cast<double>(a.cols), t = ldexp(448.0, low);
+      ex = m * m * n <= t * t * (1.0 + 0x1p-39) * (ss + a.eps * n) ? low : high;
     }
     s = ex > 127 ? __uint_as_float(0x7F800000u) : pow2i(ex);  // an infinite maximum
   }
@@ -187,8 +191,8 @@ __device__ __forceinline__ T row_sum(const float (&h)[R][8], int lanes) {
 }
 
 // 1 / sqrt(ss / cols + eps): fp32's values with one Newton step each in 64 bits
-// (about 2^-46; the 64-bit division and root take 0.5 us of a small call)
-__device__ __forceinline__ double rsqrt64(double ss, int cols, float eps) {
+// before the rounding (the 64-bit division and root take 0.5 us of a small call)
+__device__ __forceinline__ float rsqrt_mean(double ss, int cols, float eps) {
   const double r0 = 1.0f / static_cast<float>(cols);  // cols < 2^24 is exact, above off by 2^-24
   const double inv = r0 * (2.0 - static_cast<double>(cols) * r0);
   const double v = ss * inv + eps;
@@ -196,7 +200,7 @@ __device__ __forceinline__ double rsqrt64(double ss, int cols, float eps) {
   // zero, infinite and NaN roots, and those whose square leaves fp32, stand
   if (!(v > 1e-30 && v < 1e30)) return s0;
   const double s = s0;
-  return s * (1.5 - 0.5 * v * s * s);
+  return static_cast<float>(s * (1.5 - 0.5 * v * s * s));
 }
 
 // LANES: lanes of a row inside a wave (8 to 64, 256 / LANES rows to a
@@ -250,10 +254,10 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void rms_norm_kernel(const Norm
     }
   }
   float rs;
-  double rsd = 0;
+  double ss = 0;  // where a border needs it
   if (QUANT && pow2_scales(a)) {  // uniform
-    rsd = rsqrt64(row_sum<double, LANES, R>(h, lanes), cols, a.eps);
-    rs = static_cast<float>(rsd);
+    ss = row_sum<double, LANES, R>(h, lanes);
+    rs = rsqrt_mean(ss, cols, a.eps);
   } else {
     rs = 1.0f / sqrtf(row_sum<float, LANES, R>(h, lanes) / static_cast<float>(cols) + a.eps);
   }
@@ -271,7 +275,7 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void rms_norm_kernel(const Norm
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = h[c][k] * rs * w[c][k];
     if (out && on[c]) store8<E, VEC>(out, i, cols, y, nt, step);
-    if constexpr (QUANT) quant8<VEC>(a, rr, i, on[c], y, h[c], w[c], rsd, nt);
+    if constexpr (QUANT) quant8<VEC>(a, rr, i, on[c], y, h[c], w[c], ss, nt);
   }
 }
 
@@ -301,8 +305,8 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a, i
 #pragma unroll
     for (int k = 0; k < 8; ++k) ss += static_cast<double>(h[k]) * h[k];
   }
-  const double rsd = rsqrt64(workgroup_sum(ss, 16), static_cast<int>(a.cols), a.eps);
-  const float rs = static_cast<float>(rsd);
+  ss = workgroup_sum(ss, 16);
+  const float rs = rsqrt_mean(ss, static_cast<int>(a.cols), a.eps);
   for (int64_t i0 = 0; i0 < a.cols; i0 += 1024 * 8) {  // uniform: groups exchange maxima
     const int64_t i = i0 + threadIdx.x * 8;
     const bool on = i < a.cols;
@@ -321,7 +325,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a, i
     if (on && a.out)
       store8<E, VEC>(static_cast<char*>(a.out) + row_at<E>(r, a.inner, a.out_outer, a.out_inner),
                      i, a.cols, y, nt);
-    if (a.q) quant8<VEC>(a, r, static_cast<int>(on ? i : 0), on, y, h, w, rsd, nt);
+    if (a.q) quant8<VEC>(a, r, static_cast<int>(on ? i : 0), on, y, h, w, ss, nt);
   }
 }
 

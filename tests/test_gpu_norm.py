@@ -358,3 +358,28 @@ def test_rms_norm_scales_at_powers_of_two_any_alignment(dev):
         s = _ops().rms_norm_quant(buf[:, 3:H + 3], w, 0.0, group_size=group,
                                   scale_dtype=torch.float8_e8m0fnu)[1].double()
         assert torch.equal(s, want.expand_as(s))
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_rms_norm_more_rows_than_one_launch(dev, quant):
+    """Launches take 2^21 rows each: the rows behind the first launch's, whole."""
+    T, H = (1 << 21) + 37, 32
+    x, r = _rand((T, H), torch.bfloat16, 71), _rand((T, H), torch.bfloat16, 72)
+    w = _rand((H,), torch.bfloat16, 73) + 1
+    if quant:
+        q, s, n, ro = _ops().rms_norm_quant(x, w, EPS, residual=r, group_size=32, with_norm=True)
+    else:
+        n, ro = _ops().rms_norm(x, w, EPS, residual=r)
+    for a in (0, (1 << 21) - 100, T - 1000):
+        i = slice(a, a + 1000)
+        h, y = _exact(x[i], w, r[i])
+        _close(n[i], y)
+        _close(ro[i], h, 2.0 ** -24)
+        if quant:
+            _check_quant(q[i], s[i].double(), y, 32, False)
+    # 16 columns, several rows to a wave, without a residual
+    x = _rand((T, 16), torch.bfloat16, 74)
+    w = _rand((16,), torch.bfloat16, 75) + 1
+    out = _ops().rms_norm(x, w, EPS)
+    for a in (0, (1 << 21) - 100, T - 1000):
+        _close(out[a:a + 1000], _exact(x[a:a + 1000], w)[1])

@@ -169,3 +169,79 @@ def test_rms_norm_quant_refuses_groups(group):
     x = torch.zeros(2, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="group_size must be 32, 64, or 128"):
         ops.rms_norm_quant(x, x[0], residual=x, residual_out=x, group_size=group)
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype, device="meta")
+
+
+def _calls(ops, t):
+    """Every wrapper, with `t` (a function of the argument's name) choosing each tensor."""
+    yield "rms_norm", ("x", "weight", "residual", "residual_out", "out"), lambda: ops.rms_norm(
+        t("x", 2, 128), t("weight", 128), residual=t("residual", 2, 128),
+        residual_out=t("residual_out", 2, 128), out=t("out", 2, 128))
+    yield "rms_norm_quant", ("x", "weight", "residual", "residual_out"), lambda: ops.rms_norm_quant(
+        t("x", 2, 128), t("weight", 128), residual=t("residual", 2, 128),
+        residual_out=t("residual_out", 2, 128))
+    yield "linear", ("x", "weight", "bias", "residual", "out"), lambda: ops.linear(
+        t("x", 2, 128), t("weight", 8, 128), t("bias", 8), residual=t("residual", 2, 8), out=t("out", 2, 8))
+    f8 = torch.float8_e4m3fn
+    yield "linear_fp8", ("x", "x_scale", "weight", "weight_scale", "bias", "residual", "out"), \
+        lambda: ops.linear_fp8(
+            t("x", 2, 128, dtype=f8), t("x_scale", 2, 1, dtype=torch.float32),
+            t("weight", 8, 128, dtype=f8), t("weight_scale", 1, 1, dtype=torch.float32), t("bias", 8),
+            residual=t("residual", 2, 8), out=t("out", 2, 8))
+
+
+def test_wrappers_refuse_every_tensor_that_needs_a_gradient():
+    """Inputs and given outputs alike, e4m3 codes cast from a tensor with a gradient too; without
+    gradients the same calls run."""
+    from vllm_xpu_kernels import ops
+    chosen = [None]
+
+    def t(name, *shape, dtype=torch.bfloat16):
+        if name != chosen[0]:
+            return _meta(*shape, dtype=dtype)
+        return _meta(*shape, dtype=torch.float32).requires_grad_().to(dtype) if dtype != torch.float32 \
+            else _meta(*shape, dtype=dtype).requires_grad_()
+
+    for op, names, call in _calls(ops, t):
+        chosen[0] = None
+        call()
+        for n in names:
+            chosen[0] = n
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad():
+                call()
+
+
+def test_wrappers_refuse_forward_mode_duals():
+    """A tangent would be lost, under no_grad too (it does not end forward mode)."""
+    import torch.autograd.forward_ad as fw
+    from vllm_xpu_kernels import ops
+    chosen = [None]
+
+    def t(name, *shape, dtype=torch.bfloat16):
+        v = _meta(*shape, dtype=dtype)
+        return fw.make_dual(v, _meta(*shape, dtype=dtype)) if name == chosen[0] else v
+
+    with fw.dual_level():
+        for op, names, call in _calls(ops, t):
+            chosen[0] = None
+            call()
+            for n in names:
+                chosen[0] = n
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    call()
+                with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                    call()
+
+
+def test_wrappers_refuse_function_transforms():
+    from vllm_xpu_kernels import ops
+    w, x = _meta(8, 128), _meta(2, 128)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.func.grad(lambda v: ops.linear(v, w).float().sum())(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.func.jvp(lambda v: ops.linear(v, w), (x,), (x,))

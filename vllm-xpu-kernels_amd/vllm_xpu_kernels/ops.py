@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ops  # noqa: F401
 
@@ -265,10 +266,14 @@ def silu_and_mul_mxfp4_quant(input: torch.Tensor, group_size: int = 32,
 
 
 def _no_grad_needed(*tensors) -> None:
-    """The operators below have no backward pass: refuse to lose a gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("this operator has no gradient: call it under torch.no_grad() or "
-                           "detach its inputs")
+    """The operators below have no derivative: refuse to lose a gradient of an
+    input, to write a given output that has one, and to lose a tangent (which
+    no_grad does not end)."""
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or (
+            forward_ad._current_level >= 0 and
+            any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
+        raise RuntimeError("this operator has no gradient: detach its tensors, or call it under "
+                           "torch.no_grad() where no tangent is asked for")
 
 
 _rms_norm = torch.ops._mi355_C.rms_norm.default
@@ -290,7 +295,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     weight [H] of x's type or float32.  Returns out, with a residual
     (out, h).  h is written to residual_out, which may be residual itself
     (in place); out may be x."""
-    _no_grad_needed(x, weight, residual)
+    _no_grad_needed(x, weight, residual, residual_out, out)
     if out is None and residual_out is None:
         got = _rms_norm_new(x, weight, residual, eps)
         return got[0] if residual is None else (got[0], got[1])
@@ -318,7 +323,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     (q, scales [rows, H / group_size]), then the norm in x's type
     (with_norm: the router's input), then the new residual (with a residual).
     The scales are a transposed view when is_scale_transposed."""
-    _no_grad_needed(x, weight, residual)
+    _no_grad_needed(x, weight, residual, residual_out)
     if residual_out is None:
         return tuple(_rms_norm_new(x, weight, residual, eps, with_norm, group_size, scale_dtype,
                                    scale_ue8m0, is_scale_transposed))
@@ -374,7 +379,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     "gelu_tanh", "relu2", or a gated one, "silu_and_mul", "gelu_and_mul",
     "gelu_tanh_and_mul": f of the first half of the weight rows' results
     times the second half's, N / 2 columns.  out may be residual (in place)."""
-    _no_grad_needed(x, weight, bias, residual)
+    _no_grad_needed(x, weight, bias, residual, out)
     return _run_linear(x, None, weight, None, bias, activation, residual, out_dtype, out, x.dtype)
 
 
@@ -389,7 +394,7 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     layer's block-scaled recipe).  K % 128 == 0.  out_dtype: bfloat16 by
     default, float16 or float32 (whose sums have fp32's precision; 16-bit
     outputs may use the e4m3 matrix instruction, 1.5e-5 coarser)."""
-    _no_grad_needed(x_scale, weight_scale, bias, residual)
+    _no_grad_needed(x, x_scale, weight, weight_scale, bias, residual, out)
     return _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
                        torch.bfloat16)
 

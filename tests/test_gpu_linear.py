@@ -502,3 +502,31 @@ def test_linear_between_few_rows_and_tiles(dev, M, K, N):
 def test_linear_fp8_between_few_rows_and_tiles(dev, M, K, N):
     _fp8_case(M, K, N, "gelu_tanh_and_mul", residual="bf16", seed=80)
     _fp8_case(M, K, N, bias="bf16", out="fp32", seed=90)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 7168, 256), (1, 128, 40), (3, 2048, 300), (4, 384, 4100), (7, 7168, 72),
+                                   (8, 2048, 1030), (16, 4096, 576), (16, 1152, 4100), (61, 4096, 512),
+                                   (300, 1152, 520)])
+def test_linear_fp8_infinite_scales(dev, M, K, N):
+    """A block whose scale is infinite makes its rows' (columns') sums infinite, not NaN, wherever
+    it lies in K; the others stay."""
+    one = torch.ones(max(M, 2 * N), K, device=dev).to(torch.float8_e4m3fn)
+    blocks = K // 128
+    for at in {0, blocks // 2, blocks - 1}:
+        for act in (None, "silu_and_mul"):
+            rows = 2 * N if act else N
+            xs = torch.full((M, blocks), 2.0 ** -4, device=dev)
+            ws = torch.full(((rows + 127) // 128, blocks), 2.0 ** -4, device=dev)
+            want = _ops().linear_fp8(one[:M], xs, one[:rows], ws, activation=act)
+            assert bool(want.isfinite().all())
+            x2 = xs.clone()
+            x2[M - 1, at] = float("inf")
+            got = _ops().linear_fp8(one[:M], x2, one[:rows], ws, activation=act)
+            assert bool((got[M - 1] == float("inf")).all()) and torch.equal(got[:M - 1], want[:M - 1])
+            w2 = ws.clone()
+            w2[-1, at] = float("inf")      # the last block of weight rows
+            got = _ops().linear_fp8(one[:M], xs, one[:rows], w2, activation=act)
+            inf = torch.arange(N, device=dev) + (N if act else 0) >= (rows - 1) // 128 * 128
+            if act:                        # the gate's rows that share the block
+                inf |= torch.arange(N, device=dev) >= (rows - 1) // 128 * 128
+            assert bool((got[:, inf] == float("inf")).all()) and torch.equal(got[:, ~inf], want[:, ~inf])

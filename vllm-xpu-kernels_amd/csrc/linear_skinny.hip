@@ -87,26 +87,28 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   };
 
   // e4m3: scales of the strips' rows and of the group's rows of x, all K blocks:
-  // s_ws[kb][strip][row], s_xs[kb][group row]
+  // s_ws[kb][strip][row], s_xs[kb][group row]; block `kblocks` of zeros is for chunks
+  // that were cleared (0 times an infinite scale would be NaN)
   const int kblocks = FP8 ? static_cast<int>(a.K / 128) : 0;
   float* s_ws = lds;
-  float* s_xs = s_ws + (FP8 ? kblocks * NS * R : 0);
-  float* red = s_xs + (FP8 ? kblocks * MT * R : 0);
+  float* s_xs = s_ws + (FP8 ? (kblocks + 1) * NS * R : 0);
+  float* red = s_xs + (FP8 ? (kblocks + 1) * MT * R : 0);
 
   const bool any = s0 < s1;  // uniform per wave
   if (any) load(w0, x0, s0);
   if constexpr (FP8) {
-    for (int i = tid; i < kblocks * NS * R; i += blockDim.x) {
+    for (int i = tid; i < (kblocks + 1) * NS * R; i += blockDim.x) {
       const int kb = i / (NS * R), s = (i / R) % NS, r = i % R;
       int64_t n = n0 + r;
       n = (n < a.N ? n : a.N - 1) + s * a.N;
-      s_ws[i] = a.weight_scale[(n / 128) * a.weight_scale_row + kb * a.weight_scale_blk];
+      s_ws[i] = kb < kblocks ? a.weight_scale[(n / 128) * a.weight_scale_row + kb * a.weight_scale_blk]
+                             : 0.f;
     }
-    for (int i = tid; i < kblocks * MT * R; i += blockDim.x) {
+    for (int i = tid; i < (kblocks + 1) * MT * R; i += blockDim.x) {
       const int kb = i / (MT * R);
       int64_t m = mbase + i % (MT * R);
       m = m < a.M ? m : a.M - 1;
-      s_xs[i] = a.x_scale[m * a.x_scale_row + kb * a.x_scale_blk];
+      s_xs[i] = kb < kblocks ? a.x_scale[m * a.x_scale_row + kb * a.x_scale_blk] : 0.f;
     }
     __syncthreads();
   }
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
         xb[j][1] = fp8x8_to16<false, false>(make_uint2(x[j].z, x[j].w));
       }
       const int kr = (s * STEP + co * 64) / 128;  // K block of the lane's results
-      const int kb = kr < kblocks ? kr : kblocks - 1;
+      const int kb = s < s1 && kr < kblocks ? kr : kblocks;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const uint4 wa = fp8x8_to16<false, false>(make_uint2(w[i].x, w[i].y));
@@ -229,9 +231,9 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
 template <bool FP8, bool F16, bool GATED, int R, int MT, int U>
 int launch(const LinArgs& a, int waves, hipStream_t st) {
   constexpr int NS = GATED ? 2 : 1;
-  const int64_t kblocks = FP8 ? a.K / 128 : 0;
-  // at most 48 KiB of scales (linear_skinny_takes) and 8 KiB of sums
-  const size_t lds = 4 * (kblocks * (NS + MT) * R + static_cast<size_t>(waves) * NS * MT * 16 * R);
+  const int64_t blocks = FP8 ? a.K / 128 + 1 : 0;
+  // at most 48 KiB of scales (linear_skinny_takes), a block of zeros and 8 KiB of sums
+  const size_t lds = 4 * (blocks * (NS + MT) * R + static_cast<size_t>(waves) * NS * MT * 16 * R);
   const dim3 grid(static_cast<unsigned>(cdiv(a.N, R)), static_cast<unsigned>(cdiv(a.M, R * MT)));
   linear_skinny_kernel<FP8, F16, GATED, R, MT, U><<<grid, dim3(64 * waves), lds, st>>>(a);
   MI_LAUNCH_CHECK();

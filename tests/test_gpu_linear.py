@@ -530,3 +530,33 @@ def test_linear_fp8_infinite_scales(dev, M, K, N):
             if act:                        # the gate's rows that share the block
                 inf |= torch.arange(N, device=dev) >= (rows - 1) // 128 * 128
             assert bool((got[:, inf] == float("inf")).all()) and torch.equal(got[:, ~inf], want[:, ~inf])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu2", "silu_and_mul", "gelu_and_mul",
+                                 "gelu_tanh_and_mul"])
+@pytest.mark.parametrize("M,K,N", [(1, 64, 8), (40, 512, 96), (61, 4096, 512), (300, 264, 200), (300, 77, 19)])
+def test_linear_activations_of_infinity(dev, M, K, N, act):
+    """Infinite sums: the formulas' values in fp32.  +inf stays; -inf times a factor that is 0 there is
+    NaN (x sigmoid(x), x (1 + erf) and x (1 + tanh) alike), relu2 gives 0.  Finite neighbours stay."""
+    inf = float("inf")
+    gated = act.endswith("_and_mul")
+    x = _rand((M, K), torch.bfloat16, 1)
+    w = _rand((2 * N if gated else N, K), torch.bfloat16, 2, 1 / math.sqrt(K))
+    b = torch.zeros(w.shape[0], device=dev)
+    b[1], b[2] = inf, -inf
+    if gated:
+        b[N:] = 30.0                       # the factor: positive
+    got = _ops().linear(x, w, b, act, out_dtype=torch.float32)
+    assert bool((got[:, 1] == inf).all())
+    assert bool((got[:, 2] == 0).all()) if act == "relu2" else bool(got[:, 2].isnan().all())
+    keep = torch.arange(N, device=dev) > 2
+    y, e = _want(x.double(), w.double(), b, act, None)
+    _close(got[:, keep], y[:, keep], e[:, keep])
+    # an infinite value of x reaches its row through the product, with the weight's sign
+    x[M - 1, K - 1] = inf
+    w[:, K - 1] = 1.0
+    w[3, K - 1] = -1.0
+    got = _ops().linear(x, w, None, act, out_dtype=torch.float32)
+    other = torch.arange(N, device=dev) != 3
+    assert bool((got[M - 1, other] == inf).all()) and bool(got[:M - 1].isfinite().all())
+    assert bool(got[M - 1, 3] == 0) if act == "relu2" else bool(got[M - 1, 3].isnan())

@@ -47,8 +47,9 @@ __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
 }
 
 // f of the activation (gated ones: f of the gate).  x sigmoid(k x) with the
-// hardware exp2 and reciprocal (about 1 ulp each): k x -> -inf gives x *
-// rcp(inf) = -0, k x -> +inf gives x.  SiLU is k = 1; the tanh form of GELU is
+// hardware exp2 and reciprocal (about 1 ulp each): a finite x whose exp2
+// overflows gives x * rcp(inf) = -0, one whose exp2 vanishes gives x; x = inf
+// stays, x = -inf is -inf * 0 = NaN, as x / (1 + exp(-x)) is.  SiLU is k = 1; the tanh form of GELU is
 // exactly x sigmoid(2 t), t = sqrt(2/pi) (x + 0.044715 x^3), since (1 + tanh t) / 2
 // = sigmoid(2 t); it takes 8 instructions instead of tanhf's 40.
 __device__ __forceinline__ float mul_sigmoid(float x, float t) {

@@ -526,6 +526,12 @@ constexpr Tile kTiles8[] = {
     {T128X256, 128, 256, 1, true, 1.45f}, {T128X128X2, 128, 128, 2, true, 1.73f},
     {T128X128, 128, 128, 1, true, 1.08f}, {T64X128, 64, 128, 1, true, 0.70f},
     {T64X64, 64, 64, 1, true, 0.44f}};
+// e4m3 with float32 outputs (EXACT): the bf16 fragments take the registers of two
+// workgroups per CU (276 to 304 of a lane's 512), so 128 x 128 with two stages runs
+// alone there, and no slower than with four (1.32 and 1.39 us a stage).
+constexpr Tile kTiles8Exact[] = {
+    {T128X256, 128, 256, 1, true, 1.94f}, {T128X128X2, 128, 128, 1, true, 1.32f},
+    {T64X128, 64, 128, 1, true, 0.85f}, {T64X64, 64, 64, 1, true, 0.59f}};
 constexpr int kMaxSplits = 16;
 constexpr int kMaxSplitTiles = 1 << 16;  // workgroups of a split product: far more than fill the CUs
 
@@ -558,7 +564,7 @@ Plan plan(const LinArgs& a) {
                            cdiv(gates ? a.N : lin_rows(a), gates ? c.bn / 2 : c.bn) * s;
       if (s > 1 && tiles > kMaxSplitTiles) continue;
       const double rounds = __builtin_ceil(tiles / (256.0 * c.per_cu));
-      double us = rounds * (c.us * (exact ? 2 : 1) * per + 3.0);
+      double us = rounds * (c.us * per + 3.0);
       if (s > 1) us += 4.0 + 2.0 * s * a.M * rows * 4 / 3.5e6;
       if (best_us < 0 || us < best_us) {
         best = {c.shape, s, per};
@@ -566,7 +572,9 @@ Plan plan(const LinArgs& a) {
       }
     }
   };
-  if (fp8)
+  if (exact)
+    for (const Tile& c : kTiles8Exact) look(c);
+  else if (fp8)
     for (const Tile& c : kTiles8) look(c);
   else
     for (const Tile& c : kTiles16) look(c);
@@ -599,10 +607,11 @@ int launch_tiles(const LinArgs& a, const Plan& p, hipStream_t st) {
   }
   if constexpr (KIND >= K_FP8 || !GATED)
     if (p.shape == T64X64) return launch_uni<KIND, GATED, 64, 64, 2, 2, 8>(a, p, st);
+  if constexpr (KIND != K_FP8_EXACT)
+    if (p.shape == T128X128) return launch_uni<KIND, GATED, 128, 128, 2, 2, 4>(a, p, st);
   switch (p.shape) {
     case T128X256: return launch_uni<KIND, GATED, 128, 256, 2, 4, 3>(a, p, st);
     case T128X128X2: return launch_uni<KIND, GATED, 128, 128, 2, 2, 2>(a, p, st);
-    case T128X128: return launch_uni<KIND, GATED, 128, 128, 2, 2, 4>(a, p, st);
     default: return launch_uni<KIND, GATED, 64, 128, 2, 2, 4>(a, p, st);
   }
 }

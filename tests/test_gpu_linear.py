@@ -560,3 +560,26 @@ def test_linear_activations_of_infinity(dev, M, K, N, act):
     other = torch.arange(N, device=dev) != 3
     assert bool((got[M - 1, other] == inf).all()) and bool(got[:M - 1].isfinite().all())
     assert bool(got[M - 1, 3] == 0) if act == "relu2" else bool(got[M - 1, 3].isnan())
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 7168, 256), (4, 4224, 72), (16, 4096, 96), (61, 4096, 512), (250, 1152, 520),
+                                   (700, 1152, 1024), (1500, 512, 2048)])
+def test_linear_fp8_sums_under_cancellation(dev, M, K, N):
+    """Among 8 consecutive k one product of +-2^8, the sign alternating from 8 to 8, and seven of 2^-6:
+    float32 outputs are the small products' exact sum whatever kernel runs; 16-bit outputs are within
+    7 * 2^-13 of the largest product for each 8 consecutive k (and fp32's and the output's rounding)."""
+    k = torch.arange(K, device=dev)
+    x = torch.where(k % 8 == 0, torch.where(k // 8 % 2 == 0, 16.0, -16.0), 0.125)
+    w = torch.where(k % 8 == 0, 16.0, 0.125)
+    xq = x.expand(M, K).contiguous().to(torch.float8_e4m3fn)
+    wq = w.expand(N, K).contiguous().to(torch.float8_e4m3fn)
+    xs = torch.ones(M, K // 128, device=dev)
+    ws = torch.ones((N + 127) // 128, K // 128, device=dev)
+    want = 7 * 2.0 ** -6 * (K // 8)
+    exact = _ops().linear_fp8(xq, xs, wq, ws, out_dtype=torch.float32)
+    # every partial sum is a multiple of 2^-6 below 2^9 (a wave's or a split's too): no rounding at all
+    assert bool((exact == want).all()), float((exact - want).abs().max())
+    for dt in (torch.bfloat16, torch.float16):
+        got = _ops().linear_fp8(xq, xs, wq, ws, out_dtype=dt).double()
+        lim = (7 * 2.0 ** -13 * 256 * (K // 8)) * (1 + torch.finfo(dt).eps) + torch.finfo(dt).eps / 2 * want
+        assert bool(((got - want).abs() <= lim).all())

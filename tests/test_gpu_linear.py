@@ -583,3 +583,64 @@ def test_linear_fp8_sums_under_cancellation(dev, M, K, N):
         got = _ops().linear_fp8(xq, xs, wq, ws, out_dtype=dt).double()
         lim = (7 * 2.0 ** -13 * 256 * (K // 8)) * (1 + torch.finfo(dt).eps) + torch.finfo(dt).eps / 2 * want
         assert bool(((got - want).abs() <= lim).all())
+
+
+def test_linear_into_other_columns_of_a_batch(dev):
+    """out and residual beside x in the rows of one buffer, with several leading dimensions."""
+    K, N = 256, 96
+    w = _rand((N, K), torch.bfloat16, 1, 0.06)
+    for lead in ((5,), (2, 3), (2, 3, 4)):
+        buf = _rand(lead + (K + 2 * N + 8,), torch.bfloat16, 2)
+        before = buf.clone()
+        x, r, out = buf[..., :K], buf[..., K:K + N], buf[..., K + N:K + 2 * N]
+        want = _ops().linear(before[..., :K].contiguous(), w, residual=before[..., K:K + N].contiguous())
+        _ops().linear(x, w, residual=r, out=out)
+        assert torch.equal(out, want)
+        assert torch.equal(buf[..., :K + N], before[..., :K + N])
+        assert torch.equal(buf[..., K + 2 * N:], before[..., K + 2 * N:])
+        with pytest.raises(RuntimeError, match="out must not overlap input"):
+            _ops().linear(x, w, out=buf[..., K - 1:K - 1 + N])
+        with pytest.raises(RuntimeError, match="out must not overlap residual"):
+            _ops().linear(x, w, residual=r, out=buf[..., K + N - 1:K + 2 * N - 1])
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 256, 48), (3, 7168, 40), (10, 384, 100), (61, 1152, 520), (300, 512, 200),
+                                   (1100, 256, 1030)])
+@pytest.mark.parametrize("out", ["bf16", "fp32"])
+def test_linear_fp8_nan_codes(dev, M, K, N, out):
+    """A NaN code or scale reaches its own row or column only."""
+    nan = float("nan")
+    xq, xs, wq, ws = _fp8_inputs(M, K, N, N, 5)
+    want = _ops().linear_fp8(xq, xs, wq, ws, out_dtype=DT[out])
+    xb = xq.view(torch.uint8).clone()
+    xb[M - 1, K - 1] = 0x7F
+    got = _ops().linear_fp8(xb.view(xq.dtype), xs, wq, ws, out_dtype=DT[out])
+    assert bool(got[M - 1].isnan().all()) and torch.equal(got[:M - 1], want[:M - 1])
+    wb = wq.view(torch.uint8).clone()
+    wb[N // 2, 0] = 0xFF
+    got = _ops().linear_fp8(xq, xs, wb.view(xq.dtype), ws, out_dtype=DT[out])
+    keep = torch.arange(N, device=dev) != N // 2
+    assert bool(got[:, N // 2].isnan().all()) and torch.equal(got[:, keep], want[:, keep])
+    x2 = xs.clone()
+    x2[0, K // 128 - 1] = nan
+    got = _ops().linear_fp8(xq, x2, wq, ws, out_dtype=DT[out])
+    assert bool(got[0].isnan().all()) and torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 256, 48), (5, 1000, 96), (17, 4096, 512), (61, 4096, 96), (61, 77, 33),
+                                   (250, 512, 4090), (1003, 512, 2881)])
+def test_linear_writes_no_row_behind_its_last(dev, M, K, N):
+    for kind in ("bf16", "fp8"):
+        if kind == "fp8" and K % 128:
+            continue
+        buf = torch.full((M + 260, N), 7.0, dtype=torch.bfloat16, device=dev)
+        if kind == "bf16":
+            x, w = _rand((M, K), torch.bfloat16, 1), _rand((N, K), torch.bfloat16, 2, 1 / math.sqrt(K))
+            want = _ops().linear(x, w)
+            _ops().linear(x, w, out=buf[1:M + 1])
+        else:
+            ins = _fp8_inputs(M, K, N, N, 5)
+            want = _ops().linear_fp8(*ins)
+            _ops().linear_fp8(*ins, out=buf[1:M + 1])
+        assert torch.equal(buf[1:M + 1], want)
+        assert bool((buf[0] == 7).all()) and bool((buf[M + 1:] == 7).all())

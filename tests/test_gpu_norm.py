@@ -383,3 +383,20 @@ def test_rms_norm_more_rows_than_one_launch(dev, quant):
     out = _ops().rms_norm(x, w, EPS)
     for a in (0, (1 << 21) - 100, T - 1000):
         _close(out[a:a + 1000], _exact(x[a:a + 1000], w)[1])
+
+
+def test_rms_norm_into_other_heads_of_a_batch(dev):
+    """Outputs between the inputs' rows, of any number of leading dimensions that fold: no overlap."""
+    w = _rand((64,), torch.bfloat16, 81) + 1
+    packed = _rand((2, 3, 10, 64), torch.bfloat16, 82)
+    before = packed.clone()
+    want, wr = _ops().rms_norm(before[:, :, :4].contiguous(), w, EPS, residual=before[:, :, :4].contiguous())
+    got, r = _ops().rms_norm(packed[:, :, :4], w, EPS, residual=packed[:, :, :4],
+                             residual_out=packed[:, :, :4], out=packed[:, :, 5:9])
+    assert torch.equal(packed[:, :, 5:9], want) and torch.equal(packed[:, :, :4], wr)
+    assert torch.equal(packed[:, :, 4], before[:, :, 4]) and torch.equal(packed[:, :, 9], before[:, :, 9])
+    # heads that do meet, of one and of several leading dimensions
+    for p in (packed, packed[0], packed.view(6, 10, 64)):
+        for a, b in ((slice(0, 4), slice(3, 7)), (slice(2, 6), slice(0, 4))):
+            with pytest.raises(RuntimeError, match="out must not overlap"):
+                _ops().rms_norm(p[..., a, :], w, EPS, out=p[..., b, :])

@@ -714,17 +714,31 @@ std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
   for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
   return {p, p + static_cast<uintptr_t>(last + 1) * t.element_size()};
 }
+// Rows of one stride: (row stride, width) in bytes of the outermost dimension once those
+// that fold into one are folded; the tensor's bytes lie in [0, width) of every row.
+std::pair<int64_t, int64_t> folded_rows(const at::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> s;  // (stride, size), the outermost last
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) > 0) s.emplace_back(t.stride(i), t.size(i));
+  std::sort(s.begin(), s.end());
+  size_t n = 0;
+  for (size_t i = 1; i < s.size(); ++i)
+    if (s[i].first == s[n].first * s[n].second) s[n].second *= s[i].second;
+    else s[++n] = s[i];
+  int64_t width = 1;
+  for (size_t i = 0; i < n; ++i) width += s[i].first * (s[i].second - 1);
+  const int64_t size = static_cast<int64_t>(t.element_size());
+  return {s.empty() ? 0 : s[n].first * size, width * size};
+}
 // rows of one stride whose columns lie apart: both tensors step through memory
 // by the same row stride, and within it their rows' bytes do not meet (a head
 // range of a packed projection beside another)
 bool interleaved_apart(const at::Tensor& a, const at::Tensor& b) {
-  if (a.dim() < 2 || b.dim() < 2) return false;
-  const int64_t row = a.stride(0) * static_cast<int64_t>(a.element_size());
-  if (row <= 0 || row != b.stride(0) * static_cast<int64_t>(b.element_size())) return false;
-  const auto x = extent(a.select(0, 0)), y = extent(b.select(0, 0));
-  const int64_t wa = static_cast<int64_t>(x.second - x.first);
-  const int64_t wb = static_cast<int64_t>(y.second - y.first);
-  int64_t d = static_cast<int64_t>(y.first) - static_cast<int64_t>(x.first);
+  const auto [row, wa] = folded_rows(a);
+  const auto [rowb, wb] = folded_rows(b);
+  if (row <= 0 || row != rowb) return false;
+  int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()) -
+                                   reinterpret_cast<uintptr_t>(a.data_ptr()));
   d = ((d % row) + row) % row;
   return d >= wa && d + wb <= row;
 }

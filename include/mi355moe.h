@@ -415,7 +415,7 @@ int mi355moe_silu_and_mul_mxfp4_quant(uint8_t* out, const void* input, int in_dt
  * scale of (row r, group g) is at element r * scale_row + g * scale_group.
  * out and residual_out may each be x or residual (same pointer and strides)
  * but not the same of them; otherwise no output may overlap an input or
- * another output. */
+ * another output, nor one of its rows another. */
 typedef struct {
   int dtype;          /* F32, BF16 or F16: x, residual, residual_out, out     */
   int weight_dtype;   /* dtype, or F32                                        */
@@ -455,13 +455,17 @@ typedef enum {
 
 /* Matrix product with bias, activation and residual in its epilogue (no
  * counterpart among the reference's MoE ops: the router's logits and the
- * dense products beside the experts).  fp32 accumulation, one rounding:
+ * dense products beside the experts).  fp32 accumulation (but see below), one
+ * rounding:
  *   z[m, n] = sum_k x[m, k] weight[n, k] + bias[n]
  *   out[m, n] = T(act(z)[m, n] + residual[m, n]),  0 <= n < N;
  * gated activations: act(z)[m, n] = f(z[m, n]) * z[m, N + n].
  * x_dtype BF16 or F16: weight of the same type.  x_dtype FP8E4M3: weight
  * e4m3, K % 128 == 0, z[m, n] = sum over 128-blocks b of K of
- * x_scale[m, b] * weight_scale[n / 128, b] * sum_{k in b} x[m, k] weight[n, k].
+ * x_scale[m, b] * weight_scale[n / 128, b] * sum_{k in b} x[m, k] weight[n, k];
+ * with a BF16 or F16 output that inner sum may lose, for each 8 consecutive k,
+ * up to 7 * 2^-13 of their largest product towards zero (the e4m3 matrix
+ * instruction's), with an F32 output it has fp32's precision.
  * Row strides ld* and scale strides are in elements; columns of x, weight,
  * bias, residual and out are contiguous.  M may be 0; N and K are positive.
  * out may be residual with the same stride and type; otherwise it may overlap

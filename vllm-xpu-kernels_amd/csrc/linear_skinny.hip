@@ -166,10 +166,11 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
       product(w[u], x[u], s + u);
     }
   };
-  // GUARD: no loads behind the range.  Narrow gated e4m3 strips gain (3 x 7168 x 2048
-  // 12.2 -> 10.8 us, 1 x 2048 x 1536 7.2 -> 5.4); the branches cost the others
-  // more than the loads, which hit the caches (bf16 1 x 7168 x 256 5.3 -> 5.7, 8 x 7168 x
-  // 2048 gated 16.1 -> 18.1).
+  // GUARD: no loads behind the range.  Narrow gated e4m3 strips gain (us, kernels
+  // alone, without / with: 3 x 7168 x 4096 15.0 / 11.1, 4 x 4096 x 4096 13.7 / 8.2, 4 x
+  // 2048 x 4096 7.4 / 6.2, 1 x 2048 x 1536 5.5 / 4.7, 4 x 7168 x 2048 8.5 / 8.5; 2 x 2816 x
+  // 2560 loses, 6.8 / 7.4); the branches cost the others more than the loads, which
+  // hit the caches (bf16 1 x 7168 x 256 5.3 -> 5.7, 8 x 7168 x 4096 gated 16.1 -> 18.1).
   constexpr bool GUARD = FP8 && GATED && R * MT == 4;
   if (any) {
     for (int s = s0; s < s1; s += 2 * U) {
@@ -241,7 +242,8 @@ int launch(const LinArgs& a, int waves, hipStream_t st) {
 }
 
 // Strip height and waves, from sweeps over all of them at 1 to 48 rows of the
-// products below.  Strips of 4 or 8 rows win while strips of 16 leave CUs
+// products below (here and above: rows x K x weight rows, both halves of a gated
+// weight counted).  Strips of 4 or 8 rows win while strips of 16 leave CUs
 // without work (16-bit, 8 rows, 7168 x 4096 gated: 4-row strips 16.0 us, 16-row
 // 24.0); strips of 16 read x a quarter as often (4 x 7168 x 7168 23.8 against
 // 26.0, 16 x 4096 x 4096 12.2 against 15.1) and stage e4m3 scales once per 16 rows

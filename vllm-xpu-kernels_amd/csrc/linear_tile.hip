@@ -497,7 +497,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
 // The tiles that calls choose from.  us: time of one stage (128 bytes of K) on
 // every CU at once; per_cu: workgroups of the tile that a CU holds; gated: takes
 // both halves of a gated weight (a split product needs no gates; 16-bit 64 x 64
-// with two waves of 32 x 64 gained nothing there, 200 x 2048 x 768 13.4 -> 14.9).
+// with two waves of 32 x 64 gained nothing there, 200 x 2048 x 1536 13.4 -> 14.9).
 enum Shape { T256X256, T128X256, T128X128X2, T128X128, T96X128, T64X128, T64X64 };
 struct Tile {
   Shape shape;
@@ -505,11 +505,13 @@ struct Tile {
   bool gated;
   float us;
 };
+// (Sizes: rows x K x weight rows, both halves of a gated weight counted.)
 // 16-bit.  256 x 256: 8 waves of 128 x 64 and two stages (four of 64 bytes: 5 %
-// slower; 4 waves of 128 x 128: alike).  Two workgroups of 128 x 128 per CU hide
+// slower; 4 waves of 128 x 128: alike); 26 (gated) and 70 registers are spilled, once
+// behind the K loop, for the epilogue.  Two workgroups of 128 x 128 per CU hide
 // each other's epilogues, one with four stages hides the latency where tiles are
 // few.  The others fill the CUs where these leave some idle (us, K = 4096 unless
-// said, best of the others after it): 128 x 256 1500 x 4096 65 / 69, 2048 x 2048
+// said, best of the others after it): 128 x 256 1500 x 4096 65 / 69, 2048 x 4096
 // gated 71 / 77; 96 x 128 1003 x 2880 x 2880 30.6 / 34.9, 700 x 4096 39.6 / 41.8;
 // 64 x 64, eight stages, 250 x 4096 24.4 / 31.5 (64 x 128), 61 x 4096 split by 4
 // 16.5 / 17.1 (64 x 128 by 8).
@@ -520,7 +522,7 @@ constexpr Tile kTiles16[] = {
     {T64X64, 64, 64, 1, false, 0.31f}};
 // e4m3.  256 x 256 leaves no registers for the scaled sums (spills: 8192 x 4096 x
 // 4096 288 us, 128 x 256 210); 96 rows are no whole copies of scales.  64 x 64: 250 x
-// 4096 x 4096 18.8 us (64 x 128 24.9), 61 x 2048 x 7168 12.4 (16.1), 250 x 4096 x 2048
+// 4096 x 4096 18.8 us (64 x 128 24.9), 61 x 2048 x 7168 12.4 (16.1), 250 x 4096 x 4096
 // gated 18.2 (24.6).
 constexpr Tile kTiles8[] = {
     {T128X256, 128, 256, 1, true, 1.45f}, {T128X128X2, 128, 128, 2, true, 1.73f},

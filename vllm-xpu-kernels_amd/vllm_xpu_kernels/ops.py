@@ -395,7 +395,7 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     default, float16 or float32.  float32 outputs have fp32's sums whatever the
     batch; 16-bit outputs may use the e4m3 matrix instruction (from 5 to 65 rows
     on, by the weight), which takes up to 7 * 2^-13 of the largest product off
-    every 8 consecutive k: 1.5e-5 of a normal result, more where products cancel."""
+    every 8 consecutive k: 2e-5 of a normal result, more where products cancel."""
     _no_grad_needed(x, x_scale, weight, weight_scale, bias, residual, out)
     return _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
                        torch.bfloat16)

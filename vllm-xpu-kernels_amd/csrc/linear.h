@@ -22,6 +22,10 @@
 // the time.  Tiles use the e4m3 MFMA for 16-bit outputs and convert for float32
 // outputs; the kernels that stream weights (bound by the stream) and the one for any
 // alignment always convert.
+//
+// int8 products.  Sums of 8-bit products are int32 and exact (K < 2^17: 2^17 products
+// of -128 reach 2^31), so a result is the same whichever kernel, tile or split made
+// it:  z[m, n] = float(sum) * (x_scale[m] * weight_scale[n]) + bias[n].
 #pragma once
 
 #include <type_traits>
@@ -31,6 +35,21 @@
 namespace mi355 {
 
 typedef mi355moe_linear_args LinArgs;
+typedef int lin_i32x4 __attribute__((ext_vector_type(4)));
+
+// operands of a kernel; K_FP8_EXACT: e4m3 with the bf16 MFMA's sums
+enum { K_BF16 = 0, K_F16 = 1, K_FP8 = 2, K_FP8_EXACT = 3, K_I8 = 4 };
+constexpr __host__ __device__ bool kind_fp8(int kind) { return kind == K_FP8 || kind == K_FP8_EXACT; }
+constexpr __host__ __device__ int kind_bytes(int kind) { return kind == K_BF16 || kind == K_F16 ? 2 : 1; }
+inline int kind_of(const LinArgs& a) {
+  return a.x_dtype == MI355MOE_FP8E4M3 ? K_FP8 : a.x_dtype == MI355MOE_I8 ? K_I8
+         : a.x_dtype == MI355MOE_F16 ? K_F16 : K_BF16;
+}
+// a kernel's sums: int32 of int8 products, else float
+template <int KIND, int N>
+struct SumVec { typedef float T __attribute__((ext_vector_type(N))); };
+template <int N>
+struct SumVec<K_I8, N> { typedef int T __attribute__((ext_vector_type(N))); };
 
 __host__ __device__ constexpr bool lin_gated(int act) {
   return act >= MI355MOE_LINEAR_SILU_AND_MUL;
@@ -48,6 +67,33 @@ __device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
 __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
   if (dtype == MI355MOE_F32) static_cast<float*>(p)[i] = v;
   else static_cast<uint16_t*>(p)[i] = dtype == MI355MOE_BF16 ? f32_to_bf16(v) : f32_to_f16(v);
+}
+
+// K step of 16 bytes per lane: 16 rows x 16 columns (32 16-bit or 64 8-bit k) ...
+template <int KIND>
+__device__ __forceinline__ typename SumVec<KIND, 4>::T mfma_16x16(uint4 a, uint4 b,
+                                                                  typename SumVec<KIND, 4>::T c) {
+  if constexpr (KIND == K_I8)
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(lin_i32x4, a),
+                                                 __builtin_bit_cast(lin_i32x4, b), c, 0, 0, 0);
+  else return mfma16_16x16x32<KIND == K_F16>(a, b, c);
+}
+// ... and 32 x 32 (16 16-bit or 32 8-bit k)
+template <int KIND>
+__device__ __forceinline__ typename SumVec<KIND, 16>::T mfma_32x32(uint4 a, uint4 b,
+                                                                   typename SumVec<KIND, 16>::T c) {
+  if constexpr (KIND == K_I8)
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(lin_i32x4, a),
+                                                 __builtin_bit_cast(lin_i32x4, b), c, 0, 0, 0);
+  else return mfma16_32x32x16<KIND == K_F16>(a, b, c);
+}
+
+// int8: row m's and weight row n's scales
+__device__ __forceinline__ float x_scale_of(const LinArgs& a, int64_t m) {
+  return a.x_scale[m * a.x_scale_row];
+}
+__device__ __forceinline__ float w_scale_of(const LinArgs& a, int64_t n) {
+  return a.weight_scale[n * a.weight_scale_row];
 }
 
 // f of the activation (gated ones: f of the gate).  x sigmoid(k x) with the
@@ -98,6 +144,8 @@ __device__ __forceinline__ void lin_act(int act, float (&y)[N]) {
 }
 
 // One output: z and, for gated activations, the factor u, both without bias.
+// KEEP: z and u with their biases are kept too (a.z).
+template <bool KEEP = false>
 __device__ __forceinline__ float lin_value(const LinArgs& a, int64_t m, int64_t n, float z,
                                            float u) {
   if (a.bias) z += ld_any(a.bias, a.bias_dtype, n);
@@ -107,6 +155,10 @@ __device__ __forceinline__ float lin_value(const LinArgs& a, int64_t m, int64_t 
   if (lin_gated(a.activation)) {
     if (a.bias) u += ld_any(a.bias, a.bias_dtype, a.N + n);
     y *= u;
+  }
+  if constexpr (KEEP) {
+    a.z[m * 2 * a.N + n] = z;
+    a.z[(m * 2 + 1) * a.N + n] = u;
   }
   if (a.residual) y += ld_any(a.residual, a.residual_dtype, m * a.ldr + n);
   return y;
@@ -142,15 +194,27 @@ __device__ __forceinline__ void ld8_any(const void* p, int dtype, int64_t i, flo
   }
 }
 
+// 8 floats to p, by 16 bytes where `vec`
+__device__ __forceinline__ void st8_f32(float* p, const float (&y)[8], bool vec) {
+  if (vec) {
+    float4* o = reinterpret_cast<float4*>(p);
+    o[0] = make_float4(y[0], y[1], y[2], y[3]);
+    o[1] = make_float4(y[4], y[5], y[6], y[7]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) p[k] = y[k];
+  }
+}
 // Outputs n .. n + 7 (those below N) of row m from their sums z and, for gated
 // activations, u.  vec: out's rows start at multiples of 16 bytes.  early: res
 // holds the 8 (16-bit) residuals, loaded before.
+template <bool KEEP = false>
 __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t n, const float* zp,
                                            const float* up, bool vec, bool early = false,
                                            uint4 res = uint4{}) {
   if (n + 8 > a.N) {
     for (int k = 0; k < 8 && n + k < a.N; ++k)
-      st_any(a.out, a.out_dtype, m * a.ldo + n + k, lin_value(a, m, n + k, zp[k], up[k]));
+      st_any(a.out, a.out_dtype, m * a.ldo + n + k, lin_value<KEEP>(a, m, n + k, zp[k], up[k]));
     return;
   }
   const bool gated = lin_gated(a.activation);
@@ -162,6 +226,7 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] += t[k];
   }
+  if constexpr (KEEP) st8_f32(a.z + m * 2 * a.N + n, y, (a.N & 3) == 0);
   lin_act(a.activation, y);
   if (gated) {
     float u[8];
@@ -172,6 +237,7 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
 #pragma unroll
       for (int k = 0; k < 8; ++k) u[k] += t[k];
     }
+    if constexpr (KEEP) st8_f32(a.z + (m * 2 + 1) * a.N + n, u, (a.N & 3) == 0);
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] *= u[k];
   }
@@ -188,9 +254,7 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
 #pragma unroll
     for (int k = 0; k < 8; ++k) st_any(a.out, a.out_dtype, m * a.ldo + n + k, y[k]);
   } else if (a.out_dtype == MI355MOE_F32) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + m * a.ldo + n);
-    o[0] = make_float4(y[0], y[1], y[2], y[3]);
-    o[1] = make_float4(y[4], y[5], y[6], y[7]);
+    st8_f32(static_cast<float*>(a.out) + m * a.ldo + n, y, true);
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -202,6 +266,53 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
   }
 }
 
+// The same from the sums of int8 products; `raw`: a split's sums, as they are, into
+// the int32 partial sums at a.out.
+__device__ __forceinline__ void lin_store8_i32(const LinArgs& a, int64_t m, int64_t n, const int* zp,
+                                               const int* up, bool vec, bool early = false,
+                                               uint4 res = uint4{}, bool raw = false) {
+  if (raw) {
+    int* o = static_cast<int*>(a.out) + m * a.ldo + n;
+    if (vec && n + 8 <= a.N) {
+      reinterpret_cast<int4*>(o)[0] = make_int4(zp[0], zp[1], zp[2], zp[3]);
+      reinterpret_cast<int4*>(o)[1] = make_int4(zp[4], zp[5], zp[6], zp[7]);
+    } else {
+      for (int k = 0; k < 8 && n + k < a.N; ++k) o[k] = zp[k];
+    }
+    return;
+  }
+  const float xs = x_scale_of(a, m);
+  float z[8], u[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int64_t c = n + k < a.N ? n + k : a.N - 1;
+    z[k] = static_cast<float>(zp[k]) * (xs * w_scale_of(a, c));
+    u[k] = lin_gated(a.activation) ? static_cast<float>(up[k]) * (xs * w_scale_of(a, a.N + c)) : 0.f;
+  }
+  lin_store8(a, m, n, z, u, vec, early, res);
+}
+
+// 16 bytes from column byte c of a row of `bytes` bytes, from any address;
+// zeros past its end and for rows that do not exist.
+typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ uint4 row16(const uint8_t* row, bool ok, int64_t c, int64_t bytes) {
+  if (!ok || c >= bytes) return make_uint4(0, 0, 0, 0);
+  if (c + 16 <= bytes) {
+    const any_u32x4 v = *reinterpret_cast<const any_u32x4*>(row + c);
+    return make_uint4(v.x, v.y, v.z, v.w);
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 15; ++k)
+    if (c + k < bytes) w[k >> 2] |= static_cast<uint32_t>(row[c + k]) << (8 * (k & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// codes and scales of 16- or 32-bit rows (int8_quant.hip)
+int launch_int8_quant(int dtype, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
+                      int64_t scale_row, int64_t rows, int64_t cols, hipStream_t st);
+// the sum of a split product's partial sums, in their order, then the epilogue (linear.hip)
+int launch_linear_finish(const LinArgs& a, const void* part, int splits, hipStream_t st);
 // few rows of x (linear_skinny.hip), any alignment; tile: the tiles can take them too
 bool linear_skinny_takes(const LinArgs& a, bool tile);
 int launch_linear_skinny(const LinArgs& a, hipStream_t st);

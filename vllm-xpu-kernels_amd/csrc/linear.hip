@@ -11,26 +11,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int GM = 64, GN = 64;
 
-// 16 bytes from column byte c of a row of `bytes` bytes, from any address;
-// zeros past its end and for rows that do not exist.
-typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
-__device__ __forceinline__ uint4 row16(const uint8_t* row, bool ok, int64_t c, int64_t bytes) {
-  if (!ok || c >= bytes) return make_uint4(0, 0, 0, 0);
-  if (c + 16 <= bytes) {
-    const any_u32x4 v = *reinterpret_cast<const any_u32x4*>(row + c);
-    return make_uint4(v.x, v.y, v.z, v.w);
-  }
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int k = 0; k < 15; ++k)
-    if (c + k < bytes) w[k >> 2] |= static_cast<uint32_t>(row[c + k]) << (8 * (k & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // K stages [split * per, ...) of 128 bytes; the next stage's rows are in registers
 // while this one's products run.
-template <bool FP8, bool F16, bool GATED>
+// KEEP: the sums go to a.z too.  RAW (int8): a split's sums, as they are.
+template <int KIND, bool GATED, bool KEEP, bool RAW>
 __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int per) {
+  constexpr bool FP8 = KIND == K_FP8;
+  using Sum = typename SumVec<KIND, 4>::T;
   constexpr int SB = 128;                // bytes of a K stage per row
   constexpr int PITCH = SB + 16;
   constexpr int WR = GATED ? 2 * GN : GN;
@@ -42,7 +29,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int pe
   const int l16 = lane & 15, q = lane >> 4;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * GM;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * GN;
-  constexpr int EB = FP8 ? 1 : 2;
+  constexpr int EB = kind_bytes(KIND);
   const int64_t kbytes = a.K * EB;
   const uint8_t* x = static_cast<const uint8_t*>(a.x);
   const uint8_t* w = static_cast<const uint8_t*>(a.weight);
@@ -50,11 +37,11 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int pe
   const int64_t kend = kfirst + static_cast<int64_t>(per) * SB < kbytes
                            ? kfirst + static_cast<int64_t>(per) * SB : kbytes;
 
-  f32x4 acc[NH][4];
+  Sum acc[NH][4];
 #pragma unroll
   for (int h = 0; h < NH; ++h)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j) acc[h][j] = Sum{0, 0, 0, 0};
 
   uint4 px[XC], pw[WC];
   auto fetch = [&](int64_t k) __attribute__((always_inline)) {
@@ -131,7 +118,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int pe
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint4 bv = *reinterpret_cast<const uint4*>(sx + (16 * j + l16) * PITCH + 64 * t + 16 * q);
-            acc[h][j] = mfma16_16x16x32<F16>(av, bv, acc[h][j]);
+            acc[h][j] = mfma_16x16<KIND>(av, bv, acc[h][j]);
           }
         }
       }
@@ -147,18 +134,31 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int pe
     for (int r = 0; r < 4; ++r) {
       const int64_t n = n0 + 16 * wave + 4 * q + r;
       if (n >= a.N) continue;
-      st_any(a.out, a.out_dtype, part + m * a.ldo + n,
-             lin_value(a, m, n, acc[0][j][r], acc[NH - 1][j][r]));
+      if constexpr (RAW) {
+        static_cast<int*>(a.out)[part + m * a.ldo + n] = acc[0][j][r];
+      } else if constexpr (KIND == K_I8) {
+        const float xs = x_scale_of(a, m);
+        const float z = static_cast<float>(acc[0][j][r]) * (xs * w_scale_of(a, n));
+        const float u = GATED ? static_cast<float>(acc[NH - 1][j][r]) * (xs * w_scale_of(a, a.N + n)) : 0.f;
+        st_any(a.out, a.out_dtype, part + m * a.ldo + n, lin_value(a, m, n, z, u));
+      } else {
+        st_any(a.out, a.out_dtype, part + m * a.ldo + n,
+               lin_value<KEEP>(a, m, n, acc[0][j][r], acc[NH - 1][j][r]));
+      }
     }
   }
 }
 
-template <bool FP8, bool F16>
+template <int KIND>
 int launch_any(const LinArgs& a, int splits, int per, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(cdiv(a.N, GN)), static_cast<unsigned>(cdiv(a.M, GM)),
                   static_cast<unsigned>(splits));
-  if (lin_gated(a.activation)) linear_any_kernel<FP8, F16, true><<<grid, dim3(256), 0, st>>>(a, per);
-  else linear_any_kernel<FP8, F16, false><<<grid, dim3(256), 0, st>>>(a, per);
+  constexpr bool W16 = KIND == K_BF16 || KIND == K_F16, I8 = KIND == K_I8;
+  if (W16 && a.z) linear_any_kernel<KIND, true, W16, false><<<grid, dim3(256), 0, st>>>(a, per);
+  else if (I8 && splits > 1) linear_any_kernel<KIND, false, false, I8><<<grid, dim3(256), 0, st>>>(a, per);
+  else if (lin_gated(a.activation))
+    linear_any_kernel<KIND, true, false, false><<<grid, dim3(256), 0, st>>>(a, per);
+  else linear_any_kernel<KIND, false, false, false><<<grid, dim3(256), 0, st>>>(a, per);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
@@ -166,45 +166,49 @@ int launch_any(const LinArgs& a, int splits, int per, hipStream_t st) {
 // K is split until there are about 1000 workgroups (four per CU), 8 stages each
 // at least.
 int any_stages(const LinArgs& a) {
-  const int64_t nk = cdiv(a.K * (a.x_dtype == MI355MOE_FP8E4M3 ? 1 : 2), 128);
+  const int64_t nk = cdiv(a.K * kind_bytes(kind_of(a)), 128);
   const int64_t tiles = cdiv(a.M, GM) * cdiv(lin_rows(a), GN);
   const int64_t most = nk / 8 > 1 ? nk / 8 : 1, want = cdiv(1000, tiles);
   return static_cast<int>(cdiv(nk, want < most ? want : most));
 }
 int any_splits(const LinArgs& a) {
-  return static_cast<int>(cdiv(cdiv(a.K * (a.x_dtype == MI355MOE_FP8E4M3 ? 1 : 2), 128), any_stages(a)));
+  return static_cast<int>(cdiv(cdiv(a.K * kind_bytes(kind_of(a)), 128), any_stages(a)));
 }
 
 // Split K: the sum of the splits' partial sums, in their order, then the epilogue.
 // The loads of kAhead splits are on their way at once, and workgroups are one wave
 // so that few outputs reach many CUs (24 x 4096 x 4096, both kernels: 13.9 us; one
 // split after the other 15.3, four at once 14.5, workgroups of 256 14.0).
-template <bool GATED>
+// I8: int32 partial sums.  KEEP: the sums go to a.z too.
+template <bool GATED, bool I8, bool KEEP>
 __global__ __launch_bounds__(64) void linear_finish_kernel(const LinArgs a,
-                                                            const float* __restrict__ part,
+                                                            const void* __restrict__ parts,
                                                             int splits, int64_t rows) {
   constexpr int kAhead = 8, H = GATED ? 2 : 1;
+  using S = std::conditional_t<I8, int, float>;
+  using S4 = typename SumVec<I8 ? K_I8 : K_BF16, 4>::T;
+  const S* part = static_cast<const S*>(parts);
   const int64_t chunks = (a.N + 7) / 8;
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
   if (idx >= a.M * chunks) return;
   const int64_t m = idx / chunks, n = (idx % chunks) * 8;
-  float z[H][8];
+  S z[H][8];
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) z[h][k] = 0.f;
+    for (int k = 0; k < 8; ++k) z[h][k] = 0;
   const int64_t step = a.M * rows;
-  const float* p = part + m * rows + n;
+  const S* p = part + m * rows + n;
   if ((rows & 3) == 0 && (a.N & 3) == 0 && n + 8 <= a.N) {
     for (int s = 0; s < splits; s += kAhead) {
-      f32x4 v[kAhead][H][2];
+      S4 v[kAhead][H][2];
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
-        const float* q = p + (s + e < splits ? s + e : splits - 1) * step;  // surplus: unused
+        const S* q = p + (s + e < splits ? s + e : splits - 1) * step;  // surplus: unused
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          v[e][h][0] = reinterpret_cast<const f32x4*>(q + h * a.N)[0];
-          v[e][h][1] = reinterpret_cast<const f32x4*>(q + h * a.N)[1];
+          v[e][h][0] = reinterpret_cast<const S4*>(q + h * a.N)[0];
+          v[e][h][1] = reinterpret_cast<const S4*>(q + h * a.N)[1];
         }
       }
 #pragma unroll
@@ -226,8 +230,14 @@ __global__ __launch_bounds__(64) void linear_finish_kernel(const LinArgs a,
         }
   }
   const int osize = a.out_dtype == MI355MOE_F32 ? 4 : 2;
-  lin_store8(a, m, n, z[0], z[H - 1],
-             ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * osize)) & 15) == 0);
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * osize)) & 15) == 0;
+  if constexpr (I8) lin_store8_i32(a, m, n, z[0], z[H - 1], vec);
+  else lin_store8<KEEP>(a, m, n, z[0], z[H - 1], vec);
+}
+
+// 16-bit x that becomes int8 in the call
+bool quantises(const LinArgs& a) {
+  return a.weight_dtype == MI355MOE_I8 && a.x_dtype != MI355MOE_I8;
 }
 
 bool float_dtype(int d) {
@@ -235,9 +245,11 @@ bool float_dtype(int d) {
 }
 
 int check(const LinArgs& a) {
-  const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
-  MI_ARG(fp8 || a.x_dtype == MI355MOE_BF16 || a.x_dtype == MI355MOE_F16,
-         "linear: x must be bfloat16, float16 or float8_e4m3fn");
+  const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3, i8 = a.x_dtype == MI355MOE_I8;
+  MI_ARG(fp8 || i8 || a.x_dtype == MI355MOE_BF16 || a.x_dtype == MI355MOE_F16,
+         "linear: x must be bfloat16, float16 or float8_e4m3fn, or int8");
+  MI_ARG(a.weight_dtype == 0 || a.weight_dtype == a.x_dtype || (a.weight_dtype == MI355MOE_I8 && !fp8),
+         "linear: weight must have x's type, or be int8 for bfloat16 and float16 x");
   MI_ARG(float_dtype(a.out_dtype), "linear: out must be float32, bfloat16 or float16");
   MI_ARG(!a.bias || float_dtype(a.bias_dtype), "linear: bias must be float32, bfloat16 or float16");
   MI_ARG(!a.residual || float_dtype(a.residual_dtype),
@@ -252,6 +264,9 @@ int check(const LinArgs& a) {
          "linear: negative stride");
   MI_ARG(a.M <= 1 || a.ldo >= a.N, "linear: rows of out overlap");
   MI_ARG(!fp8 || a.K % 128 == 0, "linear: K must be divisible by 128 for float8 operands");
+  MI_ARG(!(i8 || quantises(a)) || a.K < (1 << 17), "linear: K must be below 131072 for int8 operands");
+  MI_ARG(!a.z || (lin_gated(a.activation) && !fp8 && !i8 && !quantises(a)),
+         "linear: z is kept for gated activations of 16-bit operands");
   return MI355MOE_OK;
 }
 
@@ -260,64 +275,108 @@ int check(const LinArgs& a) {
 
 using namespace mi355;
 
-namespace {
-int launch_linear_finish(const LinArgs& a, const float* part, int splits, hipStream_t st) {
+namespace mi355 {
+int launch_linear_finish(const LinArgs& a, const void* part, int splits, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(cdiv(a.M * cdiv(a.N, 8), 64)));
-  if (lin_gated(a.activation))
-    linear_finish_kernel<true><<<grid, dim3(64), 0, st>>>(a, part, splits, lin_rows(a));
-  else linear_finish_kernel<false><<<grid, dim3(64), 0, st>>>(a, part, splits, lin_rows(a));
+  const int64_t rows = lin_rows(a);
+  const bool i8 = a.x_dtype == MI355MOE_I8;
+  if (lin_gated(a.activation)) {
+    if (a.z) linear_finish_kernel<true, false, true><<<grid, dim3(64), 0, st>>>(a, part, splits, rows);
+    else if (i8) linear_finish_kernel<true, true, false><<<grid, dim3(64), 0, st>>>(a, part, splits, rows);
+    else linear_finish_kernel<true, false, false><<<grid, dim3(64), 0, st>>>(a, part, splits, rows);
+  } else if (i8) {
+    linear_finish_kernel<false, true, false><<<grid, dim3(64), 0, st>>>(a, part, splits, rows);
+  } else {
+    linear_finish_kernel<false, false, false><<<grid, dim3(64), 0, st>>>(a, part, splits, rows);
+  }
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
+}  // namespace mi355
+
+namespace {
 size_t lin_partials(const LinArgs& a, int splits) {
   return splits == 1 ? 0 : static_cast<size_t>(splits) * a.M * lin_rows(a) * sizeof(float);
 }
 enum Path { SKINNY, TILE, ANY };
 Path path_of(const LinArgs& a) {
   const bool tile = linear_tile_supported(a);
-  if (linear_skinny_takes(a, tile)) return SKINNY;
+  if (!a.z && linear_skinny_takes(a, tile)) return SKINNY;
   return tile ? TILE : ANY;
+}
+int splits_of(const LinArgs& a, Path path) {
+  return path == SKINNY ? 1 : path == TILE ? linear_tile_splits(a) : any_splits(a);
+}
+// Where x is quantised in the call: its codes (rows at multiples of 16 bytes) and
+// scales in the workspace, before the partial sums; `c` becomes the product of them.
+size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
+size_t code_bytes(LinArgs& c, uintptr_t workspace) {
+  c.ldx = static_cast<int64_t>(up16(static_cast<size_t>(c.K)));
+  const size_t codes = static_cast<size_t>(c.M) * c.ldx;
+  c.x_dtype = MI355MOE_I8;
+  c.x = reinterpret_cast<const void*>(workspace);
+  c.x_scale = reinterpret_cast<const float*>(workspace + codes);
+  c.x_scale_row = 1;
+  return codes + up16(static_cast<size_t>(c.M) * sizeof(float));
 }
 }  // namespace
 
 extern "C" size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* p) {
   if (!p || check(*p) || p->M == 0) return 0;
-  const Path path = path_of(*p);
-  return path == SKINNY ? 0
-                        : lin_partials(*p, path == TILE ? linear_tile_splits(*p) : any_splits(*p));
+  LinArgs a = *p;
+  const size_t codes = quantises(a) ? code_bytes(a, 0) : 0;
+  return codes + lin_partials(a, splits_of(a, path_of(a)));
 }
 
 extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
                                size_t workspace_bytes, void* stream) {
   MI_ARG(p, "null pointer");
-  const LinArgs a = *p;
+  LinArgs a = *p;
   if (const int rc = check(a)) return rc;
   if (a.M == 0) return MI355MOE_OK;
-  const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
+  const bool quant = quantises(a);
   MI_ARG(a.x && a.weight && a.out, "null pointer");
-  MI_ARG(!fp8 || (a.x_scale && a.weight_scale), "linear: scales missing");
+  MI_ARG((a.x_dtype != MI355MOE_FP8E4M3 && a.x_dtype != MI355MOE_I8 && !quant) ||
+             ((a.x_scale || quant) && a.weight_scale), "linear: scales missing");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const LinArgs given = a;
+  const size_t codes = quant ? code_bytes(a, reinterpret_cast<uintptr_t>(workspace)) : 0;
   const Path path = path_of(a);
-  if (path == SKINNY) return launch_linear_skinny(a, st);
-  const int splits = path == TILE ? linear_tile_splits(a) : any_splits(a);
-  MI_CHECK(splits == 1 || (workspace && workspace_bytes >= lin_partials(a, splits)),
-           MI355MOE_ERR_WORKSPACE, "linear: workspace too small");
-  MI_ARG(splits == 1 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+  const int splits = splits_of(a, path);
+  const size_t need = codes + lin_partials(a, splits);
+  MI_CHECK(need == 0 || (workspace && workspace_bytes >= need), MI355MOE_ERR_WORKSPACE,
+           "linear: workspace too small");
+  MI_ARG(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
          "linear: workspace must be 16-byte aligned");
-  // a split product leaves fp32 partial sums of all weight rows
+  if (quant) {
+    const int rc = launch_int8_quant(given.x_dtype, given.x, given.ldx, static_cast<int8_t*>(workspace),
+                                     a.ldx, const_cast<float*>(a.x_scale), 1, a.M, a.K, st);
+    if (rc) return rc;
+  }
+  if (path == SKINNY) return launch_linear_skinny(a, st);
+  // a split product leaves partial sums (fp32, of int8 products int32) of all weight rows
+  void* parts = static_cast<uint8_t*>(workspace) + codes;
   LinArgs b = a;
   if (splits > 1) {
     b.N = b.ldo = lin_rows(a);
     b.activation = MI355MOE_LINEAR_NONE;
     b.bias = b.residual = nullptr;
-    b.out = workspace;
+    b.out = parts;
     b.out_dtype = MI355MOE_F32;
+    b.z = nullptr;
   }
   int rc;
-  if (path == TILE) rc = launch_linear_tile(a, b, st);
-  else if (fp8) rc = launch_any<true, false>(b, splits, any_stages(a), st);
-  else if (a.x_dtype == MI355MOE_F16) rc = launch_any<false, true>(b, splits, any_stages(a), st);
-  else rc = launch_any<false, false>(b, splits, any_stages(a), st);
+  if (path == TILE) {
+    rc = launch_linear_tile(a, b, st);
+  } else {
+    const int per = any_stages(a);
+    switch (kind_of(a)) {
+      case K_FP8: rc = launch_any<K_FP8>(b, splits, per, st); break;
+      case K_I8: rc = launch_any<K_I8>(b, splits, per, st); break;
+      case K_F16: rc = launch_any<K_F16>(b, splits, per, st); break;
+      default: rc = launch_any<K_BF16>(b, splits, per, st);
+    }
+  }
   if (rc || splits == 1) return rc;
-  return launch_linear_finish(a, static_cast<const float*>(workspace), splits, st);
+  return launch_linear_finish(a, parts, splits, st);
 }

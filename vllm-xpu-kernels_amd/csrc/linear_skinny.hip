@@ -32,12 +32,15 @@ __device__ __forceinline__ uint4 as4(u32x4 v) { return make_uint4(v.x, v.y, v.z,
 
 constexpr int kScaleBytes = 48 * 1024;  // LDS for the e4m3 scales
 
-template <bool FP8, bool F16, bool GATED, int R, int MT, int U>
+template <int KIND, bool GATED, int R, int MT, int U>
 __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   constexpr int C = 16 / R;
   constexpr int STEP = C * 64;                // bytes of a row per K step
   constexpr int NS = GATED ? 2 : 1;           // strips: the gate's, the factor's
-  constexpr int EB = FP8 ? 1 : 2;
+  constexpr bool FP8 = KIND == K_FP8, I8 = KIND == K_I8;
+  using Sum = typename SumVec<KIND, 4>::T;
+  using S = std::conditional_t<I8, int, float>;
+  constexpr int EB = kind_bytes(KIND);
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   const int kblocks = FP8 ? static_cast<int>(a.K / 128) : 0;
   float* s_ws = lds;
   float* s_xs = s_ws + (FP8 ? (kblocks + 1) * NS * R : 0);
-  float* red = s_xs + (FP8 ? (kblocks + 1) * MT * R : 0);
+  S* red = reinterpret_cast<S*>(s_xs + (FP8 ? (kblocks + 1) * MT * R : 0));
 
   const bool any = s0 < s1;  // uniform per wave
   if (any) load(w0, x0, s0);
@@ -113,11 +116,11 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
     __syncthreads();
   }
 
-  f32x4 acc[NS][MT];
+  Sum acc[NS][MT];
 #pragma unroll
   for (int i = 0; i < NS; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MT; ++j) acc[i][j] = Sum{0, 0, 0, 0};
   // the lane's results: rows 4 q .. 4 q + 3 of the 16 (chunk co, strip rows
   // ro .. ro + 3), column l16 (chunk ci, row of x ri)
   const int co = (4 * q) / R, ro = (4 * q) % R;
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int j = 0; j < MT; ++j)
-          acc[i][j] = mfma16_16x16x32<F16>(as4(w[i]), as4(x[j]), acc[i][j]);
+          acc[i][j] = mfma_16x16<KIND>(as4(w[i]), as4(x[j]), acc[i][j]);
     }
   };
   auto compute = [&](u32x4 (&w)[U][NS], u32x4 (&x)[U][MT], int s) __attribute__((always_inline)) {
@@ -181,16 +184,23 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
       compute(w1, x1, s + U);
     }
   }
-  // the last K % 8 values of 16-bit rows: wave 0, element by element
+  // the last K % 8 values of 16-bit rows, K % 16 of int8 ones: wave 0, element by element
   if constexpr (!FP8) {
     if (kfull < kbytes && wave == 0) {
       auto tail = [&](const uint8_t* row) __attribute__((always_inline)) {
         uint32_t v[4] = {0, 0, 0, 0};
+        if constexpr (I8) {
 #pragma unroll
-        for (int k = 0; k < 7; ++k)
-          if (ci == 0 && q == 0 && kfull + 2 * k < kbytes)
-            v[k >> 1] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + kfull + 2 * k))
-                         << (16 * (k & 1));
+          for (int k = 0; k < 15; ++k)
+            if (ci == 0 && q == 0 && kfull + k < kbytes)
+              v[k >> 2] |= static_cast<uint32_t>(row[kfull + k]) << (8 * (k & 3));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 7; ++k)
+            if (ci == 0 && q == 0 && kfull + 2 * k < kbytes)
+              v[k >> 1] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + kfull + 2 * k))
+                           << (16 * (k & 1));
+        }
         return u32x4{v[0], v[1], v[2], v[3]};
       };
       u32x4 w[NS], x[MT];
@@ -209,7 +219,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
     for (int i = 0; i < NS; ++i)
 #pragma unroll
       for (int j = 0; j < MT; ++j)
-        *reinterpret_cast<f32x4*>(red + ((wave * NS + i) * MT + j) * TILE + (ci * R + ri) * R + ro) =
+        *reinterpret_cast<Sum*>(red + ((wave * NS + i) * MT + j) * TILE + (ci * R + ri) * R + ro) =
             acc[i][j];
   }
   __syncthreads();
@@ -217,26 +227,32 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
     const int r = o % R, mr = (o / R) % R, j = o / (R * R);
     const int64_t n = n0 + r, m = mbase + R * j + mr;
     if (n >= a.N || m >= a.M) continue;
-    float z = 0.f, u = 0.f;
+    S z = 0, u = 0;
     for (int w = 0; w < waves; ++w)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float* p = red + (w * NS * MT + j) * TILE + (c * R + mr) * R + r;
+        const S* p = red + (w * NS * MT + j) * TILE + (c * R + mr) * R + r;
         z += p[0];
         if constexpr (GATED) u += p[MT * TILE];
       }
-    st_any(a.out, a.out_dtype, m * a.ldo + n, lin_value(a, m, n, z, u));
+    float zf = static_cast<float>(z), uf = static_cast<float>(u);
+    if constexpr (I8) {
+      const float xs = x_scale_of(a, m);
+      zf *= xs * w_scale_of(a, n);
+      if constexpr (GATED) uf *= xs * w_scale_of(a, a.N + n);
+    }
+    st_any(a.out, a.out_dtype, m * a.ldo + n, lin_value(a, m, n, zf, uf));
   }
 }
 
-template <bool FP8, bool F16, bool GATED, int R, int MT, int U>
+template <int KIND, bool GATED, int R, int MT, int U>
 int launch(const LinArgs& a, int waves, hipStream_t st) {
   constexpr int NS = GATED ? 2 : 1;
-  const int64_t blocks = FP8 ? a.K / 128 + 1 : 0;
+  const int64_t blocks = KIND == K_FP8 ? a.K / 128 + 1 : 0;
   // at most 48 KiB of scales (linear_skinny_takes), a block of zeros and 8 KiB of sums
   const size_t lds = 4 * (blocks * (NS + MT) * R + static_cast<size_t>(waves) * NS * MT * 16 * R);
   const dim3 grid(static_cast<unsigned>(cdiv(a.N, R)), static_cast<unsigned>(cdiv(a.M, R * MT)));
-  linear_skinny_kernel<FP8, F16, GATED, R, MT, U><<<grid, dim3(64 * waves), lds, st>>>(a);
+  linear_skinny_kernel<KIND, GATED, R, MT, U><<<grid, dim3(64 * waves), lds, st>>>(a);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
@@ -250,21 +266,21 @@ int launch(const LinArgs& a, int waves, hipStream_t st) {
 // (4 x 2048 x 7168 7.6 against 8.5).  More waves per strip shorten the walk over a
 // long K and lengthen the sum at its end (1 x 7168 x 7168 with 1 / 2 / 4 waves 21.0 /
 // 21.9 / 23.4, e4m3 1 x 7168 x 4096 gated 19.1 / 13.9 / 11.7, before GUARD).
-template <bool FP8, bool F16, bool GATED>
+template <int KIND, bool GATED>
 int launch_rows(const LinArgs& a, hipStream_t st) {
   const bool few = a.N <= 2048;  // at most 128 strips of 16
-  if constexpr (FP8) {
+  if constexpr (KIND == K_FP8) {
     const bool lng = a.K >= 4096;
-    if (a.M <= 4 && few) return launch<FP8, F16, GATED, 4, 1, 4>(a, lng ? 4 : 2, st);
-    if (a.M <= 8 && few && lng) return launch<FP8, F16, GATED, 4, 2, 4>(a, 4, st);
-    if (few && lng) return launch<FP8, F16, GATED, 8, 2, 4>(a, 4, st);
-    return launch<FP8, F16, GATED, 16, 1, 4>(a, 4, st);
+    if (a.M <= 4 && few) return launch<KIND, GATED, 4, 1, 4>(a, lng ? 4 : 2, st);
+    if (a.M <= 8 && few && lng) return launch<KIND, GATED, 4, 2, 4>(a, 4, st);
+    if (few && lng) return launch<KIND, GATED, 8, 2, 4>(a, 4, st);
+    return launch<KIND, GATED, 16, 1, 4>(a, 4, st);
   } else {
     if (a.M == 1 || (a.M <= 4 && a.N < 4096))
-      return launch<FP8, F16, GATED, 4, 1, 4>(a, few ? 2 : 1, st);
-    if (a.M <= 8 && few) return launch<FP8, F16, GATED, 4, 2, 4>(a, a.N <= 1024 ? 2 : 1, st);
-    if (few && (a.M <= 16 || a.N <= 512)) return launch<FP8, F16, GATED, 8, 2, 4>(a, 2, st);
-    return launch<FP8, F16, GATED, 16, 1, 4>(a, a.N <= 5120 && a.M <= 16 ? 4 : 2, st);
+      return launch<KIND, GATED, 4, 1, 4>(a, few ? 2 : 1, st);
+    if (a.M <= 8 && few) return launch<KIND, GATED, 4, 2, 4>(a, a.N <= 1024 ? 2 : 1, st);
+    if (few && (a.M <= 16 || a.N <= 512)) return launch<KIND, GATED, 8, 2, 4>(a, 2, st);
+    return launch<KIND, GATED, 16, 1, 4>(a, a.N <= 5120 && a.M <= 16 ? 4 : 2, st);
   }
 }
 
@@ -291,10 +307,12 @@ bool linear_skinny_takes(const LinArgs& a, bool tile) {
 int launch_linear_skinny(const LinArgs& a, hipStream_t st) {
   const bool g = lin_gated(a.activation);
   if (a.x_dtype == MI355MOE_FP8E4M3)
-    return g ? launch_rows<true, false, true>(a, st) : launch_rows<true, false, false>(a, st);
+    return g ? launch_rows<K_FP8, true>(a, st) : launch_rows<K_FP8, false>(a, st);
+  if (a.x_dtype == MI355MOE_I8)
+    return g ? launch_rows<K_I8, true>(a, st) : launch_rows<K_I8, false>(a, st);
   if (a.x_dtype == MI355MOE_F16)
-    return g ? launch_rows<false, true, true>(a, st) : launch_rows<false, true, false>(a, st);
-  return g ? launch_rows<false, false, true>(a, st) : launch_rows<false, false, false>(a, st);
+    return g ? launch_rows<K_F16, true>(a, st) : launch_rows<K_F16, false>(a, st);
+  return g ? launch_rows<K_BF16, true>(a, st) : launch_rows<K_BF16, false>(a, st);
 }
 
 }  // namespace mi355

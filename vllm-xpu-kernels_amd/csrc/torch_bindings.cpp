@@ -958,17 +958,24 @@ int64_t row_stride(const at::Tensor& t, const char* name) {
   return ld;
 }
 
-void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
-            const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
-            const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual,
-            int64_t activation) {
+// int8: the weight is int8 with a scale per row, the input int8 with a scale per row or
+// 16-bit without.  z: [rows, 2 out_features] float32 that keeps the gated sums.
+void run_linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
+                const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
+                const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual,
+                int64_t activation, bool int8, const std::optional<at::Tensor>& z) {
   TORCH_CHECK(input.is_cuda(), "input must be on a GPU device");
   TORCH_CHECK(input.dim() >= 1, "input must have at least one dimension");
-  const bool fp8 = input.scalar_type() == at::kFloat8_e4m3fn;
-  TORCH_CHECK(fp8 || input.scalar_type() == at::kBFloat16 || input.scalar_type() == at::kHalf,
-              "input must be bfloat16, float16 or float8_e4m3fn");
+  const bool fp8 = !int8 && input.scalar_type() == at::kFloat8_e4m3fn;
+  const bool in16 = input.scalar_type() == at::kBFloat16 || input.scalar_type() == at::kHalf;
   check_here(weight, "weight", input);
-  TORCH_CHECK(weight.scalar_type() == input.scalar_type(), "weight must have the input's type");
+  if (int8) {
+    TORCH_CHECK(in16 || input.scalar_type() == at::kChar, "input must be bfloat16, float16 or int8");
+    TORCH_CHECK(weight.scalar_type() == at::kChar, "weight must be int8");
+  } else {
+    TORCH_CHECK(fp8 || in16, "input must be bfloat16, float16 or float8_e4m3fn");
+    TORCH_CHECK(weight.scalar_type() == input.scalar_type(), "weight must have the input's type");
+  }
   TORCH_CHECK(weight.dim() == 2, "weight must be 2-dimensional");
   TORCH_CHECK(weight.size(1) == input.size(-1), "weight must be [out_features, in_features] with "
               "the input's last dimension as in_features");
@@ -988,8 +995,46 @@ void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Te
   a.ldx = row_stride(input, "input");
   a.weight = weight.data_ptr();
   a.ldw = row_stride(weight, "weight");
-  TORCH_CHECK(fp8 == input_scale.has_value() && fp8 == weight_scale.has_value(),
-              "scales belong to float8_e4m3fn operands");
+  if (int8) {
+    a.weight_dtype = MI355MOE_I8;
+    TORCH_CHECK(input_scale.has_value() != in16,
+                "input_scale belongs to an int8 input (a 16-bit one is quantised here)");
+    TORCH_CHECK(weight_scale.has_value(), "weight_scale is missing");
+    auto scales = [&](const at::Tensor& t, const char* name, int64_t n, const char* shape) {
+      check_here(t, name, input);
+      TORCH_CHECK(t.scalar_type() == at::kFloat, "scales must be float32");
+      int64_t stride = 1;
+      bool ok = t.numel() == n && t.dim() >= 1;
+      for (int64_t d = 0; ok && d < t.dim(); ++d)
+        if (t.size(d) != 1) {
+          ok = t.size(d) == n;
+          stride = t.stride(d);
+        }
+      TORCH_CHECK(ok, name, " must be ", shape);
+      check_apart(out, "out", t, name, false);
+      return stride;
+    };
+    if (input_scale) {
+      // one for each row: [rows], [rows, 1], or the input's leading dimensions (and 1)
+      at::Tensor t = *input_scale;
+      const bool lead = t.dim() >= input.dim() - 1 && t.dim() <= input.dim() && t.numel() == a.M &&
+                        t.sizes().slice(0, input.dim() - 1) == input.sizes().slice(0, input.dim() - 1);
+      if (lead && input.dim() > 2) {
+        a.x_scale_row = row_stride(t.dim() == input.dim() ? t : t.unsqueeze(-1), "input_scale");
+        check_here(t, "input_scale", input);
+        TORCH_CHECK(t.scalar_type() == at::kFloat, "scales must be float32");
+        check_apart(out, "out", t, "input_scale", false);
+      } else {
+        a.x_scale_row = scales(t, "input_scale", a.M, "[num_rows] or [num_rows, 1]");
+      }
+      a.x_scale = t.data_ptr<float>();
+    }
+    a.weight_scale_row = scales(*weight_scale, "weight_scale", rows, "[out_features] or [out_features, 1]");
+    a.weight_scale = weight_scale->data_ptr<float>();
+  } else {
+    TORCH_CHECK(fp8 == input_scale.has_value() && fp8 == weight_scale.has_value(),
+                "scales belong to float8_e4m3fn operands");
+  }
   if (fp8) {
     TORCH_CHECK(K % 128 == 0, "in_features must be divisible by 128");
     check_here(*input_scale, "input_scale", input);
@@ -1042,6 +1087,7 @@ void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Te
     a.residual_dtype = dtype_code(residual->scalar_type());
     check_apart(out, "out", *residual, "residual", true);
   }
+  if (z) a.z = z->data_ptr<float>();
   if (a.M == 0) return;
   DevGuard g(input.device());
   const size_t need = mi355moe_linear_workspace_size(&a);
@@ -1050,19 +1096,185 @@ void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Te
   check_rc(mi355moe_linear(&a, need ? ws.data_ptr() : nullptr, need, cur_stream(input)), "linear");
 }
 
+void linear(at::Tensor& out, const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
+            const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
+            const std::optional<at::Tensor>& bias, const std::optional<at::Tensor>& residual,
+            int64_t activation) {
+  run_linear(out, input, input_scale, weight, weight_scale, bias, residual, activation, false,
+             std::nullopt);
+}
+
+void linear_int8(at::Tensor& out, const at::Tensor& input,
+                 const std::optional<at::Tensor>& input_scale, const at::Tensor& weight,
+                 const at::Tensor& weight_scale, const std::optional<at::Tensor>& bias,
+                 const std::optional<at::Tensor>& residual, int64_t activation) {
+  run_linear(out, input, input_scale, weight, weight_scale, bias, residual, activation, true,
+             std::nullopt);
+}
+
+// a product's output: the input's shape with out_features columns
+at::Tensor linear_out(const at::Tensor& input, const at::Tensor& weight, int64_t activation,
+                      at::ScalarType dtype) {
+  TORCH_CHECK(input.dim() >= 1, "input must have at least one dimension");
+  TORCH_CHECK(weight.dim() == 2, "weight must be 2-dimensional");
+  std::vector<c10::SymInt> sizes(input.sym_sizes().begin(), input.sym_sizes().end());
+  sizes.back() = activation >= MI355MOE_LINEAR_SILU_AND_MUL ? weight.sym_size(0) / 2 : weight.sym_size(0);
+  return at::empty_symint(sizes, input.options().dtype(dtype));
+}
+
 at::Tensor linear_new(const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
                       const at::Tensor& weight, const std::optional<at::Tensor>& weight_scale,
                       const std::optional<at::Tensor>& bias,
                       const std::optional<at::Tensor>& residual, int64_t activation,
                       at::ScalarType out_dtype) {
-  TORCH_CHECK(input.dim() >= 1, "input must have at least one dimension");
-  TORCH_CHECK(weight.dim() == 2, "weight must be 2-dimensional");
-  std::vector<c10::SymInt> sizes(input.sym_sizes().begin(), input.sym_sizes().end());
-  sizes.back() = activation >= MI355MOE_LINEAR_SILU_AND_MUL ? weight.sym_size(0) / 2 : weight.sym_size(0);
-  at::Tensor out = at::empty_symint(sizes, input.options().dtype(out_dtype));
+  at::Tensor out = linear_out(input, weight, activation, out_dtype);
   if (!input.is_meta())
     linear(out, input, input_scale, weight, weight_scale, bias, residual, activation);
   return out;
+}
+
+at::Tensor linear_int8_new(const at::Tensor& input, const std::optional<at::Tensor>& input_scale,
+                           const at::Tensor& weight, const at::Tensor& weight_scale,
+                           const std::optional<at::Tensor>& bias,
+                           const std::optional<at::Tensor>& residual, int64_t activation,
+                           at::ScalarType out_dtype) {
+  at::Tensor out = linear_out(input, weight, activation, out_dtype);
+  if (!input.is_meta())
+    linear_int8(out, input, input_scale, weight, weight_scale, bias, residual, activation);
+  return out;
+}
+
+// (codes, scales [.., 1])
+std::tuple<at::Tensor, at::Tensor> per_token_int8_quant(const at::Tensor& input) {
+  TORCH_CHECK(input.dim() >= 1 && input.sym_size(-1) > 0, "input must have columns");
+  TORCH_CHECK(float16or32(input), "input must be float32, bfloat16 or float16");
+  std::vector<c10::SymInt> sizes(input.sym_sizes().begin(), input.sym_sizes().end());
+  at::Tensor q = at::empty_symint(sizes, input.options().dtype(at::kChar));
+  sizes.back() = 1;
+  at::Tensor scales = at::empty_symint(sizes, input.options().dtype(at::kFloat));
+  if (input.is_meta()) return {q, scales};
+  TORCH_CHECK(input.is_cuda(), "input must be on a GPU device");
+  const int64_t cols = input.size(-1), rows = input.numel() / cols;
+  const int64_t ldx = row_stride(input, "input");
+  if (rows == 0) return {q, scales};
+  DevGuard g(input.device());
+  check_rc(mi355moe_int8_quant(input.data_ptr(), dtype_code(input.scalar_type()), ldx,
+                               static_cast<int8_t*>(q.data_ptr()), cols, scales.data_ptr<float>(), 1,
+                               rows, cols, cur_stream(input)),
+           "per_token_int8_quant");
+  return {q, scales};
+}
+
+// ------------------------------------------------------------- gated linear
+// (out, z): z [rows, 2 out_features] float32 holds the sums with `keep`, else nothing
+std::tuple<at::Tensor, at::Tensor> gated_linear(const at::Tensor& input, const at::Tensor& weight,
+                                                const std::optional<at::Tensor>& bias,
+                                                int64_t activation, bool keep) {
+  TORCH_CHECK(activation >= MI355MOE_LINEAR_SILU_AND_MUL &&
+                  activation <= MI355MOE_LINEAR_GELU_TANH_AND_MUL,
+              "the activation must be a gated one");
+  at::Tensor out = linear_out(input, weight, activation, input.scalar_type());
+  at::Tensor z;
+  const auto f32 = input.options().dtype(at::kFloat);
+  if (keep) {
+    c10::SymInt rows = 1;
+    for (int64_t d = 0; d + 1 < input.dim(); ++d) rows *= input.sym_size(d);
+    z = at::empty_symint({rows, weight.sym_size(0)}, f32);
+  } else {
+    z = at::empty({0}, f32);
+  }
+  if (!input.is_meta()) {
+    TORCH_CHECK(input.scalar_type() == at::kBFloat16 || input.scalar_type() == at::kHalf,
+                "input must be bfloat16 or float16");
+    run_linear(out, input, std::nullopt, weight, std::nullopt, bias, std::nullopt, activation, false,
+               keep ? std::optional<at::Tensor>(z) : std::nullopt);
+  }
+  return {out, z};
+}
+
+// Gradients of the input, the weight and the bias, those asked for (else tensors of nothing):
+// the input's where the weight is given, the weight's where the input is, the bias's
+// in its type.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(
+    const at::Tensor& grad, const std::optional<at::Tensor>& input,
+    const std::optional<at::Tensor>& weight, const at::Tensor& z, int64_t activation,
+    std::optional<at::ScalarType> bias_dtype) {
+  TORCH_CHECK(grad.dim() >= 1 && z.dim() == 2, "grad must have columns, z must be 2-dimensional");
+  const auto o = grad.options();
+  at::Tensor dx = at::empty({0}, o), dw = at::empty({0}, o), db = at::empty({0}, o);
+  if (weight) {
+    TORCH_CHECK(weight->dim() == 2, "weight must be 2-dimensional");
+    std::vector<c10::SymInt> sizes(grad.sym_sizes().begin(), grad.sym_sizes().end());
+    sizes.back() = weight->sym_size(1);
+    dx = at::empty_symint(sizes, o);
+  }
+  if (input) {
+    TORCH_CHECK(input->dim() >= 1, "input must have at least one dimension");
+    dw = at::empty_symint({z.sym_size(1), input->sym_size(-1)}, o);
+  }
+  if (bias_dtype) db = at::empty_symint({z.sym_size(1)}, o.dtype(*bias_dtype));
+  if (grad.is_meta()) return {dx, dw, db};
+  TORCH_CHECK(grad.is_cuda(), "grad must be on a GPU device");
+  TORCH_CHECK(grad.scalar_type() == at::kBFloat16 || grad.scalar_type() == at::kHalf,
+              "grad must be bfloat16 or float16");
+  TORCH_CHECK(weight || input || bias_dtype, "no gradient is asked for");
+  check_here(z, "z", grad);
+  const int64_t N = grad.size(-1);
+  mi355moe_gated_linear_backward_args a{};
+  a.dtype = dtype_code(grad.scalar_type());
+  a.activation = static_cast<int>(activation);
+  a.N = N;
+  TORCH_CHECK(N > 0, "grad must have columns");
+  a.M = grad.numel() / N;
+  TORCH_CHECK(z.scalar_type() == at::kFloat && z.is_contiguous() && z.size(0) == a.M && z.size(1) == 2 * N,
+              "z must be what gated_linear kept");
+  a.z = z.data_ptr<float>();
+  // a gradient may come expanded or permuted (a sum's, a transposed reader's)
+  at::Tensor d = grad;
+  bool fold = grad.size(-1) <= 1 || grad.stride(-1) == 1;
+  int64_t want = -1;
+  for (int64_t i = grad.dim() - 2; fold && i >= 0; --i) {
+    if (grad.size(i) <= 1) continue;
+    fold = want < 0 || grad.stride(i) == want;
+    want = grad.stride(i) * grad.size(i);
+  }
+  if (!fold) d = grad.contiguous();
+  a.dout = d.data_ptr();
+  a.ldd = row_stride(d, "grad");
+  if (weight) {
+    check_here(*weight, "weight", grad);
+    TORCH_CHECK(weight->scalar_type() == grad.scalar_type() && weight->size(0) == 2 * N,
+                "weight must be [2 out_features, in_features] of grad's type");
+    a.K = weight->size(1);
+    a.weight = weight->data_ptr();
+    a.ldw = row_stride(*weight, "weight");
+    a.dx = dx.data_ptr();
+    a.lddx = a.K;
+  }
+  if (input) {
+    check_here(*input, "input", grad);
+    TORCH_CHECK(input->scalar_type() == grad.scalar_type(), "input must have grad's type");
+    TORCH_CHECK(!weight || weight->size(1) == input->size(-1), "weight must be [2 out_features, "
+                "in_features] with the input's last dimension as in_features");
+    a.K = input->size(-1);
+    TORCH_CHECK(a.K > 0 && input->numel() / a.K == a.M, "input must have grad's rows");
+    a.x = input->data_ptr();
+    a.ldx = row_stride(*input, "input");
+    a.dweight = dw.data_ptr();
+    a.lddw = a.K;
+  }
+  if (!weight && !input) a.K = 1;  // (no product)
+  if (bias_dtype) {
+    a.dbias_dtype = dtype_code(*bias_dtype);
+    a.dbias = db.data_ptr();
+  }
+  DevGuard g(grad.device());
+  const size_t need = mi355moe_gated_linear_backward_workspace_size(&a);
+  at::Tensor ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, o.dtype(at::kByte));
+  check_rc(mi355moe_gated_linear_backward(&a, need ? ws.data_ptr() : nullptr, need, cur_stream(grad)),
+           "gated_linear_backward");
+  return {dx, dw, db};
 }
 
 // ------------------------------------------------------------- grouped GEMM
@@ -1506,6 +1718,15 @@ TORCH_LIBRARY(_mi355_C, m) {
         "bool scale_ue8m0=False, bool is_scale_transposed=False) -> Tensor[]");
   m.def("linear_new(Tensor input, Tensor? input_scale, Tensor weight, Tensor? weight_scale, "
         "Tensor? bias, Tensor? residual, int activation, ScalarType out_dtype) -> Tensor");
+  m.def("linear_int8(Tensor! out, Tensor input, Tensor? input_scale, Tensor weight, "
+        "Tensor weight_scale, Tensor? bias, Tensor? residual, int activation) -> ()");
+  m.def("linear_int8_new(Tensor input, Tensor? input_scale, Tensor weight, Tensor weight_scale, "
+        "Tensor? bias, Tensor? residual, int activation, ScalarType out_dtype) -> Tensor");
+  m.def("per_token_int8_quant(Tensor input) -> (Tensor, Tensor)");
+  m.def("gated_linear(Tensor input, Tensor weight, Tensor? bias, int activation, bool keep) -> "
+        "(Tensor, Tensor)");
+  m.def("gated_linear_backward(Tensor grad, Tensor? input, Tensor? weight, Tensor z, "
+        "int activation, ScalarType? bias_dtype) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(_mi355_C, CUDA, m) {
@@ -1513,11 +1734,20 @@ TORCH_LIBRARY_IMPL(_mi355_C, CUDA, m) {
   m.impl("linear", &linear);
   m.impl("rms_norm_new", &rms_norm_new);
   m.impl("linear_new", &linear_new);
+  m.impl("linear_int8", &linear_int8);
+  m.impl("linear_int8_new", &linear_int8_new);
+  m.impl("per_token_int8_quant", &per_token_int8_quant);
+  m.impl("gated_linear", &gated_linear);
+  m.impl("gated_linear_backward", &gated_linear_backward);
 }
 
 TORCH_LIBRARY_IMPL(_mi355_C, Meta, m) {
-  for (const char* op : {"rms_norm", "linear"})
+  for (const char* op : {"rms_norm", "linear", "linear_int8"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&meta_noop>());
   m.impl("rms_norm_new", &rms_norm_new);
   m.impl("linear_new", &linear_new);
+  m.impl("linear_int8_new", &linear_int8_new);
+  m.impl("per_token_int8_quant", &per_token_int8_quant);
+  m.impl("gated_linear", &gated_linear);
+  m.impl("gated_linear_backward", &gated_linear_backward);
 }

@@ -158,7 +158,19 @@ class LinearArgs(ctypes.Structure):
                 ("ldw", ctypes.c_int64), ("weight_scale", ctypes.c_void_p),
                 ("weight_scale_row", ctypes.c_int64), ("weight_scale_blk", ctypes.c_int64),
                 ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
-                ("ldr", ctypes.c_int64), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64)]
+                ("ldr", ctypes.c_int64), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64),
+                ("weight_dtype", ctypes.c_int), ("z", ctypes.c_void_p)]
+
+
+class GatedLinearBackwardArgs(ctypes.Structure):
+    """mi355moe_gated_linear_backward_args."""
+    _fields_ = [("dtype", ctypes.c_int), ("dbias_dtype", ctypes.c_int),
+                ("activation", ctypes.c_int), ("M", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("K", ctypes.c_int64), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+                ("weight", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("z", ctypes.c_void_p),
+                ("dout", ctypes.c_void_p), ("ldd", ctypes.c_int64), ("dx", ctypes.c_void_p),
+                ("lddx", ctypes.c_int64), ("dweight", ctypes.c_void_p),
+                ("lddw", ctypes.c_int64), ("dbias", ctypes.c_void_p)]
 
 
 lib.mi355moe_rms_norm.argtypes = [ctypes.POINTER(RmsNormArgs), ctypes.c_void_p]
@@ -166,6 +178,15 @@ lib.mi355moe_linear.argtypes = [ctypes.POINTER(LinearArgs), ctypes.c_void_p, cty
                                 ctypes.c_void_p]
 lib.mi355moe_linear_workspace_size.restype = ctypes.c_size_t
 lib.mi355moe_linear_workspace_size.argtypes = [ctypes.POINTER(LinearArgs)]
+lib.mi355moe_int8_quant.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                    ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                    ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                    ctypes.c_void_p]
+lib.mi355moe_gated_linear_backward.argtypes = [ctypes.POINTER(GatedLinearBackwardArgs),
+                                               ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+lib.mi355moe_gated_linear_backward_workspace_size.restype = ctypes.c_size_t
+lib.mi355moe_gated_linear_backward_workspace_size.argtypes = [
+    ctypes.POINTER(GatedLinearBackwardArgs)]
 
 
 class StageTimer:

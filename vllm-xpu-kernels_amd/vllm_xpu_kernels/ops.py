@@ -276,10 +276,21 @@ def _no_grad_needed(*tensors) -> None:
                            "torch.no_grad() where no tangent is asked for")
 
 
+def _no_tangent(*tensors) -> None:
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("this operator has no forward-mode derivative")
+
+
 _rms_norm = torch.ops._mi355_C.rms_norm.default
 _rms_norm_new = torch.ops._mi355_C.rms_norm_new.default
 _linear = torch.ops._mi355_C.linear.default
 _linear_new = torch.ops._mi355_C.linear_new.default
+_linear_int8 = torch.ops._mi355_C.linear_int8.default
+_linear_int8_new = torch.ops._mi355_C.linear_int8_new.default
+_per_token_int8_quant = torch.ops._mi355_C.per_token_int8_quant.default
+_gated_linear = torch.ops._mi355_C.gated_linear.default
+_gated_linear_backward = torch.ops._mi355_C.gated_linear_backward.default
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -353,16 +364,16 @@ _LINEAR_ACT = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu2": 4, "silu_
 
 
 def _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
-                default_dtype):
+                default_dtype, op=_linear, op_new=_linear_new):
     code = _LINEAR_ACT.get(activation)
     if code is None:
         raise ValueError(f"Unsupported activation: {activation}.")
     if out is None:
-        return _linear_new(x, x_scale, weight, weight_scale, bias, residual, code,
-                           default_dtype if out_dtype is None else out_dtype)
+        return op_new(x, x_scale, weight, weight_scale, bias, residual, code,
+                      default_dtype if out_dtype is None else out_dtype)
     if out_dtype is not None and out.dtype != out_dtype:
         raise ValueError("out must have out_dtype")
-    _linear(out, x, x_scale, weight, weight_scale, bias, residual, code)
+    op(out, x, x_scale, weight, weight_scale, bias, residual, code)
     return out
 
 
@@ -399,6 +410,79 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     _no_grad_needed(x, x_scale, weight, weight_scale, bias, residual, out)
     return _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
                        torch.bfloat16)
+
+
+def per_token_int8_quant(x: torch.Tensor):
+    """Rows as int8 codes with a scale each: s = max(max |x|, 1e-10) / 127, q = x / s
+    to the nearest integer (halves to the even one), in fp32.  The input of
+    linear_int8 where several products share it, and once the weight of one (its
+    scales are then the output channels').
+
+    x [.., K] float32, bfloat16 or float16, columns contiguous, rows of one stride.
+    Returns (q int8 [.., K], scales float32 [.., 1]).  A row that holds an infinity
+    or a NaN has that scale and codes of zero: a product of it is NaN."""
+    _no_grad_needed(x)
+    return _per_token_int8_quant(x)
+
+
+def linear_int8(x: torch.Tensor, x_scale: Optional[torch.Tensor], weight: torch.Tensor,
+                weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear on int8 operands with a scale for each row of x and each row of the
+    weight: x [.., K] int8 with float32 x_scale [.., 1] or [rows]
+    (per_token_int8_quant), or bfloat16 / float16 with x_scale None, quantised in the
+    call; weight [N, K] int8 with float32 weight_scale [N] or [N, 1].  K < 131072.
+    The products' sums are exact integers, so a row's result does not depend on
+    the rows beside it.  out_dtype: a 16-bit x's type, else bfloat16, by default;
+    bfloat16, float16 or float32.  Everything else as linear."""
+    _no_grad_needed(x, x_scale, weight_scale, bias, residual, out)
+    return _run_linear(x, x_scale, weight, weight_scale, bias, activation, residual, out_dtype, out,
+                       torch.bfloat16 if x.dtype == torch.int8 else x.dtype,
+                       _linear_int8, _linear_int8_new)
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, code):
+        out, z = _gated_linear(x, weight, bias, code, True)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        ctx.save_for_backward(x if need_w else None, weight if need_x else None, z)
+        ctx.code = code
+        ctx.bias_dtype = bias.dtype if need_b else None
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, z = ctx.saved_tensors
+        dx, dw, db = _gated_linear_backward(grad, x, weight, z, ctx.code, ctx.bias_dtype)
+        return (None if weight is None else dx, None if x is None else dw,
+                None if ctx.bias_dtype is None else db, None)
+
+
+def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 activation: str = "silu_and_mul") -> torch.Tensor:
+    """f(x @ gate.T + bias_gate) * (x @ up.T + bias_up) in one kernel, with gradients of
+    x, weight and bias: the gated half of a feed-forward block in training.
+
+    x [.., K] and weight [2 N, K] (the gate's rows, then the factor's) bfloat16 or
+    float16, bias [2 N] float32, bfloat16 or float16.  activation: "silu_and_mul",
+    "gelu_and_mul", "gelu_tanh_and_mul".  Returns [.., N] of x's type.
+
+    Where a gradient is needed, the sums z (8 bytes for each of rows x N) are kept
+    for the backward pass, which computes the asked gradients alone (a frozen
+    weight's not at all): fp32 sums of products whose gradient of z is rounded to
+    x's type.  Reverse mode, once: no forward mode, no gradient of a gradient."""
+    code = _LINEAR_ACT.get(activation, 0)
+    if code < 5:
+        raise ValueError(f"Unsupported activation: {activation}.")
+    _no_tangent(x, weight, bias)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        return _GatedLinear.apply(x, weight, bias, code)
+    return _gated_linear(x, weight, bias, code, False)[0]
 
 
 def init_expert_map(num_experts: int, ep_rank: int, ep_size: int,

@@ -7,6 +7,8 @@
 
 namespace mi355 {
 
+// q is a workspace's: its rows are readable to a multiple of 8 columns, and along r they
+// hold zeros there.
 struct Product {
   int dtype;          // BF16 or F16
   bool transposed;    // q is [R, I], else [I, R]
@@ -27,6 +29,11 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 __device__ __forceinline__ uint2 lds_column4(const uint8_t* at) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)at));
 }
+
+// operands that direct copies to LDS can fetch (product_tile.hip)
+bool product_tile_supported(const Product& p);
+int product_tile_splits(const Product& p);
+int launch_product_tile(const Product& p, float* part, hipStream_t st);
 
 // bytes of partial sums (0: one pass), 16-byte aligned, that launch_product wants
 size_t product_workspace(const Product& p);

@@ -100,11 +100,14 @@ size_t partials(const Product& p, int splits) {
 
 }  // namespace
 
-size_t product_workspace(const Product& p) { return p.I ? partials(p, any_splits(p)) : 0; }
+size_t product_workspace(const Product& p) {
+  if (!p.I) return 0;
+  return partials(p, product_tile_supported(p) ? product_tile_splits(p) : any_splits(p));
+}
 
-int launch_product(const Product& p, void* sums, hipStream_t st) {
-  const int splits = any_splits(p), per = any_stages(p);
-  float* part = splits > 1 ? static_cast<float*>(sums) : nullptr;
+namespace {
+int launch_any(const Product& p, int splits, float* part, hipStream_t st) {
+  const int per = any_stages(p);
   const dim3 grid(static_cast<unsigned>(cdiv(p.J, PT)), static_cast<unsigned>(cdiv(p.I, PT)),
                   static_cast<unsigned>(splits));
   if (p.dtype == MI355MOE_F16) {
@@ -115,7 +118,16 @@ int launch_product(const Product& p, void* sums, hipStream_t st) {
     else product_any_kernel<false, false><<<grid, dim3(256), 0, st>>>(p, part, per);
   }
   MI_LAUNCH_CHECK();
-  if (splits == 1) return MI355MOE_OK;
+  return MI355MOE_OK;
+}
+}  // namespace
+
+int launch_product(const Product& p, void* sums, hipStream_t st) {
+  const bool tile = product_tile_supported(p);
+  const int splits = tile ? product_tile_splits(p) : any_splits(p);
+  float* part = splits > 1 ? static_cast<float*>(sums) : nullptr;
+  const int rc = tile ? launch_product_tile(p, part, st) : launch_any(p, splits, part, st);
+  if (rc || splits == 1) return rc;
   LinArgs f{};
   f.out_dtype = p.dtype;
   f.activation = MI355MOE_LINEAR_NONE;

@@ -26,7 +26,8 @@ HIP_SOURCES = ["routing.hip", "align.hip", "elementwise.hip", "moe_gemm.hip", "m
                "moe_gemm_big.hip", "moe_gemm_pipe.hip", "moe_gemm_stream.hip",
                "moe_gemm_wide.hip", "moe_gemm_wide8.hip", "moe_gemm_wide8p.hip", "moe_gemm_wide4.hip", "moe_gemm_big8.hip", "fused_moe.hip", "prologue.hip",
                "norm.hip", "linear.hip", "linear_skinny.hip",
-               "linear_tile.hip", "int8_quant.hip", "gated_backward.hip", "product.hip", "product_tile.hip", "errors.cpp"]
+               "linear_tile.hip", "int8_quant.hip", "gated_backward.hip", "product.hip", "product_tile.hip",
+               "linear_gemm.hip", "linear_gemm_keep.hip", "errors.cpp"]
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # no packed fp32 (v_pk_*_f32) code generation

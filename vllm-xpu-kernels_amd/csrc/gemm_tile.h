@@ -1,0 +1,559 @@
+// Tiles of a matrix product on operands that direct copies to LDS can fetch: BI x BJ
+// outputs, stages of 128 bytes of each operand's row.  out[i, j] = sum_r q(i, r) p(j, r):
+// a linear's x and weight lie along r (int8 and 16-bit operands); the products of a
+// backward pass have p, and maybe q, across it (16-bit operands).
+//
+// LDS.  A ring of NSTAGE stages.  An operand along r: the rows' 128 bytes one after the
+// other, 16-byte chunk c of row i at slot c ^ swz(i), so that the 16 rows of a quarter
+// of a fragment read cover all 64 banks once.  An operand across r: 64 rows of the
+// tile's columns as they are; the transposing LDS read gives each lane 4 r of its
+// column, two reads a fragment.  A group of 16 lanes reads 32 bytes of 4 rows, 32 lanes
+// 64 bytes of them, so chunks of consecutive rows are moved by 64 bytes (cross_swz): the
+// 4 rows then cover all 64 banks once.
+//
+// 32x32x16 (int8: 32x32x32) MFMAs, p as the A operand, so that a lane's sums are
+// consecutive columns of one row of out; four steps per stage, the next step's fragments
+// read while this one's MFMAs run; the barrier that publishes the next stage sits before
+// the last step.  Rows and columns past the edges repeat the last ones and are not
+// stored; the last stage's r past R are cleared in LDS.
+//
+// The epilogue takes the sums from the registers: a swap of half waves gives each lane 8
+// consecutive columns, stored 16 bytes (32 rows x 32 bytes) at a time; the scales of int8
+// and the biases wait in LDS, residuals are loaded one row of tiles ahead.  No LDS
+// of the ring is needed for that, so a workgroup takes tile after tile (`kPersistent`)
+// and the next one's first stages are on their way meanwhile.
+#pragma once
+
+#include "linear.h"
+#include "product.h"
+#include "tile.h"
+
+namespace mi355 {
+
+constexpr int GSB = 128;         // bytes of a stage along r
+__device__ __forceinline__ int gswz(int r) { return (r >> 1) & 7; }
+// across r: chunk c of row r is at slot c ^ cross_swz<chunks of a row>(r)
+template <int CH>
+__device__ __forceinline__ int cross_swz(int r) {
+  return CH >= 16 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
+}
+
+// What a tile does with its sums: E_RAW, as they are to a.out + split M N (float, int8:
+// int32); E_PLAIN, rounded to the operands' type; E_LINEAR, a linear's epilogue; E_KEEP, the
+// same of a gated one, and the sums with their biases to a.z.
+enum { E_RAW = 0, E_PLAIN = 1, E_LINEAR = 2, E_KEEP = 3 };
+
+// 8 sums of consecutive columns in each lane: lo holds columns 4 h .. 4 h + 3, hi 8 + 4 h ..;
+// lane half h gets columns 8 h .. 8 h + 7.
+template <typename V>
+__device__ __forceinline__ void gather8(const V& acc, int g, uint32_t (&o)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const auto lo = acc[8 * g + k], hi = acc[8 * g + 4 + k];
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, lo),
+                                                    __builtin_bit_cast(uint32_t, hi), false, false);
+    o[k] = r[0];
+    o[4 + k] = r[1];
+  }
+}
+
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE>
+__global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a, int tiles_i,
+                                                                  int tiles_j, int splits,
+                                                                  int stages_per_split) {
+  constexpr bool I8 = KIND == K_I8;
+  constexpr int EB = kind_bytes(KIND);
+  static_assert(!(I8 && (TQ || TP)) && !(GATED && TP) && !(TQ && !TP), "operands");
+  constexpr int WAVES = WI * WJ, THREADS = 64 * WAVES;
+  constexpr int MT = BI / WI / 32, NT = BJ / WJ / 32;
+  constexpr int NO = GATED ? NT / 2 : NT;                     // tiles of outputs
+  static_assert(MT >= 1 && NO >= 1 && (!GATED || NT % 2 == 0), "wave tile");
+  constexpr int BJO = GATED ? BJ / 2 : BJ;                    // output columns
+  constexpr int BR = GSB / EB;                                // r of a stage
+  constexpr int STAGE = (BI + BJ) * GSB;
+  constexpr int QCH = TQ ? BI / 8 : 8, PCH = TP ? BJ / 8 : 8;  // 16-byte chunks of a staged row
+  constexpr int QRC = 64 / QCH, PRC = 64 / PCH;               // rows of a 1 KB copy
+  constexpr int QQ = BI / 8 / WAVES, PQ = BJ / 8 / WAVES, ND = QQ + PQ;  // copies per wave and stage
+  static_assert(QQ * 8 * WAVES == BI && PQ * 8 * WAVES == BJ, "copies");
+  static_assert(!GATED || PQ % 2 == 0, "a copy has rows of one half");
+  constexpr bool LIN = EPI == E_LINEAR || EPI == E_KEEP;
+  constexpr int SIDE = (LIN ? BJ : 0) + (LIN && I8 ? BI + BJ : 0);  // floats: biases, scales
+  static_assert(NSTAGE * STAGE + SIDE * 4 <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NSTAGE * STAGE + SIDE * 4];
+  float* s_bias = reinterpret_cast<float*>(lds + NSTAGE * STAGE);  // [BJ]
+  float* s_ws = s_bias + BJ;                                       // [BJ]
+  float* s_xs = s_ws + BJ;                                         // [BI]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave / WJ, wj = wave % WJ;
+  const int g4 = lane >> 4, t16 = lane & 15, h = lane >> 5, l32 = lane & 31;
+
+  // Workgroups are dealt round-robin to the 8 XCDs: XCD i takes a contiguous range of
+  // tiles, in bands of 8 tiles of q, so that the tiles that run together on an XCD
+  // share rows of both operands in its L2.
+  const int total = tiles_i * tiles_j * splits;
+  const int per = (total + 7) / 8;
+  const int xcd = static_cast<int>(blockIdx.x) & 7, lanes8 = static_cast<int>(gridDim.x) >> 3;
+  const int xend = (xcd + 1) * per < total ? (xcd + 1) * per : total;
+  int t = xcd * per + (static_cast<int>(blockIdx.x) >> 3);
+  if (t >= xend) return;  // uniform
+
+  // p's rows (along r) of weight tile i, and its columns in the output
+  auto prow = [&](int i) __attribute__((always_inline)) {
+    if constexpr (GATED)
+      return i < NO ? wj * (BJO / WJ) + 32 * i : BJO + wj * (BJO / WJ) + 32 * (i - NO);
+    else
+      return wj * (BJ / WJ) + 32 * i;
+  };
+
+  // ---- a tile: its place, its stages, its copies' offsets
+  int64_t i0, j0;
+  int split, k0, nk, tail;  // tail: r of the last stage, 0: all
+  uint64_t qbase, pbase;
+  uint32_t voff[ND];
+  const uint64_t qstep = TQ ? static_cast<uint64_t>(a.ldx) * (2 * BR) : GSB;
+  const uint64_t pstep = TP ? static_cast<uint64_t>(a.ldw) * (2 * BR) : GSB;
+  const uint64_t uhalf = GATED ? static_cast<uint64_t>(a.N) * a.ldw * EB : 0;
+  auto row_of = [=](int q) __attribute__((always_inline)) {
+    if (q < QQ) return (wave * QQ + q) * QRC + lane / QCH;
+    // (gated: a wave's first copies are the gate's rows, its others the factor's)
+    if (GATED) return (wave * (PQ / 2) + (q - QQ) % (PQ / 2)) * PRC + lane / PCH;
+    return (wave * PQ + q - QQ) * PRC + lane / PCH;
+  };
+  auto place = [&](int tile) __attribute__((always_inline)) {
+    split = tile / (tiles_i * tiles_j);
+    tile %= tiles_i * tiles_j;
+    constexpr int BAND = 8;
+    const int band = tile / (BAND * tiles_j);
+    const int bi = tiles_i - band * BAND < BAND ? tiles_i - band * BAND : BAND;
+    tile -= band * BAND * tiles_j;
+    i0 = static_cast<int64_t>(band * BAND + tile % bi) * BI;
+    j0 = static_cast<int64_t>(tile / bi) * BJO;
+    const int nk_all = static_cast<int>((a.K + BR - 1) / BR);
+    k0 = split * stages_per_split;
+    nk = nk_all - k0 < stages_per_split ? nk_all - k0 : stages_per_split;
+    tail = k0 + nk == nk_all ? static_cast<int>(a.K % BR) : 0;
+    qbase = uniform64(reinterpret_cast<uint64_t>(a.x) + static_cast<uint64_t>((TQ ? i0 : i0 * a.ldx) * EB) + k0 * qstep);
+    pbase = uniform64(reinterpret_cast<uint64_t>(a.weight) + static_cast<uint64_t>((TP ? j0 : j0 * a.ldw) * EB) + k0 * pstep);
+    // (q across r: its rows are readable to a multiple of 8 columns)
+    const int qlast = static_cast<int>(((a.M + 7) / 8 - i0 / 8 < QCH ? (a.M + 7) / 8 - i0 / 8 : QCH) - 1);
+    const int plast = static_cast<int>((a.N / 8 - j0 / 8 < PCH ? a.N / 8 - j0 / 8 : PCH) - 1);
+#pragma unroll
+    for (int q = 0; q < ND; ++q) {
+      const int r = row_of(q);
+      const bool x = q < QQ;
+      const int64_t ld = x ? a.ldx : a.ldw;
+      if (x ? TQ : TP) {
+        const int c = x ? (lane % QCH) ^ cross_swz<QCH>(r) : (lane % PCH) ^ cross_swz<PCH>(r);
+        const int last = x ? qlast : plast;
+        voff[q] = static_cast<uint32_t>(r * ld * EB + ((c < last ? c : last) << 4));
+      } else {
+        const int64_t last = x ? a.M - 1 - i0 : a.N - 1 - j0;
+        voff[q] = static_cast<uint32_t>((r < last ? r : last) * ld * EB + (((lane % 8) ^ gswz(r)) << 4));
+      }
+    }
+  };
+
+  const uint32_t ring = lds_off(lds);
+  // copy Q into the slot at LDS offset `slot`; past: the stage holds `tail` r, rows behind
+  // them repeat the last, chunks behind them the stage's first
+  auto copy = [&](auto qc, uint64_t qoff, uint64_t poff, uint32_t slot, bool past)
+      __attribute__((always_inline)) {
+    constexpr int Q = decltype(qc)::value;
+    constexpr bool X = Q < QQ;
+    constexpr bool UP = GATED && !X && Q - QQ >= PQ / 2;
+    uint32_t v = voff[Q];
+    if (past) {  // uniform
+      const int r = row_of(Q);
+      if constexpr (X ? TQ : TP) {
+        if (r >= tail) v -= static_cast<uint32_t>((r - (tail - 1)) * (X ? a.ldx : a.ldw) * EB);
+      } else {
+        const int cb = ((lane % 8) ^ gswz(r)) << 4;
+        if (cb >= EB * tail) v -= cb;
+      }
+    }
+    if constexpr (X) dma16<Q * 1024>(v, qbase + qoff, slot + wave * (QQ * 1024));
+    else if constexpr (GATED)
+      dma16<BI * GSB + (UP ? BJO * GSB : 0) + ((Q - QQ) % (PQ / 2)) * 1024>(
+          v, pbase + poff + (UP ? uhalf : 0), slot + wave * (PQ / 2 * 1024));
+    else dma16<BI * GSB + (Q - QQ) * 1024>(v, pbase + poff, slot + wave * (PQ * 1024));
+  };
+  auto issue = [&](int kt) __attribute__((always_inline)) {
+    const uint32_t slot = ring + (kt % NSTAGE) * STAGE;
+    const bool past = tail != 0 && kt == nk - 1;
+    for_each<ND>([&](auto q) __attribute__((always_inline)) {
+      copy(q, static_cast<uint64_t>(kt) * qstep, static_cast<uint64_t>(kt) * pstep, slot, past);
+    });
+  };
+  auto first_stages = [&]() __attribute__((always_inline)) {
+    for (int s = 0; s < NSTAGE && s < nk; ++s) issue(s);
+  };
+  // the last stage's r behind `tail` (along r: whole chunks; a dz row holds zeros up to one)
+  auto clear_tail = [&](int kt) __attribute__((always_inline)) {
+    uint8_t* S = lds + (kt % NSTAGE) * STAGE;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto along = [&](uint8_t* s, int rows) __attribute__((always_inline)) {
+      for (int i = tid; i < rows * 8; i += THREADS) {
+        const int r = i >> 3, c = i & 7;
+        if ((c << 4) >= EB * tail) *reinterpret_cast<uint4*>(s + r * GSB + ((c ^ gswz(r)) << 4)) = zero;
+      }
+    };
+    auto across = [&](uint8_t* s, int ch) __attribute__((always_inline)) {
+      for (int i = tail * ch + tid; i < BR * ch; i += THREADS) reinterpret_cast<uint4*>(s)[i] = zero;
+    };
+    if constexpr (TQ) across(S, QCH);
+    else along(S, BI);
+    if constexpr (TP) across(S + BI * GSB, PCH);
+    else along(S + BI * GSB, BJ);
+    lds_barrier();
+  };
+  // publishes stage kt + 1; every wave has read stage kt then
+  auto advance = [&](int kt) __attribute__((always_inline)) {
+    if (kt + 1 >= nk) return;
+    if (kt + NSTAGE <= nk) wait_vm<ND * (NSTAGE - 2)>();
+    else wait_vm<0>();
+    lds_barrier();
+    if (tail && kt + 2 == nk) clear_tail(kt + 1);
+  };
+
+  // Where this lane reads fragment n of an operand: across r, row 8 h + t / 4 (then + 4) of
+  // a step, 4 columns from 16 (g & 1) + 4 (t & 3) of the fragment's 32; along r, chunk h of
+  // row l32.
+  auto cross_at = [&](auto ch, int col) __attribute__((always_inline)) {
+    constexpr int CH = decltype(ch)::value;
+    const int r = 8 * h + (t16 >> 2);
+    return r * (CH * 16) + (((col / 8) ^ cross_swz<CH>(r)) << 4) +
+           ((2 * (g4 & 1) + ((t16 & 3) >> 1)) << 4) + 8 * (t16 & 1);
+  };
+  int pat[NT], qat[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+    pat[i] = BI * GSB + (TP ? cross_at(std::integral_constant<int, PCH>{}, wj * (BJ / WJ) + 32 * i)
+                            : (prow(i) + l32) * GSB);
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+    qat[j] = TQ ? cross_at(std::integral_constant<int, QCH>{}, wi * (BI / WI) + 32 * j)
+                : (wi * (BI / WI) + 32 * j + l32) * GSB;
+  const int sw = gswz(l32);
+
+  constexpr int KS = 4;  // steps of 32 bytes along r
+  struct Frag {
+    uint4 q[MT], p[NT];
+  };
+  constexpr int NF = MT + NT;
+  auto cross8 = [&](const uint8_t* s, int row) __attribute__((always_inline)) {
+    const uint2 lo = lds_column4(s), hi = lds_column4(s + 4 * row);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
+  auto read = [&](Frag& o, const uint8_t* S, int ks, int e) __attribute__((always_inline)) {
+    const int c = ((2 * ks + h) ^ sw) << 4;
+    if (e == 0 || e > MT) {
+      const int i = e == 0 ? 0 : e - MT;
+      if constexpr (TP) o.p[i] = cross8(S + pat[i] + ks * (16 * PCH * 16), PCH * 16);
+      else o.p[i] = lds16(S + pat[i] + c);
+    } else {
+      if constexpr (TQ) o.q[e - 1] = cross8(S + qat[e - 1] + ks * (16 * QCH * 16), QCH * 16);
+      else o.q[e - 1] = lds16(S + qat[e - 1] + c);
+    }
+  };
+  using Acc = typename SumVec<KIND, 16>::T;
+  Acc acc[NT][MT];
+  constexpr int NM = NT * MT, RPM = (NF + NM - 1) / NM, CPM = (ND + NM - 1) / NM;
+  // One step: its MFMAs, between them the reads of the next step's fragments and, with
+  // `dma`, the copies of a stage; the order is kept.
+  auto step = [&](auto last_c, bool dma, const Frag& c, Frag& next, const uint8_t* Sn, int kn,
+                  uint64_t qoff, uint64_t poff, uint32_t slot) __attribute__((always_inline)) {
+    for_each<NM>([&](auto tc) __attribute__((always_inline)) {
+      constexpr int m = decltype(tc)::value, i = m / MT, j = m % MT;
+      acc[i][j] = mfma_32x32<KIND>(c.p[i], c.q[j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = m * RPM; e < (m + 1) * RPM && e < NF; ++e) read(next, Sn, kn, e);
+      if constexpr (decltype(last_c)::value && m * CPM < ND) {
+        if (dma) {
+          for_each<CPM>([&](auto cc) __attribute__((always_inline)) {
+            constexpr int Q = m * CPM + decltype(cc)::value;
+            if constexpr (Q < ND) copy(std::integral_constant<int, Q>{}, qoff, poff, slot, false);
+          });
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+
+  const bool mul16 = ((reinterpret_cast<uintptr_t>(a.out) |
+                              static_cast<uintptr_t>(a.ldo * (a.out_dtype == MI355MOE_F32 ? 4 : 2))) & 15) == 0;
+  [[maybe_unused]] const bool res16 = LIN && a.residual && a.residual_dtype != MI355MOE_F32 &&
+                     ((reinterpret_cast<uintptr_t>(a.residual) | static_cast<uintptr_t>(a.ldr * 2)) & 15) == 0;
+
+  place(t);
+  first_stages();
+  for (;;) {
+    // stage 0 (and what the tile before stored) is there
+    if (nk >= NSTAGE && t < xcd * per + lanes8) wait_vm<ND * (NSTAGE - 1)>();
+    else wait_vm<0>();
+    lds_barrier();
+    if (tail && nk == 1) clear_tail(0);
+    // biases and scales of this tile: every wave is done with the last one's
+    if constexpr (LIN) {
+      for (int i = tid; i < BJ; i += THREADS) {
+        const bool up = GATED && i >= BJO;
+        int64_t n = j0 + (up ? i - BJO : i);
+        n = (n < a.N ? n : a.N - 1) + (up ? a.N : 0);
+        s_bias[i] = a.bias ? ld_any(a.bias, a.bias_dtype, n) : 0.f;
+        if constexpr (I8) s_ws[i] = w_scale_of(a, n);
+      }
+      if constexpr (I8)
+        for (int i = tid; i < BI; i += THREADS) s_xs[i] = x_scale_of(a, i0 + i < a.M ? i0 + i : a.M - 1);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    {
+      Frag f[2];
+#pragma unroll
+      for (int e = 0; e < NF; ++e) read(f[0], lds, 0, e);
+      const int nfull = tail ? nk - 1 : nk;
+      uint64_t qoff = NSTAGE * qstep, poff = NSTAGE * pstep;
+      int slot = 0;
+      for (int kt = 0; kt < nk; ++kt) {
+        const uint8_t* S = lds + slot * STAGE;
+        const int nslot = slot + 1 == NSTAGE ? 0 : slot + 1;
+        const uint8_t* Sn = lds + nslot * STAGE;
+#pragma unroll
+        for (int ks = 0; ks + 1 < KS; ++ks)
+          step(std::false_type{}, false, f[ks & 1], f[(ks + 1) & 1], S, ks + 1, 0, 0, 0);
+        advance(kt);
+        if (tail && kt + NSTAGE == nk - 1) issue(kt + NSTAGE);
+        // after the last stage this reads a stale slot, unused
+        step(std::true_type{}, kt + NSTAGE < nfull, f[(KS - 1) & 1], f[0], Sn, 0, qoff, poff,
+             ring + slot * STAGE);
+        qoff += qstep;
+        poff += pstep;
+        slot = nslot;
+      }
+    }
+    const int64_t ti = i0, tj = j0;
+    const int tsplit = split;
+    const bool more = t + lanes8 < xend;  // uniform
+    lds_barrier();  // every wave has read the ring; biases and scales are there
+    t += lanes8;
+
+    // ---- epilogue
+    if constexpr (!LIN) {
+      if (more) {
+        place(t);
+        first_stages();
+      }
+      const int64_t part = static_cast<int64_t>(tsplit) * a.M * a.N;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const int64_t m = ti + wi * (BI / WI) + 32 * j + l32;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int gp = 0; gp < 2; ++gp) {
+            const int64_t n = tj + prow(i) + 16 * gp + 8 * h;
+            uint32_t v[8];
+            gather8(acc[i][j], gp, v);
+            if (m >= a.M || n >= a.N) continue;
+            if constexpr (EPI == E_PLAIN) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w[k] = pack16x2<KIND == K_F16>(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+              uint16_t* o = static_cast<uint16_t*>(a.out) + m * a.ldo + n;
+              if (mul16 && n + 8 <= a.N) {
+                *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (n + k < a.N) o[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
+              }
+              continue;
+            }
+            uint32_t* o = static_cast<uint32_t*>(a.out) + part + m * a.N + n;
+            if ((a.N & 3) == 0 && n + 8 <= a.N) {
+              reinterpret_cast<uint4*>(o)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+              reinterpret_cast<uint4*>(o)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (n + k < a.N) o[k] = v[k];
+            }
+          }
+      }
+    } else {
+      const bool full = mul16 && tj + BJO <= a.N;
+      const bool early = full && res16;
+      constexpr int RUNS = 2 * NO;
+      uint4 res[2][RUNS];
+      auto load_res = [&](uint4 (&r)[RUNS], int j) __attribute__((always_inline)) {
+        int64_t m = ti + wi * (BI / WI) + 32 * j + l32;
+        m = m < a.M ? m : a.M - 1;
+#pragma unroll
+        for (int e = 0; e < RUNS; ++e)
+          r[e] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) + m * a.ldr +
+                                                 tj + prow(e >> 1) + 16 * (e & 1) + 8 * h);
+      };
+      if (early) load_res(res[0], 0);
+      if (more) {
+        place(t);
+        first_stages();
+      }
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        if (early && j + 1 < MT) load_res(res[(j + 1) & 1], j + 1);
+        const int row = wi * (BI / WI) + 32 * j + l32;
+        const int64_t m = ti + row;
+        float xs = 0.f;
+        if constexpr (I8) xs = s_xs[row];
+#pragma unroll
+        for (int e = 0; e < RUNS; ++e) {
+          const int i = e >> 1, c = prow(i) + 16 * (e & 1) + 8 * h;
+          const int64_t n = tj + c;
+          float z[8], u[8];
+          auto sums = [&](const Acc& s, int col, float (&o)[8]) __attribute__((always_inline)) {
+            uint32_t v[8];
+            gather8(s, e & 1, v);
+            float b[8], w[8];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const float4 bb = *reinterpret_cast<const float4*>(s_bias + col + 4 * q);
+              b[4 * q] = bb.x; b[4 * q + 1] = bb.y; b[4 * q + 2] = bb.z; b[4 * q + 3] = bb.w;
+              if constexpr (I8) {
+                const float4 ww = *reinterpret_cast<const float4*>(s_ws + col + 4 * q);
+                w[4 * q] = ww.x; w[4 * q + 1] = ww.y; w[4 * q + 2] = ww.z; w[4 * q + 3] = ww.w;
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              if constexpr (I8) o[k] = static_cast<float>(static_cast<int>(v[k])) * (xs * w[k]) + b[k];
+              else o[k] = __uint_as_float(v[k]) + b[k];
+            }
+          };
+          sums(acc[i][j], c, z);
+          if constexpr (GATED) sums(acc[NO + i][j], BJO + c, u);
+          const bool on = m < a.M;
+          if constexpr (EPI == E_KEEP) {
+            float* zo = a.z + m * 2 * a.N + n;
+            if (on && full && (a.N & 3) == 0) {
+              st8_f32(zo, z, true);
+              st8_f32(zo + a.N, u, true);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (on && n + k < a.N) {
+                  zo[k] = z[k];
+                  zo[a.N + k] = u[k];
+                }
+            }
+          }
+          lin_act(a.activation, z);
+          if constexpr (GATED) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] *= u[k];
+          }
+          if (early) {
+            float r[8];
+            unpack8(res[j & 1][e], a.residual_dtype, r);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] += r[k];
+          } else if (a.residual) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (on && n + k < a.N) z[k] += ld_any(a.residual, a.residual_dtype, m * a.ldr + n + k);
+          }
+          if (!on) continue;
+          if (full) {
+            if (a.out_dtype == MI355MOE_F32) {
+              st8_f32(static_cast<float*>(a.out) + m * a.ldo + n, z, true);
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w[k] = a.out_dtype == MI355MOE_BF16 ? pack16x2<false>(z[2 * k], z[2 * k + 1])
+                                                    : pack16x2<true>(z[2 * k], z[2 * k + 1]);
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + m * a.ldo + n) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (n + k < a.N) st_any(a.out, a.out_dtype, m * a.ldo + n + k, z[k]);
+          }
+        }
+      }
+    }
+    if (!more) return;
+  }
+}
+
+// A choice of tiles.  us: time of one stage on every CU at once; per_cu: workgroups of
+// the tile that a CU holds; gated: takes both halves of a gated weight.
+enum TileShape { G256X256, G128X256, G128X128X2, G128X128, G64X128, G64X64 };
+struct TileSpec {
+  TileShape shape;
+  int bi, bj, per_cu;
+  bool gated;
+  float us;
+};
+struct TilePlan {
+  TileShape shape;
+  int splits, per;  // stages per split
+};
+// The tile and the split of r with the least estimated time for `rows` (of p) x I outputs of
+// `nk` stages: rounds of the grid over the CUs, each its stages and 3 us around them, and
+// for a split the partial sums written and read at 3.5 TB/s and a second launch.
+template <int N>
+TilePlan gemm_plan(const TileSpec (&tiles)[N], int64_t I, int64_t J, int64_t rows, int nk) {
+  constexpr int kMaxSplits = 16, kMaxSplitTiles = 1 << 16;
+  TilePlan best{};
+  double best_us = -1;
+  for (const TileSpec& c : tiles)
+    for (int s = 1; s <= kMaxSplits; ++s) {
+      const int per = static_cast<int>(cdiv(nk, s));
+      if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
+      const bool gates = rows != J && s == 1;  // a split product: all rows of p, no gates
+      if (gates && !c.gated) continue;
+      const double n = static_cast<double>(cdiv(I, c.bi)) * cdiv(gates ? J : rows, gates ? c.bj / 2 : c.bj) * s;
+      if (s > 1 && n > kMaxSplitTiles) continue;
+      double us = __builtin_ceil(n / (256.0 * c.per_cu)) * (c.us * per + 3.0);
+      if (s > 1) us += 4.0 + 2.0 * s * I * rows * 4 / 3.5e6;
+      if (best_us < 0 || us < best_us) {
+        best = {c.shape, s, per};
+        best_us = us;
+      }
+    }
+  return best;
+}
+
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE>
+int launch_gemm(const LinArgs& a, const TilePlan& p, int per_cu, hipStream_t st) {
+  const int64_t ti = cdiv(a.M, BI), tj = cdiv(a.N, GATED ? BJ / 2 : BJ), total = ti * tj * p.splits;
+  const int64_t most = 256 * per_cu;  // a workgroup takes the tiles this far apart in its XCD's range
+  const dim3 grid(static_cast<unsigned>(total < most ? cdiv(total, 8) * 8 : most));
+  gemm_tile_kernel<KIND, TQ, TP, GATED, EPI, BI, BJ, WI, WJ, NSTAGE>
+      <<<grid, dim3(64 * WI * WJ), 0, st>>>(a, static_cast<int>(ti), static_cast<int>(tj), p.splits, p.per);
+  MI_LAUNCH_CHECK();
+  return MI355MOE_OK;
+}
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI>
+int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
+  switch (p.shape) {
+    case G256X256: return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, 4, 2>(a, p, 1, st);
+    case G128X256: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 256, 2, 4, 3>(a, p, 1, st);
+    case G128X128X2: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 2>(a, p, 2, st);
+    case G128X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 4>(a, p, 1, st);
+    case G64X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 128, 2, 2, 4>(a, p, 1, st);
+    default:
+      if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 64, 2, 2, 8>(a, p, 1, st);
+      return set_error(MI355MOE_ERR_INVALID, "gemm: no such tile");
+  }
+}
+
+}  // namespace mi355

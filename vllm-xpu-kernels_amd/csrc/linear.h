@@ -266,21 +266,9 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
   }
 }
 
-// The same from the sums of int8 products; `raw`: a split's sums, as they are, into
-// the int32 partial sums at a.out.
+// The same from the sums of int8 products.
 __device__ __forceinline__ void lin_store8_i32(const LinArgs& a, int64_t m, int64_t n, const int* zp,
-                                               const int* up, bool vec, bool early = false,
-                                               uint4 res = uint4{}, bool raw = false) {
-  if (raw) {
-    int* o = static_cast<int*>(a.out) + m * a.ldo + n;
-    if (vec && n + 8 <= a.N) {
-      reinterpret_cast<int4*>(o)[0] = make_int4(zp[0], zp[1], zp[2], zp[3]);
-      reinterpret_cast<int4*>(o)[1] = make_int4(zp[4], zp[5], zp[6], zp[7]);
-    } else {
-      for (int k = 0; k < 8 && n + k < a.N; ++k) o[k] = zp[k];
-    }
-    return;
-  }
+                                               const int* up, bool vec) {
   const float xs = x_scale_of(a, m);
   float z[8], u[8];
 #pragma unroll
@@ -289,7 +277,7 @@ __device__ __forceinline__ void lin_store8_i32(const LinArgs& a, int64_t m, int6
     z[k] = static_cast<float>(zp[k]) * (xs * w_scale_of(a, c));
     u[k] = lin_gated(a.activation) ? static_cast<float>(up[k]) * (xs * w_scale_of(a, a.N + c)) : 0.f;
   }
-  lin_store8(a, m, n, z, u, vec, early, res);
+  lin_store8(a, m, n, z, u, vec);
 }
 
 // 16 bytes from column byte c of a row of `bytes` bytes, from any address;
@@ -321,5 +309,8 @@ int launch_linear_skinny(const LinArgs& a, hipStream_t st);
 bool linear_tile_supported(const LinArgs& a);
 int linear_tile_splits(const LinArgs& a);
 int launch_linear_tile(const LinArgs& a0, const LinArgs& a, hipStream_t st);
+// the same for int8 operands and for kept sums (linear_gemm.hip)
+int linear_gemm_splits(const LinArgs& a);
+int launch_linear_gemm(const LinArgs& a0, const LinArgs& a, hipStream_t st);
 
 }  // namespace mi355

@@ -8,7 +8,7 @@
 // NSTAGE stages; stage kt + NSTAGE is requested as soon as every wave has read
 // stage kt, so NSTAGE - 1 stages are in flight.
 //
-// 16-bit operands: 32x32x16 MFMAs (int8: 32x32x32, the same bytes), four K steps per stage, the next step's
+// 16-bit operands: 32x32x16 MFMAs, four K steps per stage, the next step's
 // fragments read while this one's MFMAs run; the barrier that publishes stage
 // kt + 1 sits before the last step of stage kt, so that the matrix cores do not
 // start a stage behind its reads.
@@ -17,8 +17,6 @@
 // zero, each result times x_scale * weight_scale added to the sum.  EXACT
 // (float32 outputs): the fragments become bf16 and 16x16x32 MFMAs add them
 // (linear.h says what the 128-long one loses).
-//
-// int8 sums stay int32 until the epilogue, which applies both scales.
 //
 // Padding.  Rows past the edges repeat the last one, their results are not
 // stored; the last stage's columns past K are cleared in LDS.
@@ -34,18 +32,18 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+
 constexpr int SB = 128;  // bytes of a row in a K stage: one e4m3 scale block, 64 16-bit values
 // slot of 16-byte chunk c of row r: c ^ swz(r)
 __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 
-// KEEP: the sums go to a.z too.
-template <int KIND, bool GATED, bool UNI, bool KEEP, int BM, int BN, int WM, int WN, int NSTAGE>
+template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int NSTAGE>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs a, int tiles_m,
                                                                     int tiles_n, int splits,
                                                                     int stages_per_split) {
-  constexpr bool FP8 = kind_fp8(KIND), I8 = KIND == K_I8;
+  constexpr bool FP8 = KIND >= K_FP8;
   static_assert(FP8 || UNI, "scale blocks");
-  constexpr int EB = kind_bytes(KIND);
+  constexpr int EB = FP8 ? 1 : 2;
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   constexpr int TS = FP8 ? 16 : 32;              // MFMA tile side
   constexpr int MT = BM / WM / TS, NT = BN / WN / TS;
@@ -202,16 +200,15 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
     if (tail && kt + 2 == nk) clear_tail(kt + 1);
   };
 
+  using Acc = std::conditional_t<FP8, f32x4, f32x16>;
   constexpr int AR = FP8 ? 4 : 16;
-  using Acc = typename SumVec<KIND, AR>::T;
-  using Acc4 = typename SumVec<KIND, 4>::T;
   Acc acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int r = 0; r < AR; ++r) acc[i][j][r] = 0;
+      for (int r = 0; r < AR; ++r) acc[i][j][r] = 0.f;
 
   // weight tile i's first row in the stage: gated waves take the same columns
   // of both halves
@@ -223,7 +220,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
   };
 
   if constexpr (!FP8) {
-    constexpr int KS = SB / 32;  // K steps of 32 bytes per stage
+    constexpr int KS = SB / 32;  // K steps of 16 per stage
     const int l32 = lane & 31, h = lane >> 5;
     struct Frag {
       uint4 x[MT], w[NT];
@@ -250,7 +247,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
                     uint64_t koff, uint32_t slot) __attribute__((always_inline)) {
       for_each<NM>([&](auto tc) __attribute__((always_inline)) {
         constexpr int t = decltype(tc)::value, i = t / MT, j = t % MT;
-        acc[i][j] = mfma_32x32<KIND>(g.w[i], g.x[j], acc[i][j]);
+        acc[i][j] = mfma16_32x32x16<KIND == K_F16>(g.w[i], g.x[j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = t * RPM; e < (t + 1) * RPM && e < NF; ++e) read(next, Sn, kn, e);
@@ -432,8 +429,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
 #pragma unroll
         for (int g = 0; g < AR / 4; ++g) {
           const int col = wrow(i) + (FP8 ? 4 * (lane >> 4) : 8 * g + 4 * (lane >> 5));
-          *reinterpret_cast<Acc4*>(ep + row * EP + col) =
-              Acc4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+          *reinterpret_cast<f32x4*>(ep + row * EP + col) =
+              f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
         }
     }
     lds_barrier();
@@ -444,12 +441,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(const LinArgs
       const int64_t m = mp + row, n = n0 + c;
       if (m >= a.M || n >= a.N) continue;
       const float* z = ep + row * EP + c;
-      if constexpr (I8) {
-        const int* zi = reinterpret_cast<const int*>(z);
-        lin_store8_i32(o, m, n, zi, zi + (GATED ? BNO : 0), vec, early, res[e], splits > 1);
-      } else {
-        lin_store8<KEEP>(o, m, n, z, z + (GATED ? BNO : 0), vec, early, res[e]);
-      }
+      lin_store8(o, m, n, z, z + (GATED ? BNO : 0), vec, early, res[e]);
     }
   }
 }
@@ -494,7 +486,6 @@ constexpr Tile kTiles8[] = {
 constexpr Tile kTiles8Exact[] = {
     {T128X256, 128, 256, 1, true, 1.94f}, {T128X128X2, 128, 128, 1, true, 1.32f},
     {T64X128, 64, 128, 1, true, 0.85f}, {T64X64, 64, 64, 1, true, 0.59f}};
-// int8: the 16-bit kernels' stages, of twice as many k.
 constexpr int kMaxSplits = 16;
 constexpr int kMaxSplitTiles = 1 << 16;  // workgroups of a split product: far more than fill the CUs
 
@@ -512,7 +503,7 @@ bool uniform_scales(const LinArgs& a) { return !lin_gated(a.activation) || a.N %
 Plan plan(const LinArgs& a) {
   const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
   const bool exact = fp8 && a.out_dtype == MI355MOE_F32;
-  const int nk = static_cast<int>(cdiv(a.K * kind_bytes(kind_of(a)), 128));
+  const int nk = static_cast<int>(cdiv(a.K * (fp8 ? 1 : 2), 128));
   const bool g = lin_gated(a.activation);
   const double rows = static_cast<double>(lin_rows(a));
   Plan best{};
@@ -548,14 +539,7 @@ template <int KIND, bool GATED, bool UNI, int BM, int BN, int WM, int WN, int NS
 int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
   const int tm = static_cast<int>(cdiv(a.M, BM)), tn = static_cast<int>(cdiv(a.N, GATED ? BN / 2 : BN));
   const dim3 grid(static_cast<unsigned>(cdiv(static_cast<int64_t>(tm) * tn * p.splits, 8) * 8));
-  if constexpr (GATED && (KIND == K_BF16 || KIND == K_F16))
-    if (a.z) {
-      linear_tile_kernel<KIND, GATED, UNI, true, BM, BN, WM, WN, NSTAGE>
-          <<<grid, dim3(64 * WM * WN), 0, st>>>(a, tm, tn, p.splits, p.per);
-      MI_LAUNCH_CHECK();
-      return MI355MOE_OK;
-    }
-  linear_tile_kernel<KIND, GATED, UNI, false, BM, BN, WM, WN, NSTAGE>
+  linear_tile_kernel<KIND, GATED, UNI, BM, BN, WM, WN, NSTAGE>
       <<<grid, dim3(64 * WM * WN), 0, st>>>(a, tm, tn, p.splits, p.per);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
@@ -563,19 +547,19 @@ int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
 
 template <int KIND, bool GATED, int BM, int BN, int WM, int WN, int NSTAGE>
 int launch_uni(const LinArgs& a, const Plan& p, hipStream_t st) {
-  if constexpr (kind_fp8(KIND))
+  if constexpr (KIND >= K_FP8)
     if (!uniform_scales(a)) return launch<KIND, GATED, false, BM, BN, WM, WN, NSTAGE>(a, p, st);
   return launch<KIND, GATED, true, BM, BN, WM, WN, NSTAGE>(a, p, st);
 }
 
 template <int KIND, bool GATED>
 int launch_tiles(const LinArgs& a, const Plan& p, hipStream_t st) {
-  if constexpr (!kind_fp8(KIND)) {
+  if constexpr (KIND < K_FP8) {
     if (p.shape == T256X256) return launch_uni<KIND, GATED, 256, 256, 2, 4, 2>(a, p, st);
     if constexpr (!GATED)
       if (p.shape == T96X128) return launch_uni<KIND, GATED, 96, 128, 1, 4, 4>(a, p, st);
   }
-  if constexpr (kind_fp8(KIND) || !GATED)
+  if constexpr (KIND >= K_FP8 || !GATED)
     if (p.shape == T64X64) return launch_uni<KIND, GATED, 64, 64, 2, 2, 8>(a, p, st);
   if constexpr (KIND != K_FP8_EXACT)
     if (p.shape == T128X128) return launch_uni<KIND, GATED, 128, 128, 2, 2, 4>(a, p, st);
@@ -609,17 +593,21 @@ bool linear_tile_supported(const LinArgs& a) {
   return cdiv(a.M, 64) * cdiv(lin_rows(a), 64) < (int64_t(1) << 24);
 }
 
-int linear_tile_splits(const LinArgs& a) { return plan(a).splits; }
+// int8 operands and kept sums: gemm_tile.h's kernels
+bool gemm_tiles(const LinArgs& a) { return a.x_dtype == MI355MOE_I8 || a.z; }
+
+int linear_tile_splits(const LinArgs& a) {
+  return gemm_tiles(a) ? linear_gemm_splits(a) : plan(a).splits;
+}
 
 int launch_linear_tile(const LinArgs& a0, const LinArgs& a, hipStream_t st) {
+  if (gemm_tiles(a0)) return launch_linear_gemm(a0, a, st);
   const Plan p = plan(a0);
   const bool g = lin_gated(a.activation);
   if (a.x_dtype == MI355MOE_FP8E4M3 && a0.out_dtype == MI355MOE_F32)
     return g ? launch_tiles<K_FP8_EXACT, true>(a, p, st) : launch_tiles<K_FP8_EXACT, false>(a, p, st);
   if (a.x_dtype == MI355MOE_FP8E4M3)
     return g ? launch_tiles<K_FP8, true>(a, p, st) : launch_tiles<K_FP8, false>(a, p, st);
-  if (a.x_dtype == MI355MOE_I8)
-    return g ? launch_tiles<K_I8, true>(a, p, st) : launch_tiles<K_I8, false>(a, p, st);
   if (a.x_dtype == MI355MOE_F16)
     return g ? launch_tiles<K_F16, true>(a, p, st) : launch_tiles<K_F16, false>(a, p, st);
   return g ? launch_tiles<K_BF16, true>(a, p, st) : launch_tiles<K_BF16, false>(a, p, st);

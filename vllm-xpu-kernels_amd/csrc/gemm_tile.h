@@ -57,8 +57,26 @@ __device__ __forceinline__ void gather8(const V& acc, int g, uint32_t (&o)[8]) {
   }
 }
 
+// Two runs of 8 columns, a of columns 8 h .. and b of 16 + 8 h .. of row l32: a swap of
+// 16-lane groups gives runs whose lanes cover 32 columns of 16 rows (64 bytes of 16-bit
+// outputs instead of 32): columns 16 (g & 1) + 8 (g / 2) .. of row t16 in a, of row
+// 16 + t16 in b (g, t16: the lane's group of 16 and its place there).  Its own inverse.
+template <int N>
+__device__ __forceinline__ void pair16(uint32_t (&a)[N], uint32_t (&b)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a[k], b[k], false, false);
+    a[k] = r[0];
+    b[k] = r[1];
+  }
+}
+
+// (two workgroups to a CU where their LDS fits: at most 256 registers then)
+constexpr int gemm_waves_per_simd(int waves, int bi, int bj, int stages) {
+  return (waves / 4) * (2 * (stages * (bi + bj) * GSB + 4 * (2 * bj + bi)) <= 160 * 1024 ? 2 : 1);
+}
 template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE>
-__global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a, int tiles_i,
+__global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, NSTAGE)) void gemm_tile_kernel(const LinArgs a, int tiles_i,
                                                                   int tiles_j, int splits,
                                                                   int stages_per_split) {
   constexpr bool I8 = KIND == K_I8;
@@ -90,7 +108,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a
   const int g4 = lane >> 4, t16 = lane & 15, h = lane >> 5, l32 = lane & 31;
 
   // Workgroups are dealt round-robin to the 8 XCDs: XCD i takes a contiguous range of
-  // tiles, in bands of 8 tiles of q, so that the tiles that run together on an XCD
+  // tiles, in bands of 4 tiles of q, so that the tiles that run together on an XCD
   // share rows of both operands in its L2.
   const int total = tiles_i * tiles_j * splits;
   const int per = (total + 7) / 8;
@@ -124,11 +142,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a
   auto place = [&](int tile) __attribute__((always_inline)) {
     split = tile / (tiles_i * tiles_j);
     tile %= tiles_i * tiles_j;
-    constexpr int BAND = 8;
-    const int band = tile / (BAND * tiles_j);
-    const int bi = tiles_i - band * BAND < BAND ? tiles_i - band * BAND : BAND;
-    tile -= band * BAND * tiles_j;
-    i0 = static_cast<int64_t>(band * BAND + tile % bi) * BI;
+    constexpr int band_rows = 4;
+    const int band = tile / (band_rows * tiles_j);
+    const int bi = tiles_i - band * band_rows < band_rows ? tiles_i - band * band_rows : band_rows;
+    tile -= band * band_rows * tiles_j;
+    i0 = static_cast<int64_t>(band * band_rows + tile % bi) * BI;
     j0 = static_cast<int64_t>(tile / bi) * BJO;
     const int nk_all = static_cast<int>((a.K + BR - 1) / BR);
     k0 = split * stages_per_split;
@@ -289,10 +307,14 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a
 
   place(t);
   first_stages();
+  enum { NONE, SOME, WHOLE } behind = NONE;  // stores of the tile before
   for (;;) {
-    // stage 0 (and what the tile before stored) is there
-    if (nk >= NSTAGE && t < xcd * per + lanes8) wait_vm<ND * (NSTAGE - 1)>();
-    else wait_vm<0>();
+    // Stage 0 is there.  A whole tile's stores, issued behind these copies, may still be on
+    // their way: one at least for each of the wave's runs.
+    constexpr int LATER = ND * (NSTAGE - 1);
+    if (nk < NSTAGE || behind == SOME) wait_vm<0>();
+    else if (behind == NONE) wait_vm<LATER>();
+    else wait_vm<(LATER + 2 * NO * MT < 63 ? LATER + 2 * NO * MT : 63)>();
     lds_barrier();
     if (tail && nk == 1) clear_tail(0);
     // biases and scales of this tile: every wave is done with the last one's
@@ -340,151 +362,211 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a
     const int64_t ti = i0, tj = j0;
     const int tsplit = split;
     const bool more = t + lanes8 < xend;  // uniform
+    behind = mul16 && ti + BI <= a.M && tj + BJO <= a.N ? WHOLE : SOME;
     lds_barrier();  // every wave has read the ring; biases and scales are there
     t += lanes8;
 
     // ---- epilogue
+    const int xrow = wi * (BI / WI) + t16, xcol = 16 * (g4 & 1) + 8 * (g4 >> 1);  // see pair16
     if constexpr (!LIN) {
       if (more) {
         place(t);
         first_stages();
       }
       const int64_t part = static_cast<int64_t>(tsplit) * a.M * a.N;
+      const bool full = tj + BJ <= a.N && (EPI == E_PLAIN ? mul16 : (a.N & 3) == 0);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int64_t m = ti + wi * (BI / WI) + 32 * j + l32;
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NT; ++i) {
+          const int64_t m = ti + xrow + 32 * j, n = tj + prow(i) + xcol;
+          uint32_t v[2][8];
+          gather8(acc[i][j], 0, v[0]);
+          gather8(acc[i][j], 1, v[1]);
+          if constexpr (EPI == E_PLAIN) {
+            uint32_t w[2][4];
 #pragma unroll
-          for (int gp = 0; gp < 2; ++gp) {
-            const int64_t n = tj + prow(i) + 16 * gp + 8 * h;
-            uint32_t v[8];
-            gather8(acc[i][j], gp, v);
-            if (m >= a.M || n >= a.N) continue;
-            if constexpr (EPI == E_PLAIN) {
-              uint32_t w[4];
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                w[k] = pack16x2<KIND == K_F16>(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
-              uint16_t* o = static_cast<uint16_t*>(a.out) + m * a.ldo + n;
-              if (mul16 && n + 8 <= a.N) {
-                *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+                w[e][k] = pack16x2<KIND == K_F16>(__uint_as_float(v[e][2 * k]), __uint_as_float(v[e][2 * k + 1]));
+            pair16(w[0], w[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (m + 16 * e >= a.M) continue;
+              uint16_t* o = static_cast<uint16_t*>(a.out) + (m + 16 * e) * a.ldo + n;
+              if (full) {
+                *reinterpret_cast<uint4*>(o) = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
               } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                  if (n + k < a.N) o[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
+                  if (n + k < a.N) o[k] = static_cast<uint16_t>(w[e][k >> 1] >> (16 * (k & 1)));
               }
-              continue;
             }
-            uint32_t* o = static_cast<uint32_t*>(a.out) + part + m * a.N + n;
-            if ((a.N & 3) == 0 && n + 8 <= a.N) {
-              reinterpret_cast<uint4*>(o)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-              reinterpret_cast<uint4*>(o)[1] = make_uint4(v[4], v[5], v[6], v[7]);
-            } else {
+          } else {
+            pair16(v[0], v[1]);
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (n + k < a.N) o[k] = v[k];
+            for (int e = 0; e < 2; ++e) {
+              if (m + 16 * e >= a.M) continue;
+              uint32_t* o = static_cast<uint32_t*>(a.out) + part + (m + 16 * e) * a.N + n;
+              if (full) {
+                reinterpret_cast<uint4*>(o)[0] = make_uint4(v[e][0], v[e][1], v[e][2], v[e][3]);
+                reinterpret_cast<uint4*>(o)[1] = make_uint4(v[e][4], v[e][5], v[e][6], v[e][7]);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (n + k < a.N) o[k] = v[e][k];
+              }
             }
           }
-      }
+        }
     } else {
       const bool full = mul16 && tj + BJO <= a.N;
       const bool early = full && res16;
+      // Residuals: all at once where 8 runs of 16 bytes hold them, else one row of tiles
+      // ahead (memory operations end in order: a load behind stores waits for them).
       constexpr int RUNS = 2 * NO;
-      uint4 res[2][RUNS];
-      auto load_res = [&](uint4 (&r)[RUNS], int j) __attribute__((always_inline)) {
-        int64_t m = ti + wi * (BI / WI) + 32 * j + l32;
-        m = m < a.M ? m : a.M - 1;
+      constexpr bool ALL = RUNS * MT <= 8;
+      uint32_t res[ALL ? MT : 2][RUNS][4];
+      auto load_res = [&](uint32_t (&r)[RUNS][4], int j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < RUNS; ++e)
-          r[e] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) + m * a.ldr +
-                                                 tj + prow(e >> 1) + 16 * (e & 1) + 8 * h);
+        for (int e = 0; e < RUNS; ++e) {
+          int64_t m = ti + xrow + 32 * j + 16 * (e & 1);
+          m = m < a.M ? m : a.M - 1;
+          const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) +
+                                                          m * a.ldr + tj + prow(e >> 1) + xcol);
+          r[e][0] = v.x; r[e][1] = v.y; r[e][2] = v.z; r[e][3] = v.w;
+        }
       };
-      if (early) load_res(res[0], 0);
+      if (early) {
+#pragma unroll
+        for (int j = 0; j < (ALL ? MT : 1); ++j) load_res(res[j], j);
+      }
       if (more) {
         place(t);
         first_stages();
       }
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        if (early && j + 1 < MT) load_res(res[(j + 1) & 1], j + 1);
+        if (!ALL && early && j + 1 < MT) load_res(res[(j + 1) & 1], j + 1);
         const int row = wi * (BI / WI) + 32 * j + l32;
         const int64_t m = ti + row;
+        const bool on = m < a.M;
         float xs = 0.f;
         if constexpr (I8) xs = s_xs[row];
 #pragma unroll
-        for (int e = 0; e < RUNS; ++e) {
-          const int i = e >> 1, c = prow(i) + 16 * (e & 1) + 8 * h;
-          const int64_t n = tj + c;
-          float z[8], u[8];
-          auto sums = [&](const Acc& s, int col, float (&o)[8]) __attribute__((always_inline)) {
-            uint32_t v[8];
-            gather8(s, e & 1, v);
-            float b[8], w[8];
+        for (int i = 0; i < NO; ++i) {
+          uint32_t (&r0)[4] = res[ALL ? j : j & 1][2 * i];
+          uint32_t (&r1)[4] = res[ALL ? j : j & 1][2 * i + 1];
+          if (early) pair16(r0, r1);
+          float y[2][8];
+          [[maybe_unused]] uint32_t kz[2][8], ku[2][8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const float4 bb = *reinterpret_cast<const float4*>(s_bias + col + 4 * q);
-              b[4 * q] = bb.x; b[4 * q + 1] = bb.y; b[4 * q + 2] = bb.z; b[4 * q + 3] = bb.w;
-              if constexpr (I8) {
-                const float4 ww = *reinterpret_cast<const float4*>(s_ws + col + 4 * q);
-                w[4 * q] = ww.x; w[4 * q + 1] = ww.y; w[4 * q + 2] = ww.z; w[4 * q + 3] = ww.w;
+          for (int e = 0; e < 2; ++e) {
+            const int c = prow(i) + 16 * e + 8 * h;
+            const int64_t n = tj + c;
+            float(&z)[8] = y[e];
+            float u[8];
+            auto sums = [&](const Acc& s, int col, float (&o)[8]) __attribute__((always_inline)) {
+              uint32_t v[8];
+              gather8(s, e, v);
+              float b[8], w[8];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const float4 bb = *reinterpret_cast<const float4*>(s_bias + col + 4 * q);
+                b[4 * q] = bb.x; b[4 * q + 1] = bb.y; b[4 * q + 2] = bb.z; b[4 * q + 3] = bb.w;
+                if constexpr (I8) {
+                  const float4 ww = *reinterpret_cast<const float4*>(s_ws + col + 4 * q);
+                  w[4 * q] = ww.x; w[4 * q + 1] = ww.y; w[4 * q + 2] = ww.z; w[4 * q + 3] = ww.w;
+                }
+              }
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                if constexpr (I8) o[k] = static_cast<float>(static_cast<int>(v[k])) * (xs * w[k]) + b[k];
+                else o[k] = __uint_as_float(v[k]) + b[k];
+              }
+            };
+            sums(acc[i][j], c, z);
+            if constexpr (GATED) sums(acc[NO + i][j], BJO + c, u);
+            if constexpr (EPI == E_KEEP) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                kz[e][k] = __float_as_uint(z[k]);
+                ku[e][k] = __float_as_uint(u[k]);
               }
             }
+            lin_act(a.activation, z);
+            if constexpr (GATED) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              if constexpr (I8) o[k] = static_cast<float>(static_cast<int>(v[k])) * (xs * w[k]) + b[k];
-              else o[k] = __uint_as_float(v[k]) + b[k];
+              for (int k = 0; k < 8; ++k) z[k] *= u[k];
             }
-          };
-          sums(acc[i][j], c, z);
-          if constexpr (GATED) sums(acc[NO + i][j], BJO + c, u);
-          const bool on = m < a.M;
-          if constexpr (EPI == E_KEEP) {
-            float* zo = a.z + m * 2 * a.N + n;
-            if (on && full && (a.N & 3) == 0) {
-              st8_f32(zo, z, true);
-              st8_f32(zo + a.N, u, true);
+            if (early) {
+              float r[8];
+              const uint32_t(&rr)[4] = e ? r1 : r0;
+              unpack8(make_uint4(rr[0], rr[1], rr[2], rr[3]), a.residual_dtype, r);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) z[k] += r[k];
+            } else if (a.residual) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (on && n + k < a.N) z[k] += ld_any(a.residual, a.residual_dtype, m * a.ldr + n + k);
+            }
+          }
+          const int64_t mx = ti + xrow + 32 * j, n = tj + prow(i) + xcol;
+          // 8 floats of lane row mx + 16 e
+          auto put = [&](float* o, const uint32_t (&v)[8], bool vec) __attribute__((always_inline)) {
+            if (vec) {
+              reinterpret_cast<uint4*>(o)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+              reinterpret_cast<uint4*>(o)[1] = make_uint4(v[4], v[5], v[6], v[7]);
             } else {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                if (on && n + k < a.N) {
-                  zo[k] = z[k];
-                  zo[a.N + k] = u[k];
-                }
+                if (n + k < a.N) o[k] = __uint_as_float(v[k]);
             }
-          }
-          lin_act(a.activation, z);
-          if constexpr (GATED) {
+          };
+          if constexpr (EPI == E_KEEP) {
+            pair16(kz[0], kz[1]);
+            pair16(ku[0], ku[1]);
+            const bool vec = tj + BJO <= a.N && (a.N & 3) == 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] *= u[k];
+            for (int e = 0; e < 2; ++e)
+              if (mx + 16 * e < a.M) {
+                float* zo = a.z + (mx + 16 * e) * 2 * a.N + n;
+                put(zo, kz[e], vec);
+                put(zo + a.N, ku[e], vec);
+              }
           }
-          if (early) {
-            float r[8];
-            unpack8(res[j & 1][e], a.residual_dtype, r);
+          if (a.out_dtype == MI355MOE_F32) {
+            uint32_t w[2][8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) z[k] += r[k];
-          } else if (a.residual) {
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (on && n + k < a.N) z[k] += ld_any(a.residual, a.residual_dtype, m * a.ldr + n + k);
-          }
-          if (!on) continue;
-          if (full) {
-            if (a.out_dtype == MI355MOE_F32) {
-              st8_f32(static_cast<float*>(a.out) + m * a.ldo + n, z, true);
-            } else {
-              uint32_t w[4];
+              for (int k = 0; k < 8; ++k) w[e][k] = __float_as_uint(y[e][k]);
+            pair16(w[0], w[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (mx + 16 * e < a.M) put(static_cast<float*>(a.out) + (mx + 16 * e) * a.ldo + n, w[e], full);
+          } else {
+            uint32_t w[2][4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                w[k] = a.out_dtype == MI355MOE_BF16 ? pack16x2<false>(z[2 * k], z[2 * k + 1])
-                                                    : pack16x2<true>(z[2 * k], z[2 * k + 1]);
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + m * a.ldo + n) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
+                w[e][k] = a.out_dtype == MI355MOE_BF16 ? pack16x2<false>(y[e][2 * k], y[e][2 * k + 1])
+                                                       : pack16x2<true>(y[e][2 * k], y[e][2 * k + 1]);
+            pair16(w[0], w[1]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (n + k < a.N) st_any(a.out, a.out_dtype, m * a.ldo + n + k, z[k]);
+            for (int e = 0; e < 2; ++e) {
+              if (mx + 16 * e >= a.M) continue;
+              uint16_t* o = static_cast<uint16_t*>(a.out) + (mx + 16 * e) * a.ldo + n;
+              if (full) {
+                *reinterpret_cast<uint4*>(o) = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (n + k < a.N) o[k] = static_cast<uint16_t>(w[e][k >> 1] >> (16 * (k & 1)));
+              }
+            }
           }
         }
       }
@@ -493,22 +575,21 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_tile_kernel(const LinArgs a
   }
 }
 
-// A choice of tiles.  us: time of one stage on every CU at once; per_cu: workgroups of
-// the tile that a CU holds; gated: takes both halves of a gated weight.
-enum TileShape { G256X256, G128X256, G128X128X2, G128X128, G64X128, G64X64 };
+// A choice of tiles.  us: time of one stage on every CU at once, round: of the rest of a
+// round of tiles (first copies, epilogue); per_cu: workgroups of the tile that a CU holds.
+enum TileShape { G256X256, G256X128, G128X256, G128X128X2, G128X128, G64X128, G64X64 };
 struct TileSpec {
   TileShape shape;
   int bi, bj, per_cu;
-  bool gated;
-  float us;
+  float us, round;
 };
 struct TilePlan {
   TileShape shape;
   int splits, per;  // stages per split
 };
-// The tile and the split of r with the least estimated time for `rows` (of p) x I outputs of
-// `nk` stages: rounds of the grid over the CUs, each its stages and 3 us around them, and
-// for a split the partial sums written and read at 3.5 TB/s and a second launch.
+// The tile and the split of r with the least estimated time for I x `rows` (of p) outputs (J
+// columns where gates halve them) of `nk` stages: rounds of the grid over the CUs, and for a
+// split the partial sums written and read at 3.5 TB/s and a second launch.
 template <int N>
 TilePlan gemm_plan(const TileSpec (&tiles)[N], int64_t I, int64_t J, int64_t rows, int nk) {
   constexpr int kMaxSplits = 16, kMaxSplitTiles = 1 << 16;
@@ -519,10 +600,10 @@ TilePlan gemm_plan(const TileSpec (&tiles)[N], int64_t I, int64_t J, int64_t row
       const int per = static_cast<int>(cdiv(nk, s));
       if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
       const bool gates = rows != J && s == 1;  // a split product: all rows of p, no gates
-      if (gates && !c.gated) continue;
+      if (gates && c.shape == G64X64) continue;
       const double n = static_cast<double>(cdiv(I, c.bi)) * cdiv(gates ? J : rows, gates ? c.bj / 2 : c.bj) * s;
       if (s > 1 && n > kMaxSplitTiles) continue;
-      double us = __builtin_ceil(n / (256.0 * c.per_cu)) * (c.us * per + 3.0);
+      double us = __builtin_ceil(n / (256.0 * c.per_cu)) * (c.us * per + c.round);
       if (s > 1) us += 4.0 + 2.0 * s * I * rows * 4 / 3.5e6;
       if (best_us < 0 || us < best_us) {
         best = {c.shape, s, per};
@@ -542,18 +623,26 @@ int launch_gemm(const LinArgs& a, const TilePlan& p, int per_cu, hipStream_t st)
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
-template <int KIND, bool TQ, bool TP, bool GATED, int EPI>
+// Tiles and stages: 8 waves hide each other's latency (two to a SIMD, 256 registers each);
+// 4 waves of 128 x 128 read a third less from LDS (BIG4).
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI, bool BIG4>
 int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
   switch (p.shape) {
-    case G256X256: return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, 4, 2>(a, p, 1, st);
+    case G256X256:
+      // (the sums and an ungated linear's epilogue leave too few registers)
+      if constexpr (EPI != E_LINEAR || GATED)
+        return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, BIG4 ? 2 : 4, 2>(a, p, 1, st);
+      break;
+    case G256X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 128, 4, 2, 3>(a, p, 1, st);
     case G128X256: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 256, 2, 4, 3>(a, p, 1, st);
     case G128X128X2: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 2>(a, p, 2, st);
     case G128X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 4>(a, p, 1, st);
     case G64X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 128, 2, 2, 4>(a, p, 1, st);
-    default:
+    case G64X64:
       if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 64, 2, 2, 8>(a, p, 1, st);
-      return set_error(MI355MOE_ERR_INVALID, "gemm: no such tile");
+      break;
   }
+  return set_error(MI355MOE_ERR_UNSUPPORTED, "gemm: no such tile");
 }
 
 }  // namespace mi355

@@ -4,9 +4,10 @@
 namespace mi355 {
 namespace {
 
-constexpr TileSpec kTiles[] = {{G256X256, 256, 256, 1, true, 1.95f},   {G128X256, 128, 256, 1, true, 1.2f},
-                               {G128X128X2, 128, 128, 2, true, 1.25f}, {G128X128, 128, 128, 1, true, 0.72f},
-                               {G64X128, 64, 128, 1, true, 0.46f},     {G64X64, 64, 64, 1, true, 0.33f}};
+constexpr TileSpec kTiles[] = {{G256X256, 256, 256, 1, 1.52f, 6.f}, {G256X128, 256, 128, 1, 0.86f, 4.f},
+                               {G128X256, 128, 256, 1, 0.87f, 4.f}, {G128X128X2, 128, 128, 2, 0.97f, 4.f},
+                               {G128X128, 128, 128, 1, 0.54f, 3.5f}, {G64X128, 64, 128, 1, 0.38f, 3.f},
+                               {G64X64, 64, 64, 1, 0.29f, 2.5f}};
 
 TilePlan plan(const Product& p) {
   return gemm_plan(kTiles, p.I, p.J, p.J, static_cast<int>(cdiv(p.R, GSB / 2)));
@@ -15,10 +16,10 @@ TilePlan plan(const Product& p) {
 template <int KIND>
 int launch(const LinArgs& a, bool transposed, const TilePlan& n, hipStream_t st) {
   if (n.splits > 1)
-    return transposed ? launch_gemm_shape<KIND, true, true, false, E_RAW>(a, n, st)
-                      : launch_gemm_shape<KIND, false, true, false, E_RAW>(a, n, st);
-  return transposed ? launch_gemm_shape<KIND, true, true, false, E_PLAIN>(a, n, st)
-                    : launch_gemm_shape<KIND, false, true, false, E_PLAIN>(a, n, st);
+    return transposed ? launch_gemm_shape<KIND, true, true, false, E_RAW, true>(a, n, st)
+                      : launch_gemm_shape<KIND, false, true, false, E_RAW, true>(a, n, st);
+  return transposed ? launch_gemm_shape<KIND, true, true, false, E_PLAIN, true>(a, n, st)
+                    : launch_gemm_shape<KIND, false, true, false, E_PLAIN, true>(a, n, st);
 }
 
 }  // namespace

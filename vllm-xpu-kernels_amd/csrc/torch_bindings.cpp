@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -1166,33 +1167,34 @@ std::tuple<at::Tensor, at::Tensor> per_token_int8_quant(const at::Tensor& input)
 }
 
 // ------------------------------------------------------------- gated linear
-// (out, z): z [rows, 2 out_features] float32 holds the sums with `keep`, else nothing
-std::tuple<at::Tensor, at::Tensor> gated_linear(const at::Tensor& input, const at::Tensor& weight,
-                                                const std::optional<at::Tensor>& bias,
-                                                int64_t activation, bool keep) {
+// (out, z): z [rows, 2 out_features] float32 holds the sums where `keep`, else nothing
+std::tuple<at::Tensor, at::Tensor> gated_linear_forward(const at::Tensor& input,
+                                                        const at::Tensor& weight,
+                                                        const std::optional<at::Tensor>& bias,
+                                                        int64_t activation, bool keep) {
   TORCH_CHECK(activation >= MI355MOE_LINEAR_SILU_AND_MUL &&
                   activation <= MI355MOE_LINEAR_GELU_TANH_AND_MUL,
               "the activation must be a gated one");
   at::Tensor out = linear_out(input, weight, activation, input.scalar_type());
-  at::Tensor z;
-  const auto f32 = input.options().dtype(at::kFloat);
+  std::optional<at::Tensor> z;
   if (keep) {
     c10::SymInt rows = 1;
     for (int64_t d = 0; d + 1 < input.dim(); ++d) rows *= input.sym_size(d);
-    z = at::empty_symint({rows, weight.sym_size(0)}, f32);
-  } else {
-    z = at::empty({0}, f32);
+    z = at::empty_symint({rows, weight.sym_size(0)}, input.options().dtype(at::kFloat));
   }
   if (!input.is_meta()) {
     TORCH_CHECK(input.scalar_type() == at::kBFloat16 || input.scalar_type() == at::kHalf,
                 "input must be bfloat16 or float16");
-    run_linear(out, input, std::nullopt, weight, std::nullopt, bias, std::nullopt, activation, false,
-               keep ? std::optional<at::Tensor>(z) : std::nullopt);
+    run_linear(out, input, std::nullopt, weight, std::nullopt, bias, std::nullopt, activation, false, z);
   }
-  return {out, z};
+  return {out, z.value_or(at::Tensor())};
+}
+at::Tensor gated_linear(const at::Tensor& input, const at::Tensor& weight,
+                        const std::optional<at::Tensor>& bias, int64_t activation) {
+  return std::get<0>(gated_linear_forward(input, weight, bias, activation, false));
 }
 
-// Gradients of the input, the weight and the bias, those asked for (else tensors of nothing):
+// Gradients of the input, the weight and the bias, those asked for (else no tensor):
 // the input's where the weight is given, the weight's where the input is, the bias's
 // in its type.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(
@@ -1201,7 +1203,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(
     std::optional<at::ScalarType> bias_dtype) {
   TORCH_CHECK(grad.dim() >= 1 && z.dim() == 2, "grad must have columns, z must be 2-dimensional");
   const auto o = grad.options();
-  at::Tensor dx = at::empty({0}, o), dw = at::empty({0}, o), db = at::empty({0}, o);
+  at::Tensor dx, dw, db;
   if (weight) {
     TORCH_CHECK(weight->dim() == 2, "weight must be 2-dimensional");
     std::vector<c10::SymInt> sizes(grad.sym_sizes().begin(), grad.sym_sizes().end());
@@ -1275,6 +1277,61 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_linear_backward(
   check_rc(mi355moe_gated_linear_backward(&a, need ? ws.data_ptr() : nullptr, need, cur_stream(grad)),
            "gated_linear_backward");
   return {dx, dw, db};
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_linear_keep(const at::Tensor& input, const at::Tensor& weight,
+                                                     const std::optional<at::Tensor>& bias,
+                                                     int64_t activation) {
+  return gated_linear_forward(input, weight, bias, activation, true);
+}
+
+// Reverse mode: both passes go through the dispatcher, so that they trace and refuse
+// devices as other operators do.
+template <typename F>
+auto gated_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+class GatedLinear : public torch::autograd::Function<GatedLinear> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& input,
+                            const at::Tensor& weight, const std::optional<at::Tensor>& bias,
+                            int64_t activation) {
+    static const auto op = gated_op<decltype(gated_linear_keep)>("_mi355_C::gated_linear_keep");
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, z] = op.call(input, weight, bias, activation);
+    // (what no asked gradient reads is not held)
+    ctx->save_for_backward({weight.requires_grad() ? input : at::Tensor(),
+                            input.requires_grad() ? weight : at::Tensor(), z});
+    ctx->saved_data["activation"] = activation;
+    if (bias && bias->requires_grad())
+      ctx->saved_data["bias_dtype"] = static_cast<int64_t>(bias->scalar_type());
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    static const auto op = gated_op<decltype(gated_linear_backward)>("_mi355_C::gated_linear_backward");
+    TORCH_CHECK(!at::GradMode::is_enabled(), "gated_linear has no gradient of its gradient");
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto saved = ctx->get_saved_variables();
+    auto given = [](const at::Tensor& t) {
+      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+    };
+    std::optional<at::ScalarType> bias_dtype;
+    const auto it = ctx->saved_data.find("bias_dtype");
+    if (it != ctx->saved_data.end()) bias_dtype = static_cast<at::ScalarType>(it->second.toInt());
+    auto [dx, dw, db] = op.call(grads[0], given(saved[0]), given(saved[1]), saved[2],
+                                ctx->saved_data["activation"].toInt(), bias_dtype);
+    return {dx, dw, db, at::Tensor()};
+  }
+};
+at::Tensor gated_linear_autograd(const at::Tensor& input, const at::Tensor& weight,
+                                 const std::optional<at::Tensor>& bias, int64_t activation) {
+  if (at::GradMode::is_enabled() &&
+      (input.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad())))
+    return GatedLinear::apply(input, weight, bias, activation);
+  static const auto op = gated_op<decltype(gated_linear)>("_mi355_C::gated_linear");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(input, weight, bias, activation);
 }
 
 // ------------------------------------------------------------- grouped GEMM
@@ -1723,7 +1780,8 @@ TORCH_LIBRARY(_mi355_C, m) {
   m.def("linear_int8_new(Tensor input, Tensor? input_scale, Tensor weight, Tensor weight_scale, "
         "Tensor? bias, Tensor? residual, int activation, ScalarType out_dtype) -> Tensor");
   m.def("per_token_int8_quant(Tensor input) -> (Tensor, Tensor)");
-  m.def("gated_linear(Tensor input, Tensor weight, Tensor? bias, int activation, bool keep) -> "
+  m.def("gated_linear(Tensor input, Tensor weight, Tensor? bias, int activation) -> Tensor");
+  m.def("gated_linear_keep(Tensor input, Tensor weight, Tensor? bias, int activation) -> "
         "(Tensor, Tensor)");
   m.def("gated_linear_backward(Tensor grad, Tensor? input, Tensor? weight, Tensor z, "
         "int activation, ScalarType? bias_dtype) -> (Tensor, Tensor, Tensor)");
@@ -1738,6 +1796,7 @@ TORCH_LIBRARY_IMPL(_mi355_C, CUDA, m) {
   m.impl("linear_int8_new", &linear_int8_new);
   m.impl("per_token_int8_quant", &per_token_int8_quant);
   m.impl("gated_linear", &gated_linear);
+  m.impl("gated_linear_keep", &gated_linear_keep);
   m.impl("gated_linear_backward", &gated_linear_backward);
 }
 
@@ -1749,5 +1808,10 @@ TORCH_LIBRARY_IMPL(_mi355_C, Meta, m) {
   m.impl("linear_int8_new", &linear_int8_new);
   m.impl("per_token_int8_quant", &per_token_int8_quant);
   m.impl("gated_linear", &gated_linear);
+  m.impl("gated_linear_keep", &gated_linear_keep);
   m.impl("gated_linear_backward", &gated_linear_backward);
+}
+
+TORCH_LIBRARY_IMPL(_mi355_C, Autograd, m) {
+  m.impl("gated_linear", &gated_linear_autograd);
 }

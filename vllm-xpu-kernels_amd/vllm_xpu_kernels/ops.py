@@ -290,7 +290,6 @@ _linear_int8 = torch.ops._mi355_C.linear_int8.default
 _linear_int8_new = torch.ops._mi355_C.linear_int8_new.default
 _per_token_int8_quant = torch.ops._mi355_C.per_token_int8_quant.default
 _gated_linear = torch.ops._mi355_C.gated_linear.default
-_gated_linear_backward = torch.ops._mi355_C.gated_linear_backward.default
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -443,25 +442,6 @@ def linear_int8(x: torch.Tensor, x_scale: Optional[torch.Tensor], weight: torch.
                        _linear_int8, _linear_int8_new)
 
 
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, code):
-        out, z = _gated_linear(x, weight, bias, code, True)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        ctx.save_for_backward(x if need_w else None, weight if need_x else None, z)
-        ctx.code = code
-        ctx.bias_dtype = bias.dtype if need_b else None
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, z = ctx.saved_tensors
-        dx, dw, db = _gated_linear_backward(grad, x, weight, z, ctx.code, ctx.bias_dtype)
-        return (None if weight is None else dx, None if x is None else dw,
-                None if ctx.bias_dtype is None else db, None)
-
-
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                  activation: str = "silu_and_mul") -> torch.Tensor:
     """f(x @ gate.T + bias_gate) * (x @ up.T + bias_up) in one kernel, with gradients of
@@ -479,10 +459,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if code < 5:
         raise ValueError(f"Unsupported activation: {activation}.")
     _no_tangent(x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
-        return _GatedLinear.apply(x, weight, bias, code)
-    return _gated_linear(x, weight, bias, code, False)[0]
+    return _gated_linear(x, weight, bias, code)
 
 
 def init_expert_map(num_experts: int, ep_rank: int, ep_size: int,

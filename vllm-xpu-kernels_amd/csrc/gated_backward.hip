@@ -44,7 +44,8 @@ __device__ __forceinline__ void gate_grad(float z, float& f, float& df) {
 
 constexpr int kRowBlocks = 128;  // db's parts at most
 
-// Rows of x's block y, 8 columns of the gate and of the factor per lane; with DB the
+// Rows of x's block y, 8 columns of the gate and of the factor per lane (VEC: consecutive
+// ones; else 64 apart, so that a wave's accesses are runs of 64); with DB the
 // workgroup's sums of dz in fp32 go to part[y][2N].  ld: dz's row stride, a multiple of
 // 8; the columns past 2N are zeros.
 template <int ACT, bool F16, bool VEC, bool DB>
@@ -52,7 +53,8 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const GradArgs a, uint16_
                                                        int64_t ld, int64_t rows_per_block,
                                                        float* __restrict__ part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n = (static_cast<int64_t>(blockIdx.x) * 64 + lane) * 8;
+  constexpr int STEP = VEC ? 1 : 64;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 512 + (VEC ? lane * 8 : lane);
   const int64_t first = static_cast<int64_t>(blockIdx.y) * rows_per_block;
   const int64_t end = first + rows_per_block < a.M ? first + rows_per_block : a.M;
   const bool on = n < a.N;
@@ -81,10 +83,10 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const GradArgs a, uint16_
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const bool in = n + k < a.N;
-          g[k] = in ? z[k] : 0.f;
-          u[k] = in ? z[a.N + k] : 0.f;
-          e[k] = in ? ld16<F16>(d[k]) : 0.f;
+          const bool in = n + k * STEP < a.N;
+          g[k] = in ? z[k * STEP] : 0.f;
+          u[k] = in ? z[a.N + k * STEP] : 0.f;
+          e[k] = in ? ld16<F16>(d[k * STEP]) : 0.f;
         }
       }
 #pragma unroll
@@ -107,11 +109,11 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const GradArgs a, uint16_
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (n + k < a.N) {
-            o[k] = st16<F16>(r1[k]);
-            o[a.N + k] = st16<F16>(r2[k]);
+          if (n + k * STEP < a.N) {
+            o[k * STEP] = st16<F16>(r1[k]);
+            o[a.N + k * STEP] = st16<F16>(r2[k]);
           }
-        if (n + 8 >= a.N)
+        if (n == 0)
           for (int64_t c = 2 * a.N; c < ld; ++c) dz[m * ld + c] = 0;
       }
     }
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const GradArgs a, uint16_
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 16; i += 256) {
       const int l = (i >> 3) & 63, k = (i & 7) + (i >> 9) * 8;
-      const int64_t c = (static_cast<int64_t>(blockIdx.x) * 64 + l) * 8 + (i & 7);
+      const int64_t c = static_cast<int64_t>(blockIdx.x) * 512 + (VEC ? l * 8 + (i & 7) : l + (i & 7) * 64);
       if (c >= a.N) continue;
       const float v = (red[0][l][k] + red[1][l][k]) + (red[2][l][k] + red[3][l][k]);
       part[blockIdx.y * 2 * a.N + (i >> 9) * a.N + c] = v;
@@ -211,9 +213,10 @@ struct Layout {
 Layout layout(const GradArgs& a, uintptr_t ws) {
   Layout l{};
   l.ld = (2 * a.N + 7) / 8 * 8;
-  // rows of a dz workgroup: 32, so that there are workgroups for every CU; db's parts
-  // bound their number
-  l.per = 32;
+  // rows of a dz workgroup: 4 to 32, a wave's in turn, for some 1000 workgroups (61 x 1536
+  // 6.5 -> 3.6 us, 257 x 1030 29 -> 9); db's parts bound their number
+  l.per = cdiv(a.M * cdiv(a.N, 512), 1024 * 4) * 4;
+  l.per = l.per < 4 ? 4 : l.per > 32 ? 32 : l.per;
   if (a.dbias && cdiv(a.M, l.per) > kRowBlocks) l.per = cdiv(a.M, kRowBlocks);
   if (cdiv(a.M, l.per) > 65535) l.per = cdiv(a.M, 65535);
   l.blocks = static_cast<int>(cdiv(a.M, l.per));

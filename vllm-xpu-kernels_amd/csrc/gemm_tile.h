@@ -32,10 +32,13 @@ namespace mi355 {
 
 constexpr int GSB = 128;         // bytes of a stage along r
 __device__ __forceinline__ int gswz(int r) { return (r >> 1) & 7; }
-// across r: chunk c of row r is at slot c ^ cross_swz<chunks of a row>(r)
+// across r: chunk c of row r is at slot c ^ cross_swz<chunks of a row>(r): 64 bytes times r & 3
+// where rows start at the same banks (multiples of 256 bytes), 64 times r / 2 where every
+// other one does; rows of 192 bytes are 64 apart as they are
 template <int CH>
 __device__ __forceinline__ int cross_swz(int r) {
-  return CH >= 16 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
+  static_assert(CH % 8 == 0 || CH == 12, "rows");
+  return CH % 16 == 0 ? (r & 3) << 2 : CH % 8 == 0 ? ((r >> 1) & 1) << 2 : 0;
 }
 
 // What a tile does with its sums: E_RAW, as they are to a.out + split M N (float, int8:
@@ -90,7 +93,6 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
   constexpr int BR = GSB / EB;                                // r of a stage
   constexpr int STAGE = (BI + BJ) * GSB;
   constexpr int QCH = TQ ? BI / 8 : 8, PCH = TP ? BJ / 8 : 8;  // 16-byte chunks of a staged row
-  constexpr int QRC = 64 / QCH, PRC = 64 / PCH;               // rows of a 1 KB copy
   constexpr int QQ = BI / 8 / WAVES, PQ = BJ / 8 / WAVES, ND = QQ + PQ;  // copies per wave and stage
   static_assert(QQ * 8 * WAVES == BI && PQ * 8 * WAVES == BJ, "copies");
   static_assert(!GATED || PQ % 2 == 0, "a copy has rows of one half");
@@ -133,12 +135,14 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
   const uint64_t qstep = TQ ? static_cast<uint64_t>(a.ldx) * (2 * BR) : GSB;
   const uint64_t pstep = TP ? static_cast<uint64_t>(a.ldw) * (2 * BR) : GSB;
   const uint64_t uhalf = GATED ? static_cast<uint64_t>(a.N) * a.ldw * EB : 0;
-  auto row_of = [=](int q) __attribute__((always_inline)) {
-    if (q < QQ) return (wave * QQ + q) * QRC + lane / QCH;
+  // the 16 bytes that this lane copies: their number in the staged operand
+  auto piece_of = [=](int q) __attribute__((always_inline)) {
+    if (q < QQ) return (wave * QQ + q) * 64 + lane;
     // (gated: a wave's first copies are the gate's rows, its others the factor's)
-    if (GATED) return (wave * (PQ / 2) + (q - QQ) % (PQ / 2)) * PRC + lane / PCH;
-    return (wave * PQ + q - QQ) * PRC + lane / PCH;
+    if (GATED) return (wave * (PQ / 2) + (q - QQ) % (PQ / 2)) * 64 + lane;
+    return (wave * PQ + q - QQ) * 64 + lane;
   };
+  auto row_of = [=](int q) __attribute__((always_inline)) { return piece_of(q) / (q < QQ ? QCH : PCH); };
   auto place = [&](int tile) __attribute__((always_inline)) {
     split = tile / (tiles_i * tiles_j);
     tile %= tiles_i * tiles_j;
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
       const bool x = q < QQ;
       const int64_t ld = x ? a.ldx : a.ldw;
       if (x ? TQ : TP) {
-        const int c = x ? (lane % QCH) ^ cross_swz<QCH>(r) : (lane % PCH) ^ cross_swz<PCH>(r);
+        const int c = x ? (piece_of(q) % QCH) ^ cross_swz<QCH>(r) : (piece_of(q) % PCH) ^ cross_swz<PCH>(r);
         const int last = x ? qlast : plast;
         voff[q] = static_cast<uint32_t>(r * ld * EB + ((c < last ? c : last) << 4));
       } else {
@@ -577,12 +581,19 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
 
 // A choice of tiles.  us: time of one stage on every CU at once, round: of the rest of a
 // round of tiles (first copies, epilogue); per_cu: workgroups of the tile that a CU holds.
-enum TileShape { G256X256, G256X128, G128X256, G128X128X2, G128X128, G64X128, G64X64 };
+enum TileShape {
+  G256X256, G256X128, G128X256, G192X192, G192X128, G128X192, G128X128X2, G128X128, G96X128, G64X128, G64X64
+};
 struct TileSpec {
   TileShape shape;
   int bi, bj, per_cu;
   float us, round;
 };
+// a shape's waves take the same columns of both halves of a gated weight, in 32s; G128X192 is
+// for these alone
+constexpr bool gates_of(TileShape s) {
+  return s != G192X192 && s != G192X128 && s != G96X128 && s != G64X64;
+}
 struct TilePlan {
   TileShape shape;
   int splits, per;  // stages per split
@@ -600,7 +611,8 @@ TilePlan gemm_plan(const TileSpec (&tiles)[N], int64_t I, int64_t J, int64_t row
       const int per = static_cast<int>(cdiv(nk, s));
       if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
       const bool gates = rows != J && s == 1;  // a split product: all rows of p, no gates
-      if (gates && c.shape == G64X64) continue;
+      if (gates && !gates_of(c.shape)) continue;
+      if (!gates && c.shape == G128X192) continue;
       const double n = static_cast<double>(cdiv(I, c.bi)) * cdiv(gates ? J : rows, gates ? c.bj / 2 : c.bj) * s;
       if (s > 1 && n > kMaxSplitTiles) continue;
       double us = __builtin_ceil(n / (256.0 * c.per_cu)) * (c.us * per + c.round);
@@ -623,20 +635,35 @@ int launch_gemm(const LinArgs& a, const TilePlan& p, int per_cu, hipStream_t st)
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
-// Tiles and stages: 8 waves hide each other's latency (two to a SIMD, 256 registers each);
-// 4 waves of 128 x 128 read a third less from LDS (BIG4).
-template <int KIND, bool TQ, bool TP, bool GATED, int EPI, bool BIG4>
+// Waves and stages.  256 x 256: 4 waves of 128 x 128 read a third less from LDS than 8 of
+// 128 x 64 (dW 4096 x 8192 x 7168 in a row of calls, at the clock that the power allows: 388
+// against 415 us); smaller tiles take 8 where a CU holds one workgroup (int8 1003 x 2880 x 2880
+// in 128 x 128 21.0 against 23.9).
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI>
 int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
   switch (p.shape) {
     case G256X256:
       // (the sums and an ungated linear's epilogue leave too few registers)
       if constexpr (EPI != E_LINEAR || GATED)
-        return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, BIG4 ? 2 : 4, 2>(a, p, 1, st);
+        return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, 2, 2>(a, p, 1, st);
       break;
     case G256X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 128, 4, 2, 3>(a, p, 1, st);
     case G128X256: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 256, 2, 4, 3>(a, p, 1, st);
+    case G192X192:
+      if constexpr (!GATED && KIND != K_I8)  // (int8: no table has it, its epilogue spills)
+        return launch_gemm<KIND, TQ, TP, GATED, EPI, 192, 192, 2, 2, 3>(a, p, 1, st);
+      break;
+    case G192X128:
+      if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 192, 128, 2, 2, 3>(a, p, 1, st);
+      break;
+    case G96X128:
+      if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 96, 128, 1, 4, 4>(a, p, 1, st);
+      break;
+    case G128X192:
+      if constexpr (GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 192, 4, 1, 3>(a, p, 1, st);
+      break;
     case G128X128X2: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 2>(a, p, 2, st);
-    case G128X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 4>(a, p, 1, st);
+    case G128X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 4, 2, 4>(a, p, 1, st);
     case G64X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 128, 2, 2, 4>(a, p, 1, st);
     case G64X64:
       if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 64, 2, 2, 8>(a, p, 1, st);

@@ -7,7 +7,7 @@
 // rows on, by latency below.  A row stays in registers between its maximum and its
 // codes: R chunks of 8 columns per lane, the row's lanes in one wave (4 rows to a
 // workgroup) or in one workgroup.  Longer rows are read twice.
-#include "linear.h"
+#include "int8_quant.h"
 
 namespace mi355 {
 namespace {
@@ -21,46 +21,6 @@ struct QuantArgs {
   int64_t scale_row, rows, cols;
 };
 
-// Columns i .. i + 7 of a row: 16-byte loads when VEC (i a multiple of 8), else those
-// below `cols` one by one and zeros.
-template <typename E, bool VEC>
-__device__ __forceinline__ void row8(const typename E::T* p, int64_t i, int64_t cols, float (&f)[8]) {
-  if constexpr (VEC && sizeof(typename E::T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f[2 * k] = E::ld(static_cast<uint16_t>(w[k]));
-      f[2 * k + 1] = E::ld(static_cast<uint16_t>(w[k] >> 16));
-    }
-  } else if constexpr (VEC) {
-    const float4 a = reinterpret_cast<const float4*>(p + i)[0], b = reinterpret_cast<const float4*>(p + i)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = i + k < cols ? E::ld(p[i + k]) : 0.f;
-  }
-}
-
-// |v| as bits: they order as the values do, a NaN above infinity
-__device__ __forceinline__ uint32_t top8(const float (&f)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t u = __float_as_uint(f[k]) & 0x7fffffffu;
-    m = u > m ? u : m;
-  }
-  return m;
-}
-__device__ __forceinline__ uint32_t wave_top(uint32_t m) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t u = static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o, 64));
-    m = u > m ? u : m;
-  }
-  return m;
-}
 __device__ __forceinline__ uint32_t workgroup_top(uint32_t m, int waves) {
   __shared__ uint32_t part[16];
   m = wave_top(m);
@@ -71,35 +31,14 @@ __device__ __forceinline__ uint32_t workgroup_top(uint32_t m, int waves) {
   return m;
 }
 
-__device__ __forceinline__ float scale_of(uint32_t top) {
-  const float a = __uint_as_float(top);
-  return (a < 1e-10f ? 1e-10f : a) / 127.0f;
-}
-// The code of v / s.  v * (1 / s) is off by less than 2^-15 (three roundings of a value up
-// to 127), so its nearest integer is the quotient's unless it lies that near the middle
-// between two: then the division decides (a few of 100000 values).
-__device__ __forceinline__ int code_of(float v, float s, float inv) {
-  const float t = v * inv;
-  float r = __builtin_rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) < 0x1p-14f) r = __builtin_rintf(v / s);
-  return static_cast<int>(r);
-}
 template <bool VEC>
-__device__ __forceinline__ void codes8(int8_t* q, int64_t i, int64_t cols, const float (&f)[8], float s) {
-  const bool bad = !(s < __uint_as_float(0x7f800000u));  // an infinite or NaN row
-  const float inv = 1.0f / s;
-  uint32_t w[2] = {0, 0};
-  if (!bad) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      w[k >> 2] |= static_cast<uint32_t>(code_of(f[k], s, inv) & 0xff) << (8 * (k & 3));
-  }
+__device__ __forceinline__ void put8(int8_t* q, int64_t i, int64_t cols, uint2 w) {
   if constexpr (VEC) {
-    *reinterpret_cast<uint2*>(q + i) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(q + i) = w;
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (i + k < cols) q[i + k] = static_cast<int8_t>(w[k >> 2] >> (8 * (k & 3)));
+      if (i + k < cols) q[i + k] = static_cast<int8_t>((k < 4 ? w.x : w.y) >> (8 * (k & 3)));
   }
 }
 
@@ -132,7 +71,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void int8_quant_kernel(const Qua
 #pragma unroll
   for (int c = 0; c < R; ++c) {
     const int64_t i = static_cast<int64_t>(c * lanes + t) * 8;
-    if (i < a.cols) codes8<VEC>(a.q + r * a.ldq, i, a.cols, f[c], s);
+    if (i < a.cols) put8<VEC>(a.q + r * a.ldq, i, a.cols, codes8(f[c], s));
   }
 }
 
@@ -153,7 +92,7 @@ __global__ __launch_bounds__(1024) void int8_quant_long_kernel(const QuantArgs a
   for (int64_t i = threadIdx.x * 8; i < a.cols; i += 1024 * 8) {
     float f[8];
     row8<E, VEC>(x, i, a.cols, f);
-    codes8<VEC>(a.q + r * a.ldq, i, a.cols, f, s);
+    put8<VEC>(a.q + r * a.ldq, i, a.cols, codes8(f, s));
   }
 }
 

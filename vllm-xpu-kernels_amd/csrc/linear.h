@@ -304,6 +304,8 @@ int launch_linear_finish(const LinArgs& a, const void* part, int splits, hipStre
 // few rows of x (linear_skinny.hip), any alignment; tile: the tiles can take them too
 bool linear_skinny_takes(const LinArgs& a, bool tile);
 int launch_linear_skinny(const LinArgs& a, hipStream_t st);
+// 16-bit rows of x (a.weight_dtype int8) that it quantises itself
+bool linear_skinny_quantises(const LinArgs& a);
 // more rows (linear_tile.hip).  a0: the call; a: the same, or with a split K the
 // product of all weight rows into fp32 partial sums [splits][M][rows]
 bool linear_tile_supported(const LinArgs& a);

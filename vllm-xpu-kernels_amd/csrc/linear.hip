@@ -324,6 +324,7 @@ size_t code_bytes(LinArgs& c, uintptr_t workspace) {
 extern "C" size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* p) {
   if (!p || check(*p) || p->M == 0) return 0;
   LinArgs a = *p;
+  if (quantises(a) && linear_skinny_quantises(a)) return 0;
   const size_t codes = quantises(a) ? code_bytes(a, 0) : 0;
   return codes + lin_partials(a, splits_of(a, path_of(a)));
 }
@@ -339,6 +340,7 @@ extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
   MI_ARG((a.x_dtype != MI355MOE_FP8E4M3 && a.x_dtype != MI355MOE_I8 && !quant) ||
              ((a.x_scale || quant) && a.weight_scale), "linear: scales missing");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (quant && linear_skinny_quantises(a)) return launch_linear_skinny(a, st);
   const LinArgs given = a;
   const size_t codes = quant ? code_bytes(a, reinterpret_cast<uintptr_t>(workspace)) : 0;
   const Path path = path_of(a);

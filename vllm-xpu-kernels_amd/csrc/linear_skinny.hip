@@ -12,9 +12,12 @@
 // in runs of 256 bytes instead of 64 (R = 4: up to 4 rows of x, 8: up to 8,
 // 16: up to 16 per group of columns, MT groups).
 //
+// QUANT: x is one 16-bit row; every workgroup makes its int8 codes itself, into LDS, while
+// its first weights are on their way.
+//
 // e4m3 operands are converted to bf16 (exact) as they arrive; each K step's
 // product is multiplied by its blocks' scales, held in LDS.
-#include "linear.h"
+#include "int8_quant.h"
 
 namespace mi355 {
 namespace {
@@ -32,7 +35,39 @@ __device__ __forceinline__ uint4 as4(u32x4 v) { return make_uint4(v.x, v.y, v.z,
 
 constexpr int kScaleBytes = 48 * 1024;  // LDS for the e4m3 scales
 
-template <int KIND, bool GATED, int R, int MT, int U>
+// The row's scale and codes (K % 16 == 0): each of 256 threads holds 4 chunks of 8 columns
+// at most.
+constexpr int kQuantChunks = 4;
+template <typename E>
+__device__ __forceinline__ void quantise_row(const LinArgs& a, int waves, float* s_scale, uint8_t* s_code) {
+  __shared__ uint32_t s_top[4];
+  const int tid = threadIdx.x, threads = 64 * waves;
+  float f[kQuantChunks][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < kQuantChunks; ++c) {
+    const int64_t i = static_cast<int64_t>(c * threads + tid) * 8;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[c][k] = 0.f;
+    if (i < a.K) row8<E, true>(static_cast<const uint16_t*>(a.x), i, a.K, f[c]);
+    const uint32_t u = top8(f[c]);
+    top = u > top ? u : top;
+  }
+  top = wave_top(top);
+  if ((tid & 63) == 0) s_top[tid >> 6] = top;
+  __syncthreads();
+  for (int w = 0; w < waves; ++w) top = s_top[w] > top ? s_top[w] : top;
+  const float s = scale_of(top);
+  if (tid == 0) *s_scale = s;
+#pragma unroll
+  for (int c = 0; c < kQuantChunks; ++c) {
+    const int64_t i = static_cast<int64_t>(c * threads + tid) * 8;
+    if (i < a.K) *reinterpret_cast<uint2*>(s_code + i) = codes8(f[c], s);
+  }
+  __syncthreads();
+}
+
+template <int KIND, bool GATED, int R, int MT, int U, bool QUANT>
 __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   constexpr int C = 16 / R;
   constexpr int STEP = C * 64;                // bytes of a row per K step
@@ -47,6 +82,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   const int waves = static_cast<int>(blockDim.x) >> 6;
   const int l16 = lane & 15, q = lane >> 4;
   const int ri = l16 % R, ci = l16 / R;
+  static_assert(!QUANT || (I8 && MT == 1), "operands");
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * R;
   const int64_t mbase = static_cast<int64_t>(blockIdx.y) * (R * MT);
   const int kbytes = static_cast<int>(a.K) * EB, kfull = kbytes & ~15;  // K <= 2^28
@@ -65,7 +101,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   for (int j = 0; j < MT; ++j) {
     int64_t m = mbase + R * j + ri;
     m = m < a.M ? m : a.M - 1;
-    xp[j] = static_cast<const uint8_t*>(a.x) + m * a.ldx * EB;
+    xp[j] = static_cast<const uint8_t*>(a.x) + m * a.ldx * EB;  // (QUANT: not read)
   }
   const int steps = (kfull + STEP - 1) / STEP;
   const int per = (steps + waves - 1) / waves;
@@ -84,8 +120,10 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
       const int oc = s + u < s1 && o < kfull ? o : 0;
 #pragma unroll
       for (int i = 0; i < NS; ++i) w[u][i] = ld16_any(wp[i] + oc);
+      if constexpr (!QUANT) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) x[u][j] = ld16_any(xp[j] + oc);
+        for (int j = 0; j < MT; ++j) x[u][j] = ld16_any(xp[j] + oc);
+      }
     }
   };
 
@@ -99,6 +137,14 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
 
   const bool any = s0 < s1;  // uniform per wave
   if (any) load(w0, x0, s0);
+  // QUANT: the row's scale, then its codes
+  float* s_row = lds;
+  uint8_t* s_code = reinterpret_cast<uint8_t*>(lds + 4);
+  if constexpr (QUANT) {
+    red = reinterpret_cast<S*>(s_code + a.K);
+    if (a.x_dtype == MI355MOE_F16) quantise_row<F16>(a, waves, s_row, s_code);
+    else quantise_row<BF16>(a, waves, s_row, s_code);
+  }
   if constexpr (FP8) {
     for (int i = tid; i < (kblocks + 1) * NS * R; i += blockDim.x) {
       const int kb = i / (NS * R), s = (i / R) % NS, r = i % R;
@@ -165,7 +211,13 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) w[u][i] &= keep;
 #pragma unroll
-      for (int j = 0; j < MT; ++j) x[u][j] &= keep;
+      for (int j = 0; j < MT; ++j) {
+        if constexpr (QUANT) {  // (every row of the group is the one; cleared weights need no codes)
+          x[u][j] = *reinterpret_cast<const u32x4*>(s_code + (keep ? (s + u) * STEP + off : 0));
+        } else {
+          x[u][j] &= keep;
+        }
+      }
       product(w[u], x[u], s + u);
     }
   };
@@ -237,7 +289,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
       }
     float zf = static_cast<float>(z), uf = static_cast<float>(u);
     if constexpr (I8) {
-      const float xs = x_scale_of(a, m);
+      const float xs = QUANT ? *s_row : x_scale_of(a, m);
       zf *= xs * w_scale_of(a, n);
       if constexpr (GATED) uf *= xs * w_scale_of(a, a.N + n);
     }
@@ -245,14 +297,15 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   }
 }
 
-template <int KIND, bool GATED, int R, int MT, int U>
+template <int KIND, bool GATED, int R, int MT, int U, bool QUANT = false>
 int launch(const LinArgs& a, int waves, hipStream_t st) {
   constexpr int NS = GATED ? 2 : 1;
   const int64_t blocks = KIND == K_FP8 ? a.K / 128 + 1 : 0;
+  // QUANT: the row's scale and codes (K up to 8192: 8 KiB);
   // at most 48 KiB of scales (linear_skinny_takes), a block of zeros and 8 KiB of sums
-  const size_t lds = 4 * (blocks * (NS + MT) * R + static_cast<size_t>(waves) * NS * MT * 16 * R);
+  const size_t lds = (QUANT ? 16 + a.K : 0) + 4 * (blocks * (NS + MT) * R + static_cast<size_t>(waves) * NS * MT * 16 * R);
   const dim3 grid(static_cast<unsigned>(cdiv(a.N, R)), static_cast<unsigned>(cdiv(a.M, R * MT)));
-  linear_skinny_kernel<KIND, GATED, R, MT, U><<<grid, dim3(64 * waves), lds, st>>>(a);
+  linear_skinny_kernel<KIND, GATED, R, MT, U, QUANT><<<grid, dim3(64 * waves), lds, st>>>(a);
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
@@ -269,7 +322,15 @@ int launch(const LinArgs& a, int waves, hipStream_t st) {
 template <int KIND, bool GATED>
 int launch_rows(const LinArgs& a, hipStream_t st) {
   const bool few = a.N <= 2048;  // at most 128 strips of 16
-  if constexpr (KIND == K_FP8) {
+  if constexpr (KIND == K_I8) {
+    // Two steps ahead (U = 2) are enough for bytes, and shorter to fill (1 x 4096 x 4096 6.4
+    // us against 7.0 with four, 4 x 7168 x 4096 gated 10.0 / 10.6, 8 x 4096 x 4096 7.7 / 8.0,
+    // 16 x 4096 x 4096 8.3 / 8.9, 16 x 2048 x 1536 gated 5.3 / 5.7).
+    if (a.x_dtype != MI355MOE_I8) return launch<KIND, GATED, 4, 1, 2, true>(a, 4, st);
+    if (a.M <= 4) return launch<KIND, GATED, 4, 1, 2>(a, 2, st);
+    if (a.M <= 16 && few) return launch<KIND, GATED, 8, 2, 2>(a, 2, st);
+    return launch<KIND, GATED, 16, 1, 2>(a, 4, st);
+  } else if constexpr (KIND == K_FP8) {
     const bool lng = a.K >= 4096;
     if (a.M <= 4 && few) return launch<KIND, GATED, 4, 1, 4>(a, lng ? 4 : 2, st);
     if (a.M <= 8 && few && lng) return launch<KIND, GATED, 4, 2, 4>(a, 4, st);
@@ -304,11 +365,21 @@ bool linear_skinny_takes(const LinArgs& a, bool tile) {
   return a.M <= 16 || (a.M <= 64 && cdiv(a.M, 16) * weight <= (int64_t(12) << 20));
 }
 
+// x that the stream quantises itself: one row at a multiple of 16 bytes.  A launch less, but
+// each workgroup of 4 weight rows quantises it again, so up to 4 of them per CU (both ways in a
+// graph, us: 1 x 7168 x 4096 gated 12.4 / 13.2, 1 x 2048 x 1536 gated 6.0 / 7.1, 1 x 7168 x 256
+// 7.1 / 8.3, 1 x 4096 x 4096 8.4 / 8.9, but 1 x 2048 x 7168 11.6 / 9.5, 1 x 7168 x 7168 19.3 /
+// 17.6, and two rows of 7168 x 4096 gated 14.2 / 13.5).
+bool linear_skinny_quantises(const LinArgs& a) {
+  return a.M == 1 && a.N <= 4096 && a.K % 16 == 0 && a.K <= 8 * 256 * kQuantChunks &&
+         (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+}
+
 int launch_linear_skinny(const LinArgs& a, hipStream_t st) {
   const bool g = lin_gated(a.activation);
   if (a.x_dtype == MI355MOE_FP8E4M3)
     return g ? launch_rows<K_FP8, true>(a, st) : launch_rows<K_FP8, false>(a, st);
-  if (a.x_dtype == MI355MOE_I8)
+  if (a.x_dtype == MI355MOE_I8 || a.weight_dtype == MI355MOE_I8)
     return g ? launch_rows<K_I8, true>(a, st) : launch_rows<K_I8, false>(a, st);
   if (a.x_dtype == MI355MOE_F16)
     return g ? launch_rows<K_F16, true>(a, st) : launch_rows<K_F16, false>(a, st);

@@ -4,10 +4,20 @@
 namespace mi355 {
 namespace {
 
-constexpr TileSpec kTiles[] = {{G256X256, 256, 256, 1, 1.52f, 6.f}, {G256X128, 256, 128, 1, 0.86f, 4.f},
-                               {G128X256, 128, 256, 1, 0.87f, 4.f}, {G128X128X2, 128, 128, 2, 0.97f, 4.f},
-                               {G128X128, 128, 128, 1, 0.54f, 3.5f}, {G64X128, 64, 128, 1, 0.38f, 3.f},
-                               {G64X64, 64, 64, 1, 0.29f, 2.5f}};
+// Times of a stage and of the rest of a round, from dx 8192 x 4096 x 7168 and dW 4096 x 8192 x 7168
+// (I x R x J) on every shape.  Shapes for the fill of 256 CUs: 1003 x 5760 x 2880 96 x 128 43 us,
+// 128 x 128 49; 5760 x 1003 x 2880 192 x 192 42 us, 128 x 128 44 to 52, 256 x 256 77.
+constexpr TileSpec kTiles[] = {
+    {G256X256, 256, 256, 1, 1.55f, 8.0f},
+    {G256X128, 256, 128, 1, 0.9f, 5.0f},
+    {G128X256, 128, 256, 1, 0.9f, 5.0f},
+    {G192X192, 192, 192, 1, 0.98f, 4.5f},
+    {G192X128, 192, 128, 1, 0.7f, 3.5f},
+    {G128X128X2, 128, 128, 2, 0.99f, 5.0f},
+    {G128X128, 128, 128, 1, 0.56f, 3.0f},
+    {G96X128, 96, 128, 1, 0.44f, 1.5f},
+    {G64X128, 64, 128, 1, 0.385f, 1.2f},
+    {G64X64, 64, 64, 1, 0.29f, 1.2f}};
 
 TilePlan plan(const Product& p) {
   return gemm_plan(kTiles, p.I, p.J, p.J, static_cast<int>(cdiv(p.R, GSB / 2)));
@@ -16,10 +26,10 @@ TilePlan plan(const Product& p) {
 template <int KIND>
 int launch(const LinArgs& a, bool transposed, const TilePlan& n, hipStream_t st) {
   if (n.splits > 1)
-    return transposed ? launch_gemm_shape<KIND, true, true, false, E_RAW, true>(a, n, st)
-                      : launch_gemm_shape<KIND, false, true, false, E_RAW, true>(a, n, st);
-  return transposed ? launch_gemm_shape<KIND, true, true, false, E_PLAIN, true>(a, n, st)
-                    : launch_gemm_shape<KIND, false, true, false, E_PLAIN, true>(a, n, st);
+    return transposed ? launch_gemm_shape<KIND, true, true, false, E_RAW>(a, n, st)
+                      : launch_gemm_shape<KIND, false, true, false, E_RAW>(a, n, st);
+  return transposed ? launch_gemm_shape<KIND, true, true, false, E_PLAIN>(a, n, st)
+                    : launch_gemm_shape<KIND, false, true, false, E_PLAIN>(a, n, st);
 }
 
 }  // namespace

@@ -635,17 +635,17 @@ int launch_gemm(const LinArgs& a, const TilePlan& p, int per_cu, hipStream_t st)
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
-// Waves and stages.  256 x 256: 4 waves of 128 x 128 read a third less from LDS than 8 of
-// 128 x 64 (dW 4096 x 8192 x 7168 in a row of calls, at the clock that the power allows: 388
-// against 415 us); smaller tiles take 8 where a CU holds one workgroup (int8 1003 x 2880 x 2880
-// in 128 x 128 21.0 against 23.9).
+// Waves and stages.  8 waves hide each other's latency where a CU holds one workgroup: 256 x 256 in
+// 8 waves of 128 x 64 against 4 of 128 x 128, which read a third less from LDS (in turn, us: int8
+// 8192 x 7168 x 4096 gated 214 / 232, kept 421 / 447, dx 8192 x 4096 x 7168 412 / 433, dW 4096 x
+// 8192 x 7168 405 / 413); 128 x 128 in 8 and 4 (int8 1003 x 2880 x 2880 21.0 / 23.9).
 template <int KIND, bool TQ, bool TP, bool GATED, int EPI>
 int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
   switch (p.shape) {
     case G256X256:
       // (the sums and an ungated linear's epilogue leave too few registers)
       if constexpr (EPI != E_LINEAR || GATED)
-        return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, 2, 2>(a, p, 1, st);
+        return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 256, 2, 4, 2>(a, p, 1, st);
       break;
     case G256X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 256, 128, 4, 2, 3>(a, p, 1, st);
     case G128X256: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 256, 2, 4, 3>(a, p, 1, st);

@@ -22,7 +22,7 @@ constexpr TileSpec kTiles[] = {
     {G64X128, 64, 128, 1, 0.4f, 2.0f},
     {G64X64, 64, 64, 1, 0.31f, 1.7f}};
 constexpr TileSpec kTilesGated[] = {
-    {G256X256, 256, 256, 1, 1.92f, 8.0f},
+    {G256X256, 256, 256, 1, 1.78f, 7.0f},
     {G256X128, 256, 128, 1, 0.98f, 5.0f},
     {G128X256, 128, 256, 1, 0.98f, 5.0f},
     {G128X192, 128, 192, 1, 0.76f, 5.0f},
@@ -33,7 +33,7 @@ constexpr TileSpec kTilesGated[] = {
     {G96X128, 96, 128, 1, 0.49f, 2.6f},
     {G64X64, 64, 64, 1, 0.31f, 1.7f}};
 constexpr TileSpec kTilesKeep[] = {
-    {G256X256, 256, 256, 1, 1.92f, 12.0f},
+    {G256X256, 256, 256, 1, 1.77f, 12.0f},
     {G256X128, 256, 128, 1, 0.99f, 6.0f},
     {G128X256, 128, 256, 1, 0.99f, 6.0f},
     {G128X192, 128, 192, 1, 0.77f, 5.0f},

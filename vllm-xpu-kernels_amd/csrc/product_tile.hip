@@ -8,7 +8,7 @@ namespace {
 // (I x R x J) on every shape.  Shapes for the fill of 256 CUs: 1003 x 5760 x 2880 96 x 128 43 us,
 // 128 x 128 49; 5760 x 1003 x 2880 192 x 192 42 us, 128 x 128 44 to 52, 256 x 256 77.
 constexpr TileSpec kTiles[] = {
-    {G256X256, 256, 256, 1, 1.55f, 8.0f},
+    {G256X256, 256, 256, 1, 1.51f, 7.0f},
     {G256X128, 256, 128, 1, 0.9f, 5.0f},
     {G128X256, 128, 256, 1, 0.9f, 5.0f},
     {G192X192, 192, 192, 1, 0.98f, 4.5f},

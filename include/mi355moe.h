@@ -510,8 +510,9 @@ int mi355moe_linear(const mi355moe_linear_args* args, void* workspace,
                     size_t workspace_bytes, void* stream);
 
 /* Rows as int8 codes with a scale each (x, and once the weight, of an int8
- * product):  s = max(max |x|, 1e-10) / 127,  q = x / s to the nearest integer,
- * halves to the even one; both divisions are fp32's, rounded to nearest.  A row
+ * product):  s = max(max |x|, 1e-10) * (1 / 127),  q = x / s to the nearest
+ * integer, halves to the even one, in fp32 (1 / 127, the product and the quotient
+ * rounded to nearest).  A row
  * that holds an infinity or a NaN has that scale and codes of zero, so that a
  * product of it is NaN.  dtype: F32, BF16 or F16.  q [rows, cols] with row stride
  * ldq, scales with stride scale_row; cols <= 2^28. */

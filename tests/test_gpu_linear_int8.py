@@ -6,7 +6,7 @@ another each: 3 U |z|, and the bias adds U |z|.  The activations' slopes are bel
 1.13 (relu2: 2 z); their own arithmetic adds 2^-20 of the value (erf, hardware exp2
 and reciprocal, and the rounding of the exponent's argument, |z| 2^-24).  The
 residual and the output add a rounding each.  Codes and scales of the quantiser
-are those of fp32's divisions, bit for bit."""
+are those of fp32's product and division, bit for bit."""
 import math
 
 import pytest
@@ -44,7 +44,7 @@ def _scales(n, seed, size):
 def _quant(x):
     """Scales and codes in fp32 on the CPU, where a division is rounded to nearest."""
     x = x.cpu().float()
-    s = x.abs().amax(-1, keepdim=True).clamp(min=1e-10) / torch.tensor(127.0)
+    s = x.abs().amax(-1, keepdim=True).clamp(min=1e-10) * torch.tensor(1 / 127, dtype=torch.float32)
     return torch.round(x / s), s
 
 

@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t wave_top(uint32_t m) {
 }
 __device__ __forceinline__ float scale_of(uint32_t top) {
   const float a = __uint_as_float(top);
-  return (a < 1e-10f ? 1e-10f : a) / 127.0f;
+  return (a < 1e-10f ? 1e-10f : a) * (1.0f / 127.0f);
 }
 // The code of v / s.  v * (1 / s) is off by less than 2^-15 (three roundings of a value up
 // to 127), so its nearest integer is the quotient's unless it lies that near the middle

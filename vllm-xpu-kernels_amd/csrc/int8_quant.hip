@@ -1,7 +1,6 @@
 // Rows to int8 codes with a scale each (mi355moe_int8_quant), per row in fp32:
-//   s = max(max |x|, 1e-10) / 127,  q = rint(x / s)
-// both divisions rounded to nearest, so that the codes are the formula's whatever
-// computes them.
+//   s = max(max |x|, 1e-10) * fl(1 / 127),  q = rint(fl(x / s))
+// each rounded to nearest, so that the codes are the formula's whatever computes them.
 //
 // Bound by HBM (each input read once, a byte written for it) from some hundred
 // rows on, by latency below.  A row stays in registers between its maximum and its

@@ -20,7 +20,7 @@ constexpr TileSpec kTiles[] = {
     {G128X128, 128, 128, 1, 0.58f, 3.0f},
     {G96X128, 96, 128, 1, 0.49f, 2.6f},
     {G64X128, 64, 128, 1, 0.4f, 2.0f},
-    {G64X64, 64, 64, 1, 0.31f, 1.7f}};
+    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
 constexpr TileSpec kTilesGated[] = {
     {G256X256, 256, 256, 1, 1.78f, 7.0f},
     {G256X128, 256, 128, 1, 0.98f, 5.0f},
@@ -31,7 +31,7 @@ constexpr TileSpec kTilesGated[] = {
     {G64X128, 64, 128, 1, 0.385f, 2.0f},
     {G192X128, 192, 128, 1, 0.86f, 5.0f},
     {G96X128, 96, 128, 1, 0.49f, 2.6f},
-    {G64X64, 64, 64, 1, 0.31f, 1.7f}};
+    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
 constexpr TileSpec kTilesKeep[] = {
     {G256X256, 256, 256, 1, 1.77f, 12.0f},
     {G256X128, 256, 128, 1, 0.99f, 6.0f},
@@ -43,7 +43,7 @@ constexpr TileSpec kTilesKeep[] = {
     {G192X192, 192, 192, 1, 0.95f, 5.0f},
     {G192X128, 192, 128, 1, 0.69f, 4.0f},
     {G96X128, 96, 128, 1, 0.45f, 2.0f},
-    {G64X64, 64, 64, 1, 0.3f, 1.5f}};
+    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
 
 TilePlan plan(const LinArgs& a) {
   const int nk = static_cast<int>(cdiv(a.K * kind_bytes(kind_of(a)), GSB));

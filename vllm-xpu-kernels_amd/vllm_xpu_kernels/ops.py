@@ -412,7 +412,7 @@ def linear_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
 
 
 def per_token_int8_quant(x: torch.Tensor):
-    """Rows as int8 codes with a scale each: s = max(max |x|, 1e-10) / 127, q = x / s
+    """Rows as int8 codes with a scale each: s = max(max |x|, 1e-10) * (1 / 127), q = x / s
     to the nearest integer (halves to the even one), in fp32.  The input of
     linear_int8 where several products share it, and once the weight of one (its
     scales are then the output channels').

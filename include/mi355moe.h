@@ -503,7 +503,8 @@ typedef struct {
                                        quantised in the call                  */
   float* z;                         /* optional, gated activations of 16-bit
                                        operands: z [M, 2N] with its bias, kept
-                                       for mi355moe_gated_linear_backward     */
+                                       for mi355moe_gated_linear_backward (and
+                                       within its sizes), 16-byte aligned     */
 } mi355moe_linear_args;
 size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* args);
 int mi355moe_linear(const mi355moe_linear_args* args, void* workspace,

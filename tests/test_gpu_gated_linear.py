@@ -304,3 +304,54 @@ def test_a_step_of_a_block_and_its_int8_form():
     # adds 3.5 / 127 / sqrt(12) = 0.8 % of a sum's size, the gated product carries three of them
     diff = got.float() - x.float() - want
     assert float(diff.norm() / want.norm()) < 4 * 0.008 + 2 ** -7 * float(x.float().norm() / want.norm())
+
+
+def test_opcheck():
+    """Schemas, autograd registration, fake tensors and AOT dispatch of the operators here and of the int8
+    ones; the bits of two calls of one operator agree."""
+    from vllm_xpu_kernels import ops
+    assert ops
+    n = torch.ops._mi355_C
+    x, w, b = _rand((5, 64), torch.bfloat16, 1), _rand((32, 64), torch.bfloat16, 2, 0.1), _rand(32, torch.float32, 3)
+    q, s = n.per_token_int8_quant(x)
+    wq, ws = n.per_token_int8_quant(w)
+    out, z = n.gated_linear_keep(x, w, b, 5)
+    d = torch.ones_like(out)
+    for op, args in (
+            (n.per_token_int8_quant, (x,)), (n.linear_int8_new, (q, s, wq, ws, b, None, 0, torch.bfloat16)),
+            (n.linear_int8_new, (x, None, wq, ws, None, None, 5, torch.float32)),
+            (n.linear_int8, (torch.empty(5, 32, device="cuda"), q, s, wq, ws, None, None, 0)),
+            (n.gated_linear_keep, (x, w, b, 6)), (n.gated_linear_backward, (d, x, w, z, 5, torch.float32)),
+            (n.gated_linear, (x, w, b, 7)),
+            (n.gated_linear, (x.clone().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_(), 5))):
+        torch.library.opcheck(op.default, args)
+
+
+def test_traced_by_aot_autograd():
+    """A step of a compiled function (traced forward and backward, run eagerly) is the eager one's."""
+    from vllm_xpu_kernels import ops
+    x, w = _rand((6, 64), torch.bfloat16, 1).requires_grad_(), _rand((32, 64), torch.bfloat16, 2, 0.1).requires_grad_()
+    step = lambda x, w: ops.gated_linear(x, w).float().square().sum()
+    want = torch.autograd.grad(step(x, w), [x, w])
+    got = torch.autograd.grad(torch.compile(step, backend="aot_eager")(x, w), [x, w])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_changed_input_is_noticed():
+    o = _ops()
+    x, w = _rand((6, 64), torch.bfloat16, 1), _rand((32, 64), torch.bfloat16, 2, 0.1).requires_grad_()
+    out = o.gated_linear(x, w)
+    x.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("bad", ["type", "half", "columns", "strides", "bias", "device"])
+def test_refusals(bad):
+    o = _ops()
+    x, w, b = _rand((6, 64), torch.bfloat16, 1).requires_grad_(), _rand((32, 64), torch.bfloat16, 2), _rand(32, torch.float32, 3)
+    change = {"type": lambda: (x.float(), w.float(), b), "half": lambda: (x, w[:31], b[:31]),
+              "columns": lambda: (x[:, :32], w, b), "strides": lambda: (x, w.t().contiguous().t(), b),
+              "bias": lambda: (x, w, b[:16]), "device": lambda: (x, w.cpu(), b)}[bad]
+    with pytest.raises(RuntimeError):
+        o.gated_linear(*change())

@@ -39,6 +39,9 @@ def _linear_args(capi, **kw):
     ({"activation": 5, "z": 16}, b"z is kept for gated activations of 16-bit operands"),
     ({"x_dtype": BF16, "activation": 0, "z": 16}, b"z is kept for gated activations of 16-bit operands"),
     ({"x_dtype": BF16, "weight_dtype": I8, "activation": 5, "z": 16}, b"z is kept for gated"),
+    ({"x_dtype": BF16, "activation": 5, "z": 24}, b"z must be 16-byte aligned"),
+    ({"x_dtype": BF16, "activation": 5, "z": 16, "N": (1 << 20) + 1, "ldo": 1 << 21}, b"too large for a backward pass"),
+    ({"x_dtype": BF16, "activation": 5, "z": 16, "K": (1 << 24) + 1}, b"too large for a backward pass"),
     ({"x": None}, b"null pointer"),
 ])
 def test_linear_refuses(capi, kw, msg):

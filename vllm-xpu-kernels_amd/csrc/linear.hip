@@ -267,6 +267,8 @@ int check(const LinArgs& a) {
   MI_ARG(!(i8 || quantises(a)) || a.K < (1 << 17), "linear: K must be below 131072 for int8 operands");
   MI_ARG(!a.z || (lin_gated(a.activation) && !fp8 && !i8 && !quantises(a)),
          "linear: z is kept for gated activations of 16-bit operands");
+  MI_ARG(!a.z || (reinterpret_cast<uintptr_t>(a.z) & 15) == 0, "linear: z must be 16-byte aligned");
+  MI_ARG(!a.z || (a.N <= (1 << 20) && a.K <= (1 << 24)), "linear: size too large for a backward pass");
   return MI355MOE_OK;
 }
 

@@ -85,7 +85,8 @@ def _close(got, want):
 
 # rows x K x outputs: one row, few, tiles and their edges, splits, sizes that no vector divides
 SIZES = [(1, 8, 8), (1, 1, 1), (2, 33, 5), (16, 512, 128), (17, 100, 33), (61, 2048, 768), (64, 64, 64), (65, 72, 200),
-         (130, 1001, 515), (257, 264, 136), (300, 520, 1024), (512, 1024, 256), (1030, 128, 72), (2050, 256, 192)]
+         (130, 1001, 515), (257, 264, 136), (300, 520, 1024), (512, 1024, 256), (1030, 128, 72), (2050, 256, 192), (800, 1003, 327),
+         (600, 515, 129), (64, 77, 3), (100, 5003, 515)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)
@@ -210,6 +211,15 @@ def test_layouts():
             dx, dw = torch.autograd.grad(out, [x, w], d, retain_graph=True)
             _close(dx.reshape(42, 136), want["dx"])
             _close(dw, want["dw"])
+    # many rows, so that operands are copied where their rows lie anywhere
+    for k0, k in ((0, 1000), (8, 1000), (3, 1000), (0, 1003)):
+        xb, wb = _rand((700, 1016), torch.float16, 1), _rand((800, 1016), torch.float16, 2, 0.05)
+        x, w = xb[:, k0:k0 + k].detach().requires_grad_(), wb[:, k0:k0 + k].detach().requires_grad_()
+        d = _rand((700, 400), torch.float16, 3)
+        want, out = _want(x, w, None, act, d), o.gated_linear(x, w)
+        _close(out.detach(), want["out"])
+        for g, name in zip(torch.autograd.grad(out, [x, w], d), ("dx", "dw")):
+            _close(g, want[name])
     # one row for all: its gradient is the sum
     row = _rand((1, 64), torch.bfloat16, 6).requires_grad_()
     w = _rand((64, 64), torch.bfloat16, 7, 0.1)

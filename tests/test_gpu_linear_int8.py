@@ -95,7 +95,7 @@ ACTS = [None, "silu", "gelu", "gelu_tanh", "relu2", "silu_and_mul", "gelu_and_mu
 # one byte, ends inside a stage and inside 16 bytes
 SIZES = [(1, 1, 1), (1, 7168, 256), (3, 130, 37), (4, 4096, 4096), (8, 2048, 64), (16, 4096, 512), (17, 7168, 130),
          (61, 4096, 384), (64, 272, 128), (65, 2064, 200), (100, 33, 515), (250, 1001, 257), (300, 4096, 1024),
-         (513, 2880, 704), (1100, 144, 1030)]
+         (513, 2880, 704), (1100, 144, 1030), (270, 515, 131), (900, 1003, 583), (257, 4099, 515)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)
@@ -178,6 +178,18 @@ def test_strides_shapes_and_alignment():
         assert out.data_ptr() == wide[:, 3:75].data_ptr()
         _close(out, *_want(xb, s1, wb, s2, None, None, None))
         assert bool((wide[:, :3] == 7).all() and (wide[:, 75:] == 7).all())
+    # many rows: operands copied to aligned ones, each of them or both
+    for off, ld in ((0, 1100), (16, 1104), (3, 1111)):
+        xb = _codes((800 * ld + 16,), 5)[off:off + 800 * ld].view(800, ld)[:, :1024]
+        wb = _codes((720 * 1032,), 6).view(720, 1032)[:, 8:]
+        s1, s2, r = _scales(800, 7, 0.02), _scales(720, 8, 0.002), _rand((800, 721), torch.float16, 9)[:, 1:]
+        _close(o.linear_int8(xb, s1, wb, s2, None, "silu_and_mul"), *_want(xb, s1, wb, s2, None, "silu_and_mul", None))
+        wide = torch.full((800, 727), 7.0, device="cuda", dtype=torch.float16)
+        out = o.linear_int8(xb, s1, wb, s2, residual=r, out=wide[:, 3:723])
+        _close(out, *_want(xb, s1, wb, s2, None, None, r))
+        assert bool((wide[:, :3] == 7).all() and (wide[:, 723:] == 7).all())
+    xb, wb = _codes((40 * 200 + 16,), 5)[15:15 + 40 * 200].view(40, 200), _codes((73 * 200,), 6)[15:15 + 72 * 200].view(72, 200)
+    s1, s2 = _scales(40, 7, 0.02), _scales(72, 8, 0.01)
     # in place over the residual
     r = _rand((40, 72), torch.bfloat16, 9)
     want, e = _want(xb, s1, wb, s2, None, None, r)

@@ -60,6 +60,12 @@ __device__ __forceinline__ void gather8(const V& acc, int g, uint32_t (&o)[8]) {
   }
 }
 
+// 16 bytes to or from an address of any alignment (gfx950's global accesses need none)
+typedef uint32_t any16_t __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void put16(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  *static_cast<any16_t*>(p) = any16_t{a, b, c, d};
+}
+
 // Two runs of 8 columns, a of columns 8 h .. and b of 16 + 8 h .. of row l32: a swap of
 // 16-lane groups gives runs whose lanes cover 32 columns of 16 rows (64 bytes of 16-bit
 // outputs instead of 32): columns 16 (g & 1) + 8 (g / 2) .. of row t16 in a, of row
@@ -158,9 +164,9 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
     tail = k0 + nk == nk_all ? static_cast<int>(a.K % BR) : 0;
     qbase = uniform64(reinterpret_cast<uint64_t>(a.x) + static_cast<uint64_t>((TQ ? i0 : i0 * a.ldx) * EB) + k0 * qstep);
     pbase = uniform64(reinterpret_cast<uint64_t>(a.weight) + static_cast<uint64_t>((TP ? j0 : j0 * a.ldw) * EB) + k0 * pstep);
-    // (q across r: its rows are readable to a multiple of 8 columns)
+    // (rows across r are readable to a multiple of 8 columns)
     const int qlast = static_cast<int>(((a.M + 7) / 8 - i0 / 8 < QCH ? (a.M + 7) / 8 - i0 / 8 : QCH) - 1);
-    const int plast = static_cast<int>((a.N / 8 - j0 / 8 < PCH ? a.N / 8 - j0 / 8 : PCH) - 1);
+    const int plast = static_cast<int>(((a.N + 7) / 8 - j0 / 8 < PCH ? (a.N + 7) / 8 - j0 / 8 : PCH) - 1);
 #pragma unroll
     for (int q = 0; q < ND; ++q) {
       const int r = row_of(q);
@@ -304,11 +310,6 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
     });
   };
 
-  const bool mul16 = ((reinterpret_cast<uintptr_t>(a.out) |
-                              static_cast<uintptr_t>(a.ldo * (a.out_dtype == MI355MOE_F32 ? 4 : 2))) & 15) == 0;
-  [[maybe_unused]] const bool res16 = LIN && a.residual && a.residual_dtype != MI355MOE_F32 &&
-                     ((reinterpret_cast<uintptr_t>(a.residual) | static_cast<uintptr_t>(a.ldr * 2)) & 15) == 0;
-
   place(t);
   first_stages();
   enum { NONE, SOME, WHOLE } behind = NONE;  // stores of the tile before
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
     const int64_t ti = i0, tj = j0;
     const int tsplit = split;
     const bool more = t + lanes8 < xend;  // uniform
-    behind = mul16 && ti + BI <= a.M && tj + BJO <= a.N ? WHOLE : SOME;
+    behind = ti + BI <= a.M && tj + BJO <= a.N ? WHOLE : SOME;
     lds_barrier();  // every wave has read the ring; biases and scales are there
     t += lanes8;
 
@@ -378,7 +379,6 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
         first_stages();
       }
       const int64_t part = static_cast<int64_t>(tsplit) * a.M * a.N;
-      const bool full = tj + BJ <= a.N && (EPI == E_PLAIN ? mul16 : (a.N & 3) == 0);
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
@@ -399,8 +399,8 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
             for (int e = 0; e < 2; ++e) {
               if (m + 16 * e >= a.M) continue;
               uint16_t* o = static_cast<uint16_t*>(a.out) + (m + 16 * e) * a.ldo + n;
-              if (full) {
-                *reinterpret_cast<uint4*>(o) = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+              if (n + 8 <= a.N) {
+                put16(o, w[e][0], w[e][1], w[e][2], w[e][3]);
               } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
@@ -413,9 +413,9 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
             for (int e = 0; e < 2; ++e) {
               if (m + 16 * e >= a.M) continue;
               uint32_t* o = static_cast<uint32_t*>(a.out) + part + (m + 16 * e) * a.N + n;
-              if (full) {
-                reinterpret_cast<uint4*>(o)[0] = make_uint4(v[e][0], v[e][1], v[e][2], v[e][3]);
-                reinterpret_cast<uint4*>(o)[1] = make_uint4(v[e][4], v[e][5], v[e][6], v[e][7]);
+              if (n + 8 <= a.N) {
+                put16(o, v[e][0], v[e][1], v[e][2], v[e][3]);
+                put16(o + 4, v[e][4], v[e][5], v[e][6], v[e][7]);
               } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
@@ -425,8 +425,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
           }
         }
     } else {
-      const bool full = mul16 && tj + BJO <= a.N;
-      const bool early = full && res16;
+      const bool early = a.residual && a.residual_dtype != MI355MOE_F32 && tj + BJO <= a.N;
       // Residuals: all at once where 8 runs of 16 bytes hold them, else one row of tiles
       // ahead (memory operations end in order: a load behind stores waits for them).
       constexpr int RUNS = 2 * NO;
@@ -437,9 +436,10 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
         for (int e = 0; e < RUNS; ++e) {
           int64_t m = ti + xrow + 32 * j + 16 * (e & 1);
           m = m < a.M ? m : a.M - 1;
-          const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) +
-                                                          m * a.ldr + tj + prow(e >> 1) + xcol);
-          r[e][0] = v.x; r[e][1] = v.y; r[e][2] = v.z; r[e][3] = v.w;
+          const any16_t v = *reinterpret_cast<const any16_t*>(static_cast<const uint16_t*>(a.residual) +
+                                                              m * a.ldr + tj + prow(e >> 1) + xcol);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[e][k] = v[k];
         }
       };
       if (early) {
@@ -518,10 +518,10 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
           }
           const int64_t mx = ti + xrow + 32 * j, n = tj + prow(i) + xcol;
           // 8 floats of lane row mx + 16 e
-          auto put = [&](float* o, const uint32_t (&v)[8], bool vec) __attribute__((always_inline)) {
-            if (vec) {
-              reinterpret_cast<uint4*>(o)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-              reinterpret_cast<uint4*>(o)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+          auto put = [&](float* o, const uint32_t (&v)[8]) __attribute__((always_inline)) {
+            if (n + 8 <= a.N) {
+              put16(o, v[0], v[1], v[2], v[3]);
+              put16(o + 4, v[4], v[5], v[6], v[7]);
             } else {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
@@ -531,13 +531,12 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
           if constexpr (EPI == E_KEEP) {
             pair16(kz[0], kz[1]);
             pair16(ku[0], ku[1]);
-            const bool vec = tj + BJO <= a.N && (a.N & 3) == 0;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               if (mx + 16 * e < a.M) {
                 float* zo = a.z + (mx + 16 * e) * 2 * a.N + n;
-                put(zo, kz[e], vec);
-                put(zo + a.N, ku[e], vec);
+                put(zo, kz[e]);
+                put(zo + a.N, ku[e]);
               }
           }
           if (a.out_dtype == MI355MOE_F32) {
@@ -549,7 +548,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
             pair16(w[0], w[1]);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (mx + 16 * e < a.M) put(static_cast<float*>(a.out) + (mx + 16 * e) * a.ldo + n, w[e], full);
+              if (mx + 16 * e < a.M) put(static_cast<float*>(a.out) + (mx + 16 * e) * a.ldo + n, w[e]);
           } else {
             uint32_t w[2][4];
 #pragma unroll
@@ -563,8 +562,8 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
             for (int e = 0; e < 2; ++e) {
               if (mx + 16 * e >= a.M) continue;
               uint16_t* o = static_cast<uint16_t*>(a.out) + (mx + 16 * e) * a.ldo + n;
-              if (full) {
-                *reinterpret_cast<uint4*>(o) = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+              if (n + 8 <= a.N) {
+                put16(o, w[e][0], w[e][1], w[e][2], w[e][3]);
               } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)

@@ -18,6 +18,7 @@ struct QuantArgs {
   int64_t ldq;
   float* scales;
   int64_t scale_row, rows, cols;
+  int pad;  // zeros behind a row's codes: below 16
 };
 
 __device__ __forceinline__ uint32_t workgroup_top(uint32_t m, int waves) {
@@ -67,6 +68,7 @@ __global__ __launch_bounds__(WAVE ? 256 : 1024) void int8_quant_kernel(const Qua
   top = WAVE ? wave_top(top) : workgroup_top(top, lanes >> 6);
   const float s = scale_of(top);
   if (t == 0) a.scales[r * a.scale_row] = s;
+  if (a.pad && t < a.pad) a.q[r * a.ldq + a.cols + t] = 0;
 #pragma unroll
   for (int c = 0; c < R; ++c) {
     const int64_t i = static_cast<int64_t>(c * lanes + t) * 8;
@@ -88,6 +90,7 @@ __global__ __launch_bounds__(1024) void int8_quant_long_kernel(const QuantArgs a
   top = workgroup_top(top, 16);
   const float s = scale_of(top);
   if (threadIdx.x == 0) a.scales[r * a.scale_row] = s;
+  if (threadIdx.x < a.pad) a.q[r * a.ldq + a.cols + threadIdx.x] = 0;
   for (int64_t i = threadIdx.x * 8; i < a.cols; i += 1024 * 8) {
     float f[8];
     row8<E, VEC>(x, i, a.cols, f);
@@ -133,8 +136,9 @@ int launch(const QuantArgs& a, hipStream_t st) {
 }  // namespace
 
 int launch_int8_quant(int dtype, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
-                      int64_t scale_row, int64_t rows, int64_t cols, hipStream_t st) {
-  const QuantArgs a{x, ldx, q, ldq, scales, scale_row, rows, cols};
+                      int64_t scale_row, int64_t rows, int64_t cols, hipStream_t st, bool pad) {
+  const QuantArgs a{x, ldx, q, ldq, scales, scale_row, rows, cols,
+                    pad ? static_cast<int>((16 - cols % 16) % 16) : 0};
   switch (dtype) {
     case MI355MOE_F32: return launch<F32>(a, st);
     case MI355MOE_BF16: return launch<BF16>(a, st);

@@ -296,9 +296,13 @@ __device__ __forceinline__ uint4 row16(const uint8_t* row, bool ok, int64_t c, i
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// codes and scales of 16- or 32-bit rows (int8_quant.hip)
+// codes and scales of 16- or 32-bit rows (int8_quant.hip); pad: zeros behind each row's codes up
+// to a multiple of 16
 int launch_int8_quant(int dtype, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scales,
-                      int64_t scale_row, int64_t rows, int64_t cols, hipStream_t st);
+                      int64_t scale_row, int64_t rows, int64_t cols, hipStream_t st, bool pad = false);
+// rows of `bytes` bytes, ld bytes apart, to rows of a multiple of 16 with zeros behind them
+// (linear.hip)
+int launch_pack_rows(const void* src, int64_t ld, int64_t bytes, void* dst, int64_t rows, hipStream_t st);
 // the sum of a split product's partial sums, in their order, then the epilogue (linear.hip)
 int launch_linear_finish(const LinArgs& a, const void* part, int splits, hipStream_t st);
 // few rows of x (linear_skinny.hip), any alignment; tile: the tiles can take them too

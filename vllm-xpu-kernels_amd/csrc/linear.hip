@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64) void linear_finish_kernel(const LinArgs a,
                                                             int splits, int64_t rows) {
   constexpr int kAhead = 8, H = GATED ? 2 : 1;
   using S = std::conditional_t<I8, int, float>;
-  using S4 = typename SumVec<I8 ? K_I8 : K_BF16, 4>::T;
+  typedef typename SumVec<I8 ? K_I8 : K_BF16, 4>::T S4 __attribute__((aligned(4)));
   const S* part = static_cast<const S*>(parts);
   const int64_t chunks = (a.N + 7) / 8;
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64) void linear_finish_kernel(const LinArgs a,
     for (int k = 0; k < 8; ++k) z[h][k] = 0;
   const int64_t step = a.M * rows;
   const S* p = part + m * rows + n;
-  if ((rows & 3) == 0 && (a.N & 3) == 0 && n + 8 <= a.N) {
+  if (n + 8 <= a.N) {
     for (int s = 0; s < splits; s += kAhead) {
       S4 v[kAhead][H][2];
 #pragma unroll
@@ -272,7 +272,28 @@ int check(const LinArgs& a) {
   return MI355MOE_OK;
 }
 
+// Rows to multiples of 16 bytes, zeros behind them.
+__global__ __launch_bounds__(256) void pack_rows_kernel(const uint8_t* __restrict__ src, int64_t ld,
+                                                        int64_t bytes, uint8_t* __restrict__ dst,
+                                                        int64_t pitch, int64_t rows) {
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 16;
+  if (c >= pitch) return;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    *reinterpret_cast<uint4*>(dst + r * pitch + c) = row16(src + r * ld, true, c, bytes);
+}
+
 }  // namespace
+
+int launch_pack_rows(const void* src, int64_t ld, int64_t bytes, void* dst, int64_t rows, hipStream_t st) {
+  const int64_t pitch = (bytes + 15) / 16 * 16;
+  const int64_t wide = cdiv(pitch, 4096);
+  int64_t high = rows < 4096 ? rows : 4096;
+  pack_rows_kernel<<<dim3(static_cast<unsigned>(wide), static_cast<unsigned>(high)), dim3(256), 0, st>>>(
+      static_cast<const uint8_t*>(src), ld, bytes, static_cast<uint8_t*>(dst), pitch, rows);
+  MI_LAUNCH_CHECK();
+  return MI355MOE_OK;
+}
+
 }  // namespace mi355
 
 using namespace mi355;
@@ -309,59 +330,122 @@ Path path_of(const LinArgs& a) {
 int splits_of(const LinArgs& a, Path path) {
   return path == SKINNY ? 1 : path == TILE ? linear_tile_splits(a) : any_splits(a);
 }
-// Where x is quantised in the call: its codes (rows at multiples of 16 bytes) and
-// scales in the workspace, before the partial sums; `c` becomes the product of them.
 size_t up16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
-size_t code_bytes(LinArgs& c, uintptr_t workspace) {
-  c.ldx = static_cast<int64_t>(up16(static_cast<size_t>(c.K)));
-  const size_t codes = static_cast<size_t>(c.M) * c.ldx;
-  c.x_dtype = MI355MOE_I8;
-  c.x = reinterpret_cast<const void*>(workspace);
-  c.x_scale = reinterpret_cast<const float*>(workspace + codes);
-  c.x_scale_row = 1;
-  return codes + up16(static_cast<size_t>(c.M) * sizeof(float));
+// How a call runs: on which operands, and what of them is made in the workspace before the
+// partial sums.
+struct Call {
+  LinArgs a;          // the product that runs
+  bool quant = false; // x becomes codes (rows at multiples of 16 bytes, zeros behind them) ...
+  bool pack_x = false, pack_w = false;  // ... or is copied to such rows, as is the weight
+  Path path = ANY;
+  int splits = 1;
+  size_t codes = 0, scales = 0, weight = 0, parts = 0, total = 0;  // offsets, and the whole
+};
+// Operands of int8 and of kept sums that direct copies cannot fetch are copied to rows that
+// they can (launch_pack_rows), which pays where many rows share the copied weight (rows x K x
+// weight rows, both kernels in us, through registers / copied: kept 1024 x 6709 x 4094 132 / 103,
+// 512 x 1001 x 2002 27.6 / 22.3, 257 x 1001 x 1030 19.9 / 19.5, 100 x 6709 x 4094 44.8 / 50.2; int8
+// gated 1024 x 6709 x 4094 89 / 63, 257 x 1001 x 1030 27.2 / 17.7, 100 x 6709 x 4094 38.2 / 40.0).
+// Below 10^9 operations the launches of the copies cost a caller more than they save (a step of
+// 257 x 1001 x 1030 from Python 68 / 78).
+constexpr int64_t kPackRows = 256;
+constexpr double kPackWork = 1e9;
+Call call_of(const LinArgs& given, void* workspace) {
+  Call c;
+  c.a = given;
+  LinArgs& a = c.a;
+  const uintptr_t ws = reinterpret_cast<uintptr_t>(workspace);
+  c.quant = quantises(given);
+  if (c.quant && linear_skinny_quantises(given)) {
+    c.path = SKINNY;  // by the kernel itself
+    c.quant = false;
+    return c;
+  }
+  size_t at = 0;
+  if (c.quant) {
+    a.ldx = static_cast<int64_t>(up16(static_cast<size_t>(a.K)));
+    a.x_dtype = MI355MOE_I8;
+    a.x = reinterpret_cast<const void*>(ws);
+    c.scales = static_cast<size_t>(a.M) * a.ldx;
+    a.x_scale = reinterpret_cast<const float*>(ws + c.scales);
+    a.x_scale_row = 1;
+    at = c.scales + up16(static_cast<size_t>(a.M) * sizeof(float));
+  }
+  c.path = path_of(a);
+  if (c.path == ANY && (a.z || a.x_dtype == MI355MOE_I8) && a.M >= kPackRows &&
+      2.0 * a.M * a.K * lin_rows(a) >= kPackWork) {
+    const int64_t eb = kind_bytes(kind_of(a)), pitch = static_cast<int64_t>(up16(static_cast<size_t>(a.K * eb)));
+    auto rows16 = [&](const void* p, int64_t ld) {
+      return a.K * eb % 16 == 0 && ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * eb)) & 15) == 0;
+    };
+    LinArgs b = a;
+    size_t end = at;
+    c.pack_x = !c.quant && !rows16(a.x, a.ldx);
+    if (c.pack_x) {
+      b.x = reinterpret_cast<const void*>(ws + end);
+      b.ldx = pitch / eb;
+      end += static_cast<size_t>(a.M) * pitch;
+    }
+    c.pack_w = !rows16(a.weight, a.ldw);
+    if (c.pack_w) {
+      c.weight = end;
+      b.weight = reinterpret_cast<const void*>(ws + end);
+      b.ldw = pitch / eb;
+      end += static_cast<size_t>(lin_rows(a)) * pitch;
+    }
+    b.K = pitch / eb;
+    if (linear_tile_supported(b)) {
+      a = b;
+      at = end;
+      c.path = TILE;
+    } else {
+      c.pack_x = c.pack_w = false;
+    }
+  }
+  c.splits = splits_of(a, c.path);
+  c.parts = at;
+  c.total = at + lin_partials(a, c.splits);
+  return c;
 }
 }  // namespace
 
 extern "C" size_t mi355moe_linear_workspace_size(const mi355moe_linear_args* p) {
   if (!p || check(*p) || p->M == 0) return 0;
-  LinArgs a = *p;
-  if (quantises(a) && linear_skinny_quantises(a)) return 0;
-  const size_t codes = quantises(a) ? code_bytes(a, 0) : 0;
-  return codes + lin_partials(a, splits_of(a, path_of(a)));
+  return call_of(*p, nullptr).total;
 }
 
 extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
                                size_t workspace_bytes, void* stream) {
   MI_ARG(p, "null pointer");
-  LinArgs a = *p;
-  if (const int rc = check(a)) return rc;
-  if (a.M == 0) return MI355MOE_OK;
-  const bool quant = quantises(a);
-  MI_ARG(a.x && a.weight && a.out, "null pointer");
-  MI_ARG((a.x_dtype != MI355MOE_FP8E4M3 && a.x_dtype != MI355MOE_I8 && !quant) ||
-             ((a.x_scale || quant) && a.weight_scale), "linear: scales missing");
+  const LinArgs given = *p;
+  if (const int rc = check(given)) return rc;
+  if (given.M == 0) return MI355MOE_OK;
+  MI_ARG(given.x && given.weight && given.out, "null pointer");
+  const bool i8 = given.x_dtype == MI355MOE_I8 || quantises(given);
+  MI_ARG((given.x_dtype != MI355MOE_FP8E4M3 && !i8) ||
+             ((given.x_scale || quantises(given)) && given.weight_scale), "linear: scales missing");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (quant && linear_skinny_quantises(a)) return launch_linear_skinny(a, st);
-  const LinArgs given = a;
-  const size_t codes = quant ? code_bytes(a, reinterpret_cast<uintptr_t>(workspace)) : 0;
-  const Path path = path_of(a);
-  const int splits = splits_of(a, path);
-  const size_t need = codes + lin_partials(a, splits);
-  MI_CHECK(need == 0 || (workspace && workspace_bytes >= need), MI355MOE_ERR_WORKSPACE,
+  const Call c = call_of(given, workspace);
+  const LinArgs& a = c.a;
+  MI_CHECK(c.total == 0 || (workspace && workspace_bytes >= c.total), MI355MOE_ERR_WORKSPACE,
            "linear: workspace too small");
-  MI_ARG(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+  MI_ARG(c.total == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
          "linear: workspace must be 16-byte aligned");
-  if (quant) {
-    const int rc = launch_int8_quant(given.x_dtype, given.x, given.ldx, static_cast<int8_t*>(workspace),
-                                     a.ldx, const_cast<float*>(a.x_scale), 1, a.M, a.K, st);
-    if (rc) return rc;
-  }
-  if (path == SKINNY) return launch_linear_skinny(a, st);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t eb = kind_bytes(kind_of(a));
+  int rc = 0;
+  if (c.quant)
+    rc = launch_int8_quant(given.x_dtype, given.x, given.ldx, reinterpret_cast<int8_t*>(ws), a.ldx,
+                           reinterpret_cast<float*>(ws + c.scales), 1, a.M, given.K, st, true);
+  if (!rc && c.pack_x) rc = launch_pack_rows(given.x, given.ldx * eb, given.K * eb, ws, a.M, st);
+  if (!rc && c.pack_w)
+    rc = launch_pack_rows(given.weight, given.ldw * eb, given.K * eb, ws + c.weight, lin_rows(a), st);
+  if (rc) return rc;
+  if (c.path == SKINNY) return launch_linear_skinny(a, st);
   // a split product leaves partial sums (fp32, of int8 products int32) of all weight rows
-  void* parts = static_cast<uint8_t*>(workspace) + codes;
+  void* parts = ws + c.parts;
   LinArgs b = a;
-  if (splits > 1) {
+  if (c.splits > 1) {
     b.N = b.ldo = lin_rows(a);
     b.activation = MI355MOE_LINEAR_NONE;
     b.bias = b.residual = nullptr;
@@ -369,18 +453,17 @@ extern "C" int mi355moe_linear(const mi355moe_linear_args* p, void* workspace,
     b.out_dtype = MI355MOE_F32;
     b.z = nullptr;
   }
-  int rc;
-  if (path == TILE) {
+  if (c.path == TILE) {
     rc = launch_linear_tile(a, b, st);
   } else {
     const int per = any_stages(a);
     switch (kind_of(a)) {
-      case K_FP8: rc = launch_any<K_FP8>(b, splits, per, st); break;
-      case K_I8: rc = launch_any<K_I8>(b, splits, per, st); break;
-      case K_F16: rc = launch_any<K_F16>(b, splits, per, st); break;
-      default: rc = launch_any<K_BF16>(b, splits, per, st);
+      case K_FP8: rc = launch_any<K_FP8>(b, c.splits, per, st); break;
+      case K_I8: rc = launch_any<K_I8>(b, c.splits, per, st); break;
+      case K_F16: rc = launch_any<K_F16>(b, c.splits, per, st); break;
+      default: rc = launch_any<K_BF16>(b, c.splits, per, st);
     }
   }
-  if (rc || splits == 1) return rc;
-  return launch_linear_finish(a, parts, splits, st);
+  if (rc || c.splits == 1) return rc;
+  return launch_linear_finish(a, parts, c.splits, st);
 }

@@ -31,11 +31,12 @@ __device__ __forceinline__ uint2 lds_column4(const uint8_t* at) {
 }
 
 // operands that direct copies to LDS can fetch (product_tile.hip)
-bool product_tile_supported(const Product& p);
+// (padded: p's rows are readable to a multiple of 8 columns)
+bool product_tile_supported(const Product& p, bool padded = false);
 int product_tile_splits(const Product& p);
 int launch_product_tile(const Product& p, float* part, hipStream_t st);
 
-// bytes of partial sums (0: one pass), 16-byte aligned, that launch_product wants
+// bytes of workspace (copied rows, partial sums; 0: neither), 16-byte aligned, that launch_product wants
 size_t product_workspace(const Product& p);
 int launch_product(const Product& p, void* sums, hipStream_t st);
 

@@ -100,12 +100,43 @@ size_t partials(const Product& p, int splits) {
 
 }  // namespace
 
-size_t product_workspace(const Product& p) {
-  if (!p.I) return 0;
-  return partials(p, product_tile_supported(p) ? product_tile_splits(p) : any_splits(p));
+namespace {
+
+// What runs: the product on p's rows, or on a copy of them (launch_pack_rows) in the workspace,
+// before the partial sums.
+struct Run {
+  Product p;
+  bool pack = false, tile = false;
+  int splits = 1;
+  size_t parts = 0, total = 0;
+};
+// p's rows that direct copies cannot fetch are copied to rows that they can: x for dW always, the
+// weight for dx where 64 rows share the copy (rows x K x weight rows, us through registers /
+// copied: dW 1024 x 6709 x 4094 270 / 86, 257 x 1001 x 1030 20.7 / 13.7, 64 x 1001 x 1030 10.8 / 10.3; dx
+// 1024 x 6709 x 4094 360 / 92, 64 x 1001 x 1030 18.3 / 15.4, 40 x 7001 x 6002 52.5 / 56.0).
+// Products below 10^9 operations stay as they are: the copy's launch costs a caller what it saves.
+constexpr int64_t kPackRows = 64;
+constexpr double kPackWork = 1e9;
+Run run_of(const Product& given, void* workspace) {
+  Run r;
+  r.p = given;
+  r.tile = product_tile_supported(given);
+  if (!r.tile && given.R > 0 && (given.transposed || given.I >= kPackRows) &&
+      2.0 * given.I * given.J * given.R >= kPackWork) {
+    Product b = given;
+    b.p = workspace;
+    b.ldp = (given.J + 7) / 8 * 8;
+    if (product_tile_supported(b, true)) {
+      r.p = b;
+      r.pack = r.tile = true;
+      r.parts = static_cast<size_t>(b.R) * b.ldp * 2;
+    }
+  }
+  r.splits = r.tile ? product_tile_splits(r.p) : any_splits(r.p);
+  r.total = r.parts + partials(r.p, r.splits);
+  return r;
 }
 
-namespace {
 int launch_any(const Product& p, int splits, float* part, hipStream_t st) {
   const int per = any_stages(p);
   const dim3 grid(static_cast<unsigned>(cdiv(p.J, PT)), static_cast<unsigned>(cdiv(p.I, PT)),
@@ -120,14 +151,19 @@ int launch_any(const Product& p, int splits, float* part, hipStream_t st) {
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
+
 }  // namespace
 
-int launch_product(const Product& p, void* sums, hipStream_t st) {
-  const bool tile = product_tile_supported(p);
-  const int splits = tile ? product_tile_splits(p) : any_splits(p);
-  float* part = splits > 1 ? static_cast<float*>(sums) : nullptr;
-  const int rc = tile ? launch_product_tile(p, part, st) : launch_any(p, splits, part, st);
-  if (rc || splits == 1) return rc;
+size_t product_workspace(const Product& p) { return p.I ? run_of(p, nullptr).total : 0; }
+
+int launch_product(const Product& given, void* workspace, hipStream_t st) {
+  const Run r = run_of(given, workspace);
+  const Product& p = r.p;
+  if (r.pack)
+    if (const int rc = launch_pack_rows(given.p, given.ldp * 2, given.J * 2, workspace, p.R, st)) return rc;
+  float* part = r.splits > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + r.parts) : nullptr;
+  const int rc = r.tile ? launch_product_tile(p, part, st) : launch_any(p, r.splits, part, st);
+  if (rc || r.splits == 1) return rc;
   LinArgs f{};
   f.out_dtype = p.dtype;
   f.activation = MI355MOE_LINEAR_NONE;
@@ -136,7 +172,7 @@ int launch_product(const Product& p, void* sums, hipStream_t st) {
   f.K = 1;
   f.out = p.out;
   f.ldo = p.ldo;
-  return launch_linear_finish(f, part, splits, st);
+  return launch_linear_finish(f, part, r.splits, st);
 }
 
 }  // namespace mi355

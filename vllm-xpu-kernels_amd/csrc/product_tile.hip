@@ -34,12 +34,12 @@ int launch(const LinArgs& a, bool transposed, const TilePlan& n, hipStream_t st)
 
 }  // namespace
 
-bool product_tile_supported(const Product& p) {
+bool product_tile_supported(const Product& p, bool padded) {
   const int64_t lim = int64_t(1) << 32;
   auto rows16 = [](const void* b, int64_t ld) {
     return ((reinterpret_cast<uintptr_t>(b) | static_cast<uintptr_t>(ld * 2)) & 15) == 0;
   };
-  return p.R > 0 && rows16(p.q, p.ldq) && rows16(p.p, p.ldp) && p.J % 8 == 0 &&
+  return p.R > 0 && rows16(p.q, p.ldq) && rows16(p.p, p.ldp) && (p.J % 8 == 0 || padded) &&
          256 * p.ldq * 2 < lim && 256 * p.ldp * 2 < lim && p.R < (int64_t(1) << 30) &&
          cdiv(p.I, 64) * cdiv(p.J, 64) < (int64_t(1) << 24);  // tiles are counted in 32 bits
 }

@@ -581,7 +581,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
 // A choice of tiles.  us: time of one stage on every CU at once, round: of the rest of a
 // round of tiles (first copies, epilogue); per_cu: workgroups of the tile that a CU holds.
 enum TileShape {
-  G256X256, G256X128, G128X256, G192X192, G192X128, G128X192, G128X128X2, G128X128, G96X128, G64X128, G64X64X2
+  G256X256, G256X128, G128X256, G192X192, G192X128, G128X192, G128X128X2, G128X128, G96X128, G64X128X2, G64X64X3
 };
 struct TileSpec {
   TileShape shape;
@@ -591,7 +591,7 @@ struct TileSpec {
 // a shape's waves take the same columns of both halves of a gated weight, in 32s; G128X192 is
 // for these alone
 constexpr bool gates_of(TileShape s) {
-  return s != G192X192 && s != G192X128 && s != G96X128 && s != G64X64X2;
+  return s != G192X192 && s != G192X128 && s != G96X128 && s != G64X64X3;
 }
 struct TilePlan {
   TileShape shape;
@@ -614,10 +614,11 @@ TilePlan gemm_plan(const TileSpec (&tiles)[N], int64_t I, int64_t J, int64_t row
       if (!gates && c.shape == G128X192) continue;
       const double n = static_cast<double>(cdiv(I, c.bi)) * cdiv(gates ? J : rows, gates ? c.bj / 2 : c.bj) * s;
       if (s > 1 && n > kMaxSplitTiles) continue;
-      // (a CU's only workgroup has its LDS copies to itself: 128 x 128 0.62 us a stage against
-      // 0.97, 64 x 64 0.33 against 0.50)
-      const double stage = c.per_cu == 2 && n <= 256 ? 0.65 * c.us : c.us;
-      double us = __builtin_ceil(n / (256.0 * c.per_cu)) * (stage * per + c.round);
+      // (workgroups that share a CU share its LDS copies: alone, 128 x 128 takes 0.62 us a stage
+      // against 0.97 two together, 64 x 64 0.33 against 0.50 and 0.70)
+      const double most = 256.0 * c.per_cu, fill = n < most ? __builtin_ceil(n / 256) : c.per_cu;
+      const double stage = c.us * (1 + 0.6 * (fill - 1)) / (1 + 0.6 * (c.per_cu - 1));
+      double us = __builtin_ceil(n / most) * (stage * per + c.round);
       if (s > 1) us += 4.0 + 2.0 * s * I * rows * 4 / 3.5e6;
       if (best_us < 0 || us < best_us) {
         best = {c.shape, s, per};
@@ -640,9 +641,10 @@ int launch_gemm(const LinArgs& a, const TilePlan& p, int per_cu, hipStream_t st)
 // Waves and stages.  8 waves hide each other's latency where a CU holds one workgroup: 256 x 256 in
 // 8 waves of 128 x 64 against 4 of 128 x 128, which read a third less from LDS (in turn, us: int8
 // 8192 x 7168 x 4096 gated 214 / 232, kept 421 / 447, dx 8192 x 4096 x 7168 412 / 433, dW 4096 x
-// 8192 x 7168 405 / 413); 128 x 128 in 8 and 4 (int8 1003 x 2880 x 2880 21.0 / 23.9).  64 x 64: two
-// workgroups of four stages to a CU, one of eight (dx 512 x 2048 x 4096 18.6 / 25.7, int8 61 x 4096 x
-// 6144 12.8 / 13.4).
+// 8192 x 7168 405 / 413); 128 x 128 in 8 and 4 (int8 1003 x 2880 x 2880 21.0 / 23.9).  Small
+// tiles share a CU: 64 x 128 with two workgroups of three stages against one of four (dW 2048 x 512 x
+// 4096 16.6 / 21.9, int8 1003 x 2880 x 2880 22.9 / 28.9), 64 x 64 three of three, two of four and
+// one of eight (dx 512 x 2048 x 4096 16.5 / 17.0 / 25.7).
 template <int KIND, bool TQ, bool TP, bool GATED, int EPI>
 int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
   switch (p.shape) {
@@ -668,9 +670,9 @@ int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
       break;
     case G128X128X2: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 2, 2, 2>(a, p, 2, st);
     case G128X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 128, 128, 4, 2, 4>(a, p, 1, st);
-    case G64X128: return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 128, 2, 2, 4>(a, p, 1, st);
-    case G64X64X2:
-      if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 64, 2, 2, 4>(a, p, 2, st);
+    case G64X128X2: return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 128, 2, 2, 3>(a, p, 2, st);
+    case G64X64X3:
+      if constexpr (!GATED) return launch_gemm<KIND, TQ, TP, GATED, EPI, 64, 64, 2, 2, 3>(a, p, 3, st);
       break;
   }
   return set_error(MI355MOE_ERR_UNSUPPORTED, "gemm: no such tile");

@@ -19,8 +19,8 @@ constexpr TileSpec kTiles[] = {
     {G128X128X2, 128, 128, 2, 0.97f, 6.0f},
     {G128X128, 128, 128, 1, 0.58f, 3.0f},
     {G96X128, 96, 128, 1, 0.49f, 2.6f},
-    {G64X128, 64, 128, 1, 0.4f, 2.0f},
-    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
+    {G64X128X2, 64, 128, 2, 0.68f, 2.0f},
+    {G64X64X3, 64, 64, 3, 0.7f, 1.5f}};
 constexpr TileSpec kTilesGated[] = {
     {G256X256, 256, 256, 1, 1.78f, 7.0f},
     {G256X128, 256, 128, 1, 0.98f, 5.0f},
@@ -28,10 +28,10 @@ constexpr TileSpec kTilesGated[] = {
     {G128X192, 128, 192, 1, 0.76f, 5.0f},
     {G128X128X2, 128, 128, 2, 0.97f, 6.0f},
     {G128X128, 128, 128, 1, 0.55f, 3.0f},
-    {G64X128, 64, 128, 1, 0.385f, 2.0f},
+    {G64X128X2, 64, 128, 2, 0.65f, 2.0f},
     {G192X128, 192, 128, 1, 0.86f, 5.0f},
     {G96X128, 96, 128, 1, 0.49f, 2.6f},
-    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
+    {G64X64X3, 64, 64, 3, 0.7f, 1.5f}};
 constexpr TileSpec kTilesKeep[] = {
     {G256X256, 256, 256, 1, 1.77f, 12.0f},
     {G256X128, 256, 128, 1, 0.99f, 6.0f},
@@ -39,11 +39,11 @@ constexpr TileSpec kTilesKeep[] = {
     {G128X192, 128, 192, 1, 0.77f, 5.0f},
     {G128X128X2, 128, 128, 2, 1.05f, 6.0f},
     {G128X128, 128, 128, 1, 0.6f, 3.5f},
-    {G64X128, 64, 128, 1, 0.39f, 2.5f},
+    {G64X128X2, 64, 128, 2, 0.68f, 2.5f},
     {G192X192, 192, 192, 1, 0.95f, 5.0f},
     {G192X128, 192, 128, 1, 0.69f, 4.0f},
     {G96X128, 96, 128, 1, 0.45f, 2.0f},
-    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
+    {G64X64X3, 64, 64, 3, 0.7f, 1.5f}};
 
 TilePlan plan(const LinArgs& a) {
   const int nk = static_cast<int>(cdiv(a.K * kind_bytes(kind_of(a)), GSB));

@@ -16,8 +16,8 @@ constexpr TileSpec kTiles[] = {
     {G128X128X2, 128, 128, 2, 0.99f, 5.0f},
     {G128X128, 128, 128, 1, 0.56f, 3.0f},
     {G96X128, 96, 128, 1, 0.44f, 1.5f},
-    {G64X128, 64, 128, 1, 0.385f, 1.2f},
-    {G64X64X2, 64, 64, 2, 0.5f, 1.5f}};
+    {G64X128X2, 64, 128, 2, 0.65f, 1.5f},
+    {G64X64X3, 64, 64, 3, 0.7f, 1.5f}};
 
 TilePlan plan(const Product& p) {
   return gemm_plan(kTiles, p.I, p.J, p.J, static_cast<int>(cdiv(p.R, GSB / 2)));

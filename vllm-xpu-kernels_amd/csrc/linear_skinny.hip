@@ -355,12 +355,19 @@ int launch_rows(const LinArgs& a, hipStream_t st) {
 // rows it streams the weight once per 16: for weights that leave the tiles
 // short of work (32 x 2048 x 1536 gated 7.0 / 9.6 and 9.7 / 12.0, 61 x 2048 x
 // 1536 8.1 / 9.8 and 10.8 / 10.4; 32 x 2816 x 2816 11.9 / 9.9 and 15.2 / 12.4).
+// int8, whose tiles' sums of a split cost as much and whose stream is half as long, streams more
+// (16 x 7168 x 4096 gated 12.2 / 14.2, 16 x 7168 x 7168 20.2 / 17.3, 32 x 7168 x 4096 gated 14.7 /
+// 15.4, 61 x 2880 x 2880 10.7 / 14.4, 61 x 2048 x 1536 gated 6.5 / 9.9, 61 x 4096 x 4096 20.2 / 13.0;
+// a short K leaves it little to hide its start behind: 32 x 512 x 4096 5.8 / 5.3).
 // Rows that the tiles cannot fetch (`tile` false): any K, and small weights.
 bool linear_skinny_takes(const LinArgs& a, bool tile) {
   const bool fp8 = a.x_dtype == MI355MOE_FP8E4M3;
   if (fp8 && (a.K / 128) * 48 * 4 > kScaleBytes) return false;  // scales beyond their LDS
   const int64_t weight = lin_rows(a) * a.K;
   if (!tile) return a.M <= 16 || (a.M <= 64 && weight <= (int64_t(4) << 20));
+  if (a.x_dtype == MI355MOE_I8)
+    return a.M <= 8 || (a.M <= 16 && weight <= (int64_t(32) << 20)) ||
+           (a.M <= 64 && a.K >= 1024 && cdiv(a.M, 16) * weight <= (int64_t(32) << 20));
   if (a.K > 4096) return a.M <= (fp8 && weight > (int64_t(16) << 20) ? 4 : 8);
   return a.M <= 16 || (a.M <= 64 && cdiv(a.M, 16) * weight <= (int64_t(12) << 20));
 }

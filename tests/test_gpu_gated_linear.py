@@ -365,3 +365,52 @@ def test_refusals(bad):
               "bias": lambda: (x, w, b[:16]), "device": lambda: (x, w.cpu(), b)}[bad]
     with pytest.raises(RuntimeError):
         o.gated_linear(*change())
+
+
+def test_vectors_and_two_backward_passes():
+    o = _ops()
+    x, w = _rand(64, torch.bfloat16, 1).requires_grad_(), _rand((48, 64), torch.bfloat16, 2, 0.1).requires_grad_()
+    b = _rand(48, torch.float16, 3).requires_grad_()
+    out = o.gated_linear(x, w, b)
+    assert out.shape == (24,)
+    for seed in (4, 5):
+        d = _rand(24, torch.bfloat16, seed)
+        want = _want(x[None], w, b, ACTS[0], d[None])
+        dx, dw, db = torch.autograd.grad(out, [x, w, b], d, retain_graph=True)
+        _close(dx[None], want["dx"])
+        _close(dw, want["dw"])
+        _close(db, want["db"])
+        assert db.dtype == torch.float16
+
+
+def test_one_tensor_as_input_and_weight():
+    o = _ops()
+    x = _rand((64, 72), torch.bfloat16, 1, 0.3).requires_grad_()
+    d = _rand((64, 32), torch.bfloat16, 2)
+    want = _want(x, x, None, ACTS[0], d)
+    got, = torch.autograd.grad(o.gated_linear(x, x), x, d)
+    # (two rounded gradients, and the rounding of their sum)
+    half = 2.0 ** -8
+    _close(got, (want["dx"][0] + want["dw"][0], want["dx"][1] + want["dw"][1] +
+                 half * (want["dx"][0].abs() + want["dw"][0].abs() + want["dx"][1] + want["dw"][1])))
+
+
+@pytest.mark.parametrize("K,N", [(512, 768), (1000, 520)])
+def test_many_tiles(K, N):
+    """More tiles than workgroups in each of the three products; and the rows of an expanded weight."""
+    o = _ops()
+    M = 5000
+    x, w = _rand((M, K), torch.bfloat16, 1).requires_grad_(), _rand((2 * N, K), torch.bfloat16, 2, 0.05).requires_grad_()
+    d = _rand((M, N), torch.bfloat16, 3)
+    want = _want(x, w, None, ACTS[0], d)
+    out = o.gated_linear(x, w)
+    _close(out.detach(), want["out"])
+    dx, dw = torch.autograd.grad(out, [x, w], d)
+    _close(dx, want["dx"])
+    _close(dw, want["dw"])
+    row = _rand((1, K), torch.bfloat16, 4, 0.05)
+    wide = row.expand(2 * N, K)
+    want = _want(x, wide, None, ACTS[0], d)
+    out = o.gated_linear(x, wide)
+    _close(out.detach(), want["out"])
+    _close(torch.autograd.grad(out, x, d)[0], want["dx"])

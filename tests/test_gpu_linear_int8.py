@@ -289,3 +289,62 @@ def test_many_rows_and_far_offsets():
     got = o.linear_int8(x, xs, w, ws)
     for m in (0, 65535, M - 1):
         _close(got[m:m + 1], *_want(x[m:m + 1], xs[m:m + 1], w, ws, None, None, None))
+
+
+@pytest.mark.parametrize("M,K,N", [(5, 256, 40), (61, 1024, 200), (300, 256, 136), (300, 1001, 131), (515, 512, 1024)])
+def test_biases_and_residuals_of_other_types(M, K, N):
+    o = _ops()
+    x, w = _codes((M, K), 1), _codes((N, K), 2)
+    xs, ws = _scales(M, 3, 0.02), _scales(N, 4, 0.7 / (73 * math.sqrt(K)))
+    for b in DT.values():
+        for r in DT.values():
+            for out in DT.values():
+                bias, res = _rand(N, b, 5), _rand((M, N), r, 6)
+                got = o.linear_int8(x, xs, w, ws, bias, "gelu", res, out_dtype=out)
+                _close(got, *_want(x, xs, w, ws, bias, "gelu", res))
+    # a residual of rows apart at any address
+    res = _rand((M, N + 5), torch.bfloat16, 7)[:, 3:N + 3]
+    _close(o.linear_int8(x, xs, w, ws, residual=res), *_want(x, xs, w, ws, None, None, res))
+
+
+def test_vectors():
+    o = _ops()
+    w, ws = _codes((24, 64), 1), _scales(24, 2, 0.01)
+    x = _rand(64, torch.float16, 3)
+    q, s = o.per_token_int8_quant(x)
+    assert q.shape == (64,) and s.shape == (1,)
+    a, b = o.linear_int8(x, None, w, ws), o.linear_int8(q, s, w, ws, out_dtype=torch.float16)
+    assert a.shape == (24,) and torch.equal(a, b)
+    _close(a[None], *_want(q[None], s, w, ws, None, None, None))
+
+
+def test_many_tiles_in_place_on_two_streams():
+    """More tiles than workgroups, each stored over the residual that it adds, two products at once."""
+    o = _ops()
+    M, K, N = 3000, 384, 2320
+    x, w, xs, ws = _codes((M, K), 1), _codes((N, K), 2), _scales(M, 3, 0.02), _scales(N, 4, 0.001)
+    r = [_rand((M, N), torch.bfloat16, 5 + i) for i in range(2)]
+    want = [_want(x, xs, w, ws, None, None, t) for t in r]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in r]
+    for st, t in zip(streams, r):
+        with torch.cuda.stream(st):
+            o.linear_int8(x, xs, w, ws, residual=t, out=t)
+    torch.cuda.synchronize()
+    for t, v in zip(r, want):
+        _close(t, *v)
+
+
+@pytest.mark.parametrize("bad", ["scale", "no_scale", "weight_scale", "weight", "type", "fp32", "overlap", "columns", "k"])
+def test_refusals(bad):
+    o = _ops()
+    x, w, xs, ws = _codes((6, 64), 1), _codes((32, 64), 2), _scales(6, 3, 1.0), _scales(32, 4, 1.0)
+    x16 = _rand((6, 64), torch.bfloat16, 5)
+    call = {"scale": lambda: o.linear_int8(x, xs[:5], w, ws), "no_scale": lambda: o.linear_int8(x, None, w, ws),
+            "weight_scale": lambda: o.linear_int8(x, xs, w, ws[:31]), "weight": lambda: o.linear_int8(x16, None, x16, ws),
+            "type": lambda: o.linear_int8(x16, xs, w, ws), "fp32": lambda: o.linear_int8(x16.float(), None, w, ws),
+            "overlap": lambda: o.linear_int8(x16, None, w[:, :64], ws, out=x16[:, :32]),
+            "columns": lambda: o.linear_int8(x[:, :32], xs, w, ws),
+            "k": lambda: o.linear_int8(_codes((1, 1 << 17), 6), xs[:1], _codes((4, 1 << 17), 7), ws[:4])}[bad]
+    with pytest.raises(RuntimeError):
+        call()

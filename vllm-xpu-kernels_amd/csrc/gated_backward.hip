@@ -214,7 +214,7 @@ Layout layout(const GradArgs& a, uintptr_t ws) {
   Layout l{};
   l.ld = (2 * a.N + 7) / 8 * 8;
   // rows of a dz workgroup: 4 to 32, a wave's in turn, for some 1000 workgroups (61 x 1536
-  // 6.5 -> 3.6 us, 257 x 1030 29 -> 9); db's parts bound their number
+  // 6.5 -> 3.4 us, 257 x 1030 29 -> 6.5); db's parts bound their number
   l.per = cdiv(a.M * cdiv(a.N, 512), 1024 * 4) * 4;
   l.per = l.per < 4 ? 4 : l.per > 32 ? 32 : l.per;
   if (a.dbias && cdiv(a.M, l.per) > kRowBlocks) l.per = cdiv(a.M, kRowBlocks);

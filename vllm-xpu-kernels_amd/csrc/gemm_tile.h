@@ -20,8 +20,8 @@
 // The epilogue takes the sums from the registers: a swap of half waves gives each lane 8
 // consecutive columns, stored 16 bytes (32 rows x 32 bytes) at a time; the scales of int8
 // and the biases wait in LDS, residuals are loaded one row of tiles ahead.  No LDS
-// of the ring is needed for that, so a workgroup takes tile after tile (`kPersistent`)
-// and the next one's first stages are on their way meanwhile.
+// of the ring is needed for that, so a workgroup takes tile after tile, and the next one's
+// first stages are on their way meanwhile.
 #pragma once
 
 #include "linear.h"

@@ -49,25 +49,31 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
   const float a = __uint_as_float(top);
   return (a < 1e-10f ? 1e-10f : a) * (1.0f / 127.0f);
 }
-// The code of v / s.  v * (1 / s) is off by less than 2^-15 (three roundings of a value up
-// to 127), so its nearest integer is the quotient's unless it lies that near the middle
-// between two: then the division decides (a few of 100000 values).
-__device__ __forceinline__ int code_of(float v, float s, float inv) {
-  const float t = v * inv;
-  float r = __builtin_rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) < 0x1p-14f) r = __builtin_rintf(v / s);
-  return static_cast<int>(r);
-}
-// 8 codes of a row with scale s: zeros where that is infinite or NaN
+// 8 codes of a row with scale s: zeros where that is infinite or NaN.  v * (1 / s), added
+// to 1.5 * 2^23 in one rounding, leaves its nearest integer (halves to the even one) in the
+// sum's low bits.  1 / s is off by 2^-24 of itself, so that is the quotient's integer unless
+// the quotient lies within 2^-15 of the middle between two (|q| <= 127: 127 * 2^-23 and
+// what the difference's rounding adds): then divisions decide (8 values in a few thousand).
 __device__ __forceinline__ uint2 codes8(const float (&f)[8], float s) {
-  uint32_t w[2] = {0, 0};
-  if (s < __uint_as_float(0x7f800000u)) {
-    const float inv = 1.0f / s;
+  constexpr float kMagic = 12582912.0f;
+  if (!(s < __uint_as_float(0x7f800000u))) return make_uint2(0, 0);
+  const float inv = 1.0f / s;
+  float m[8], off = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      w[k >> 2] |= static_cast<uint32_t>(code_of(f[k], s, inv) & 0xff) << (8 * (k & 3));
+  for (int k = 0; k < 8; ++k) {
+    m[k] = __builtin_fmaf(f[k], inv, kMagic);
+    off = fmaxf(off, fabsf(__builtin_fmaf(f[k], inv, kMagic - m[k])));
   }
-  return make_uint2(w[0], w[1]);
+  if (off > 0.5f - 0x1p-14f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = __builtin_rintf(f[k] / s) + kMagic;
+  }
+  auto bytes4 = [&](int k) __attribute__((always_inline)) {
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(m[k + 1]), __float_as_uint(m[k]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(m[k + 3]), __float_as_uint(m[k + 2]), 0x04000c0cu);
+    return lo | hi;
+  };
+  return make_uint2(bytes4(0), bytes4(4));
 }
 
 }  // namespace mi355

@@ -5,7 +5,8 @@
 // Bound by HBM (each input read once, a byte written for it) from some hundred
 // rows on, by latency below.  A row stays in registers between its maximum and its
 // codes: R chunks of 8 columns per lane, the row's lanes in one wave (4 rows to a
-// workgroup) or in one workgroup.  Longer rows are read twice.
+// workgroup) or in one workgroup.  Longer rows are read twice.  16 x 4096 in fp16 2.6 us,
+// 1003 x 2880 in bf16 4.8, 8192 x 7168 39 (4.5 TB/s; a large copy reaches 5.2).
 #include "int8_quant.h"
 
 namespace mi355 {

@@ -414,3 +414,38 @@ def test_many_tiles(K, N):
     out = o.gated_linear(x, wide)
     _close(out.detach(), want["out"])
     _close(torch.autograd.grad(out, x, d)[0], want["dx"])
+
+
+def test_a_pass_that_asks_for_less():
+    """Gradients of some of the tensors that require one: the same bits, and no tensor for the others."""
+    o = _ops()
+    x, w = _rand((130, 96), torch.bfloat16, 1).requires_grad_(), _rand((128, 96), torch.bfloat16, 2, 0.1).requires_grad_()
+    b, d = _rand(128, torch.float32, 3).requires_grad_(), _rand((130, 64), torch.bfloat16, 4)
+    y = o.gated_linear(x, w, b)
+    want = torch.autograd.grad(y, [x, w, b], d, retain_graph=True)
+    for which in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        got = torch.autograd.grad(y, [(x, w, b)[i] for i in which], d, retain_graph=True)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, which))
+
+
+def test_capture_beside_a_graph_of_the_same_leaves():
+    """A step captured while an eager graph of its leaves lives is refused before it records anything; without
+    the graph it is captured."""
+    o = _ops()
+    x, w = _rand((64, 64), torch.bfloat16, 1).requires_grad_(), _rand((128, 64), torch.bfloat16, 2, 0.1).requires_grad_()
+    d = _rand((64, 64), torch.bfloat16, 3)
+    run = lambda: torch.autograd.grad(o.gated_linear(x, w), [x, w], d)
+    want = run()
+    lives = o.gated_linear(x, w)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="same leaves"), torch.cuda.graph(g):
+        o.gated_linear(x, w)
+    del lives
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, run()))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1291,12 +1291,31 @@ template <typename F>
 auto gated_op(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
+// A graph of a leaf that lives has the leaf's gradient accumulate on its own stream.  The
+// default stream can take no part in a capture, and the attempt would end the process in
+// autograd's thread: a captured step of such a leaf is refused before it records anything.
+void check_capture(const at::Tensor& t) {
+  if (!t.is_cuda() || t.unsafeGetTensorImpl()->is_python_dispatch() || !t.requires_grad() || !t.is_leaf())
+    return;
+  const auto base = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(t.device().index());
+  const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
+  if (here == base) return;
+  const auto sum = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!sum || sum->stream() != base.unwrap()) return;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(here.stream(), &status) == hipSuccess, "gated_linear: stream");
+  TORCH_CHECK(status == hipStreamCaptureStatusNone, "gated_linear: a graph of the same leaves, made on "
+              "the default stream, lives; drop its outputs before a step is captured");
+}
 class GatedLinear : public torch::autograd::Function<GatedLinear> {
  public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& input,
                             const at::Tensor& weight, const std::optional<at::Tensor>& bias,
                             int64_t activation) {
     static const auto op = gated_op<decltype(gated_linear_keep)>("_mi355_C::gated_linear_keep");
+    check_capture(input);
+    check_capture(weight);
+    if (bias) check_capture(*bias);
     at::AutoDispatchBelowADInplaceOrView below;
     auto [out, z] = op.call(input, weight, bias, activation);
     // (what no asked gradient reads is not held)
@@ -1313,13 +1332,16 @@ class GatedLinear : public torch::autograd::Function<GatedLinear> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "gated_linear has no gradient of its gradient");
     at::AutoDispatchBelowADInplaceOrView below;
     const auto saved = ctx->get_saved_variables();
-    auto given = [](const at::Tensor& t) {
-      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+    // (this pass may ask for less than requires a gradient; inputs 0 to 2: input, weight, bias)
+    auto given = [&](const at::Tensor& t, size_t of) {
+      return t.defined() && ctx->needs_input_grad(of) ? std::optional<at::Tensor>(t) : std::nullopt;
     };
     std::optional<at::ScalarType> bias_dtype;
     const auto it = ctx->saved_data.find("bias_dtype");
-    if (it != ctx->saved_data.end()) bias_dtype = static_cast<at::ScalarType>(it->second.toInt());
-    auto [dx, dw, db] = op.call(grads[0], given(saved[0]), given(saved[1]), saved[2],
+    if (it != ctx->saved_data.end() && ctx->needs_input_grad(2))
+      bias_dtype = static_cast<at::ScalarType>(it->second.toInt());
+    if (!bias_dtype && !given(saved[0], 1) && !given(saved[1], 0)) return {{}, {}, {}, {}};
+    auto [dx, dw, db] = op.call(grads[0], given(saved[0], 1), given(saved[1], 0), saved[2],
                                 ctx->saved_data["activation"].toInt(), bias_dtype);
     return {dx, dw, db, at::Tensor()};
   }

@@ -600,31 +600,44 @@ struct TilePlan {
 // The tile and the split of r with the least estimated time for I x `rows` (of p) outputs (J
 // columns where gates halve them) of `nk` stages: rounds of the grid over the CUs, and for a
 // split the partial sums written and read at 3.5 TB/s and a second launch.
+// (A call prices its tiles more than once, and small steps wait for the host: about 0.5 us here.)
 template <int N>
 TilePlan gemm_plan(const TileSpec (&tiles)[N], int64_t I, int64_t J, int64_t rows, int nk) {
   constexpr int kMaxSplits = 16, kMaxSplitTiles = 1 << 16;
+  int splits[kMaxSplits], pers[kMaxSplits], count = 0;
+  for (int s = 1; s <= kMaxSplits; ++s) {
+    const int per = (nk + s - 1) / s;
+    if (s > 1 && per < 4) break;
+    if (s > 1 && (nk + per - 1) / per != s) continue;
+    splits[count] = s;
+    pers[count++] = per;
+  }
   TilePlan best{};
   double best_us = -1;
-  for (const TileSpec& c : tiles)
-    for (int s = 1; s <= kMaxSplits; ++s) {
-      const int per = static_cast<int>(cdiv(nk, s));
-      if (s > 1 && (per < 4 || cdiv(nk, per) != s)) continue;
-      const bool gates = rows != J && s == 1;  // a split product: all rows of p, no gates
-      if (gates && !gates_of(c.shape)) continue;
-      if (!gates && c.shape == G128X192) continue;
-      const double n = static_cast<double>(cdiv(I, c.bi)) * cdiv(gates ? J : rows, gates ? c.bj / 2 : c.bj) * s;
-      if (s > 1 && n > kMaxSplitTiles) continue;
-      // (workgroups that share a CU share its LDS copies: alone, 128 x 128 takes 0.62 us a stage
-      // against 0.97 two together, 64 x 64 0.33 against 0.50 and 0.70)
-      const double most = 256.0 * c.per_cu, fill = n < most ? __builtin_ceil(n / 256) : c.per_cu;
-      const double stage = c.us * (1 + 0.6 * (fill - 1)) / (1 + 0.6 * (c.per_cu - 1));
-      double us = __builtin_ceil(n / most) * (stage * per + c.round);
+  for (const TileSpec& c : tiles) {
+    const bool halves = rows != J;  // gates; a split product has none: all rows of p
+    const int64_t ti = cdiv(I, c.bi), whole = ti * cdiv(rows, c.bj);
+    const int64_t gated = halves ? ti * cdiv(J, c.bj / 2) : whole;
+    const int64_t most = 256 * c.per_cu;
+    // (workgroups that share a CU share its LDS copies: alone, 128 x 128 takes 0.62 us a stage
+    // against 0.97 two together, 64 x 64 0.33 against 0.50 and 0.70)
+    const double alone = c.us / (1 + 0.6 * (c.per_cu - 1));
+    for (int k = 0; k < count; ++k) {
+      const int s = splits[k];
+      const bool gates = halves && s == 1;
+      if (gates ? !gates_of(c.shape) : c.shape == G128X192) continue;
+      const int64_t n = gates ? gated : whole * s;
+      if (s > 1 && n > kMaxSplitTiles) break;
+      double us;
+      if (n < most) us = alone * (1 + 0.6 * static_cast<double>((n + 255) / 256 - 1)) * pers[k] + c.round;
+      else us = static_cast<double>((n + most - 1) / most) * (c.us * pers[k] + c.round);
       if (s > 1) us += 4.0 + 2.0 * s * I * rows * 4 / 3.5e6;
       if (best_us < 0 || us < best_us) {
-        best = {c.shape, s, per};
+        best = {c.shape, s, pers[k]};
         best_us = us;
       }
     }
+  }
   return best;
 }
 

@@ -5,18 +5,22 @@
 
 namespace mi355 {
 
+// 8 values of 16 bits
+template <typename E>
+__device__ __forceinline__ void unpack_row8(uint4 u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[2 * k] = E::ld(static_cast<uint16_t>(w[k]));
+    f[2 * k + 1] = E::ld(static_cast<uint16_t>(w[k] >> 16));
+  }
+}
 // Columns i .. i + 7 of a row: 16-byte loads when VEC (i a multiple of 8), else those
 // below `cols` one by one and zeros.
 template <typename E, bool VEC>
 __device__ __forceinline__ void row8(const typename E::T* p, int64_t i, int64_t cols, float (&f)[8]) {
   if constexpr (VEC && sizeof(typename E::T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f[2 * k] = E::ld(static_cast<uint16_t>(w[k]));
-      f[2 * k + 1] = E::ld(static_cast<uint16_t>(w[k] >> 16));
-    }
+    unpack_row8<E>(*reinterpret_cast<const uint4*>(p + i), f);
   } else if constexpr (VEC) {
     const float4 a = reinterpret_cast<const float4*>(p + i)[0], b = reinterpret_cast<const float4*>(p + i)[1];
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;

@@ -38,18 +38,23 @@ constexpr int kScaleBytes = 48 * 1024;  // LDS for the e4m3 scales
 // The row's scale and codes (K % 16 == 0): each of 256 threads holds 4 chunks of 8 columns
 // at most.
 constexpr int kQuantChunks = 4;
+__device__ __forceinline__ void load_row(const LinArgs& a, int waves, uint4 (&row)[kQuantChunks]) {
+#pragma unroll
+  for (int c = 0; c < kQuantChunks; ++c) {
+    const int64_t i = static_cast<int64_t>(c * 64 * waves + threadIdx.x) * 8;
+    row[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + (i < a.K ? i : 0));
+  }
+}
 template <typename E>
-__device__ __forceinline__ void quantise_row(const LinArgs& a, int waves, float* s_scale, uint8_t* s_code) {
+__device__ __forceinline__ void quantise_row(const LinArgs& a, int waves, const uint4 (&row)[kQuantChunks],
+                                             float* s_scale, uint8_t* s_code) {
   __shared__ uint32_t s_top[4];
   const int tid = threadIdx.x, threads = 64 * waves;
   float f[kQuantChunks][8];
   uint32_t top = 0;
 #pragma unroll
   for (int c = 0; c < kQuantChunks; ++c) {
-    const int64_t i = static_cast<int64_t>(c * threads + tid) * 8;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[c][k] = 0.f;
-    if (i < a.K) row8<E, true>(static_cast<const uint16_t*>(a.x), i, a.K, f[c]);
+    unpack_row8<E>(row[c], f[c]);  // (chunks past the row repeat its first)
     const uint32_t u = top8(f[c]);
     top = u > top ? u : top;
   }
@@ -136,14 +141,26 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   S* red = reinterpret_cast<S*>(s_xs + (FP8 ? (kblocks + 1) * MT * R : 0));
 
   const bool any = s0 < s1;  // uniform per wave
-  if (any) load(w0, x0, s0);
-  // QUANT: the row's scale, then its codes
+  // QUANT: the row's loads before the weights' (loads end in order), which are on their way
+  // while the row's scale and then its codes are made
+  [[maybe_unused]] uint4 row[kQuantChunks];
+  if constexpr (QUANT) {
+    load_row(a, waves, row);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (any) {
+    load(w0, x0, s0);
+    if constexpr (QUANT) {
+      load(w1, x1, s0 + U);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
   float* s_row = lds;
   uint8_t* s_code = reinterpret_cast<uint8_t*>(lds + 4);
   if constexpr (QUANT) {
     red = reinterpret_cast<S*>(s_code + a.K);
-    if (a.x_dtype == MI355MOE_F16) quantise_row<F16>(a, waves, s_row, s_code);
-    else quantise_row<BF16>(a, waves, s_row, s_code);
+    if (a.x_dtype == MI355MOE_F16) quantise_row<F16>(a, waves, row, s_row, s_code);
+    else quantise_row<BF16>(a, waves, row, s_row, s_code);
   }
   if constexpr (FP8) {
     for (int i = tid; i < (kblocks + 1) * NS * R; i += blockDim.x) {
@@ -229,7 +246,7 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
   constexpr bool GUARD = FP8 && GATED && R * MT == 4;
   if (any) {
     for (int s = s0; s < s1; s += 2 * U) {
-      if (!GUARD || s + U < s1) load(w1, x1, s + U);
+      if (QUANT ? s != s0 : !GUARD || s + U < s1) load(w1, x1, s + U);
       compute(w0, x0, s);
       if (GUARD && s + U >= s1) break;
       if (!GUARD || s + 2 * U < s1) load(w0, x0, s + 2 * U);
@@ -327,7 +344,12 @@ int launch_rows(const LinArgs& a, hipStream_t st) {
     // us against 7.0 with four, 4 x 7168 x 4096 gated 10.0 / 10.6, 8 x 4096 x 4096 7.7 / 8.0,
     // 16 x 4096 x 4096 8.3 / 8.9, 16 x 2048 x 1536 gated 5.3 / 5.7).
     if (a.x_dtype != MI355MOE_I8) return launch<KIND, GATED, 4, 1, 2, true>(a, 4, st);
-    if (a.M <= 4) return launch<KIND, GATED, 4, 1, 2>(a, 2, st);
+    // One row over a long K: four waves to a strip where there are not many of them (us, two /
+    // four: 1 x 7168 x 7168 14.1 / 13.1, 1 x 8192 x 8192 gated 17.0 / 15.7, 1 x 2880 x 5760 7.2 / 6.5,
+    // 1 x 4096 x 4096 6.2 / 6.2, but 1 x 2048 x 7168 5.9 / 7.6, 1 x 4096 x 22016 gated 21.0 / 22.6,
+    // 4 x 7168 x 4096 gated 10.2 / 10.4).
+    const bool four = a.M == 1 && a.K >= 2880 && lin_rows(a) <= 8192;
+    if (a.M <= 4) return launch<KIND, GATED, 4, 1, 2>(a, four ? 4 : 2, st);
     if (a.M <= 16 && few) return launch<KIND, GATED, 8, 2, 2>(a, 2, st);
     return launch<KIND, GATED, 16, 1, 2>(a, 4, st);
   } else if constexpr (KIND == K_FP8) {
@@ -374,9 +396,10 @@ bool linear_skinny_takes(const LinArgs& a, bool tile) {
 
 // x that the stream quantises itself: one row at a multiple of 16 bytes.  A launch less, but
 // each workgroup of 4 weight rows quantises it again, so up to 4 of them per CU (both ways in a
-// graph, us: 1 x 7168 x 4096 gated 12.4 / 13.2, 1 x 2048 x 1536 gated 6.0 / 7.1, 1 x 7168 x 256
-// 7.1 / 8.3, 1 x 4096 x 4096 8.4 / 8.9, but 1 x 2048 x 7168 11.6 / 9.5, 1 x 7168 x 7168 19.3 /
-// 17.6, and two rows of 7168 x 4096 gated 14.2 / 13.5).
+// graph, us: 1 x 7168 x 4096 gated 11.7 / 12.7, 1 x 8192 x 8192 gated 16.0 / 18.9, 1 x 2048 x 1536
+// gated 5.6 / 7.1, 1 x 7168 x 256 6.3 / 7.8, 1 x 4096 x 4096 8.2 / 8.9, but 1 x 4096 x 6144 10.8 /
+// 10.1, 1 x 4096 x 14336 17.7 / 15.8).  The row's loads go first: behind the weights' its codes
+// would wait for them (1 x 8192 x 8192 gated 18.7, with fewer weights ahead 19.3).
 bool linear_skinny_quantises(const LinArgs& a) {
   return a.M == 1 && a.N <= 4096 && a.K % 16 == 0 && a.K <= 8 * 256 * kQuantChunks &&
          (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;

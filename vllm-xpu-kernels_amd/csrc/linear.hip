@@ -339,7 +339,7 @@ struct Call {
   bool pack_x = false, pack_w = false;  // ... or is copied to such rows, as is the weight
   Path path = ANY;
   int splits = 1;
-  size_t codes = 0, scales = 0, weight = 0, parts = 0, total = 0;  // offsets, and the whole
+  size_t scales = 0, weight = 0, parts = 0, total = 0;  // offsets, and the whole
 };
 // Operands of int8 and of kept sums that direct copies cannot fetch are copied to rows that
 // they can (launch_pack_rows), which pays where many rows share the copied weight (rows x K x

@@ -449,3 +449,27 @@ def test_capture_beside_a_graph_of_the_same_leaves():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, run()))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("M,K,N,dtype", [(4323, 8456, 684, torch.bfloat16), (3216, 8960, 2039, torch.float16),
+                                         (4078, 8856, 737, torch.bfloat16)])
+def test_gradients_together_and_alone(M, K, N, dtype):
+    """Sizes at which both products run in one launch: their bits are those of each alone, which a sample of
+    rows and columns holds to the formula."""
+    o = _ops()
+    x, w = _rand((M, K), dtype, 1).requires_grad_(), _rand((2 * N, K), dtype, 2, 0.02).requires_grad_()
+    d = _rand((M, N), dtype, 3)
+    y = o.gated_linear(x, w)
+    dx, dw = torch.autograd.grad(y, [x, w], d, retain_graph=True)
+    assert torch.equal(dx, torch.autograd.grad(y, x, d, retain_graph=True)[0])
+    assert torch.equal(dw, torch.autograd.grad(y, w, d)[0])
+    # the product, and its fp32 sum's error: 2^-24 of the sum of sizes for each of its terms
+    both = lambda a, b: (a @ b, a.shape[1] * 2 ** -24 * (a.abs() @ b.abs()))
+    with torch.no_grad():
+        dz = torch.ops._mi355_C.gated_linear_backward.default(
+            d, torch.eye(M, device="cuda", dtype=dtype), None, torch.ops._mi355_C.gated_linear_keep(x, w, None, 5)[1], 5,
+            None)[1]  # [2 N, M]: dz itself, which the products take
+        rows = torch.tensor([0, 1, 255, 256, M // 2, M - 1], device="cuda")
+        _close(dx[rows], both(dz[:, rows].double().t().contiguous(), w.double()))
+        cols = torch.tensor([0, 1, N - 1, N, N + 255, 2 * N - 1], device="cuda")
+        _close(dw[cols], both(dz[cols].double(), x.double()))

@@ -3,7 +3,8 @@
 //   dz1 = dout z2 f'(z1),  dz2 = dout f(z1)
 //   dx = dz W,  dW = dz^T x,  db = sum_m dz
 // Three launches and two more where they are needed: dz (HBM: 8 bytes of z and 2 of
-// dout read, 4 written for each of M x N), the two products (matrix cores), and the
+// dout read, 4 written for each of M x N), the two products (matrix cores; one launch
+// where large ones then fill the last rounds of the CUs), and the
 // sums of split products and of db's parts.
 //
 // Precision.  z stays fp32 (16-bit z would add its rounding to every factor of dz);
@@ -280,6 +281,7 @@ extern "C" int mi355moe_gated_linear_backward(const mi355moe_gated_linear_backwa
         part, l.blocks, 2 * a.N, a.dbias, a.dbias_dtype);
     MI_LAUNCH_CHECK();
   }
+  if (a.dx && a.dweight && a.M && product_pair_supported(l.dx, l.dw)) return launch_product_pair(l.dx, l.dw, st);
   if (a.dx && a.M)
     if (const int rc = launch_product(l.dx, sums, st)) return rc;
   if (a.dweight) return launch_product(l.dw, sums, st);

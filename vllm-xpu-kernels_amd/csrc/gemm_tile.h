@@ -84,10 +84,32 @@ __device__ __forceinline__ void pair16(uint32_t (&a)[N], uint32_t (&b)[N]) {
 constexpr int gemm_waves_per_simd(int waves, int bi, int bj, int stages) {
   return (waves / 4) * (2 * (stages * (bi + bj) * GSB + 4 * (2 * bj + bi)) <= 160 * 1024 ? 2 : 1);
 }
+// The tiles that a workgroup takes, of [t, end): `pre` of them `pre_step` apart, then from `main` on every
+// step-th.
+struct TileWalk {
+  int t, end, step, pre, pre_step, main;
+  __device__ __forceinline__ bool next() {
+    if (pre > 0) t = --pre ? t + pre_step : main;
+    else t += step;
+    return t < end;
+  }
+};
+// Workgroups are dealt round-robin to the 8 XCDs: XCD i takes a contiguous range of
+// tiles, in bands of 4 tiles of q, so that the tiles that run together on an XCD
+// share rows of both operands in its L2.
+__device__ __forceinline__ TileWalk xcd_walk(int total) {
+  const int per = (total + 7) / 8;
+  const int xcd = static_cast<int>(blockIdx.x) & 7;
+  const int end = (xcd + 1) * per < total ? (xcd + 1) * per : total;
+  return {xcd * per + (static_cast<int>(blockIdx.x) >> 3), end, static_cast<int>(gridDim.x) >> 3, 0, 0, 0};
+}
+// floats of biases and scales behind the ring
+constexpr int gemm_side(int kind, int epi, int bi, int bj) {
+  return epi == E_LINEAR || epi == E_KEEP ? bj + (kind == K_I8 ? bi + bj : 0) : 0;
+}
 template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE>
-__global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, NSTAGE)) void gemm_tile_kernel(const LinArgs a, int tiles_i,
-                                                                  int tiles_j, int splits,
-                                                                  int stages_per_split) {
+__device__ __forceinline__ void gemm_tiles(const LinArgs& a, int tiles_i, int tiles_j, int stages_per_split,
+                                           TileWalk walk, uint8_t* lds) {
   constexpr bool I8 = KIND == K_I8;
   constexpr int EB = kind_bytes(KIND);
   static_assert(!(I8 && (TQ || TP)) && !(GATED && TP) && !(TQ && !TP), "operands");
@@ -103,9 +125,6 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
   static_assert(QQ * 8 * WAVES == BI && PQ * 8 * WAVES == BJ, "copies");
   static_assert(!GATED || PQ % 2 == 0, "a copy has rows of one half");
   constexpr bool LIN = EPI == E_LINEAR || EPI == E_KEEP;
-  constexpr int SIDE = (LIN ? BJ : 0) + (LIN && I8 ? BI + BJ : 0);  // floats: biases, scales
-  static_assert(NSTAGE * STAGE + SIDE * 4 <= 160 * 1024, "LDS");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[NSTAGE * STAGE + SIDE * 4];
   float* s_bias = reinterpret_cast<float*>(lds + NSTAGE * STAGE);  // [BJ]
   float* s_ws = s_bias + BJ;                                       // [BJ]
   float* s_xs = s_ws + BJ;                                         // [BI]
@@ -115,15 +134,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
   const int wi = wave / WJ, wj = wave % WJ;
   const int g4 = lane >> 4, t16 = lane & 15, h = lane >> 5, l32 = lane & 31;
 
-  // Workgroups are dealt round-robin to the 8 XCDs: XCD i takes a contiguous range of
-  // tiles, in bands of 4 tiles of q, so that the tiles that run together on an XCD
-  // share rows of both operands in its L2.
-  const int total = tiles_i * tiles_j * splits;
-  const int per = (total + 7) / 8;
-  const int xcd = static_cast<int>(blockIdx.x) & 7, lanes8 = static_cast<int>(gridDim.x) >> 3;
-  const int xend = (xcd + 1) * per < total ? (xcd + 1) * per : total;
-  int t = xcd * per + (static_cast<int>(blockIdx.x) >> 3);
-  if (t >= xend) return;  // uniform
+  if (walk.t >= walk.end) return;  // uniform
 
   // p's rows (along r) of weight tile i, and its columns in the output
   auto prow = [&](int i) __attribute__((always_inline)) {
@@ -310,7 +321,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
     });
   };
 
-  place(t);
+  place(walk.t);
   first_stages();
   enum { NONE, SOME, WHOLE } behind = NONE;  // stores of the tile before
   for (;;) {
@@ -366,16 +377,15 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
     }
     const int64_t ti = i0, tj = j0;
     const int tsplit = split;
-    const bool more = t + lanes8 < xend;  // uniform
+    const bool more = walk.next();  // uniform
     behind = ti + BI <= a.M && tj + BJO <= a.N ? WHOLE : SOME;
     lds_barrier();  // every wave has read the ring; biases and scales are there
-    t += lanes8;
 
     // ---- epilogue
     const int xrow = wi * (BI / WI) + t16, xcol = 16 * (g4 & 1) + 8 * (g4 >> 1);  // see pair16
     if constexpr (!LIN) {
       if (more) {
-        place(t);
+        place(walk.t);
         first_stages();
       }
       const int64_t part = static_cast<int64_t>(tsplit) * a.M * a.N;
@@ -447,7 +457,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
         for (int j = 0; j < (ALL ? MT : 1); ++j) load_res(res[j], j);
       }
       if (more) {
-        place(t);
+        place(walk.t);
         first_stages();
       }
 #pragma unroll
@@ -576,6 +586,16 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
     }
     if (!more) return;
   }
+}
+
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE>
+__global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, NSTAGE)) void gemm_tile_kernel(
+    const LinArgs a, int tiles_i, int tiles_j, int splits, int stages_per_split) {
+  constexpr int BYTES = NSTAGE * (BI + BJ) * GSB + 4 * gemm_side(KIND, EPI, BI, BJ);
+  static_assert(BYTES <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[BYTES];
+  gemm_tiles<KIND, TQ, TP, GATED, EPI, BI, BJ, WI, WJ, NSTAGE>(a, tiles_i, tiles_j, stages_per_split,
+                                                              xcd_walk(tiles_i * tiles_j * splits), lds);
 }
 
 // A choice of tiles.  us: time of one stage on every CU at once, round: of the rest of a

@@ -36,6 +36,10 @@ bool product_tile_supported(const Product& p, bool padded = false);
 int product_tile_splits(const Product& p);
 int launch_product_tile(const Product& p, float* part, hipStream_t st);
 
+// dx and dW in one launch, where that fills the CUs better than one after the other
+bool product_pair_supported(const Product& x, const Product& w);
+int launch_product_pair(const Product& x, const Product& w, hipStream_t st);
+
 // bytes of workspace (copied rows, partial sums; 0: neither), 16-byte aligned, that launch_product wants
 size_t product_workspace(const Product& p);
 int launch_product(const Product& p, void* sums, hipStream_t st);

@@ -32,7 +32,83 @@ int launch(const LinArgs& a, bool transposed, const TilePlan& n, hipStream_t st)
                     : launch_gemm_shape<KIND, false, true, false, E_PLAIN>(a, n, st);
 }
 
+// Two products in one launch, 256 x 256 tiles on 256 workgroups: those of w, then those of x.
+// The workgroups of an XCD that get one tile of w less than the others (`light`, its last
+// ones) take `extra` tiles of x first.
+template <int KIND>
+__global__ __launch_bounds__(512, gemm_waves_per_simd(8, 256, 256, 2)) void product_pair_kernel(
+    const LinArgs w, const LinArgs x, int wi, int wj, int wn, int xi, int xj, int xn, int extra) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * 512 * GSB];
+  const int each = static_cast<int>(gridDim.x) >> 3, lane = static_cast<int>(blockIdx.x) >> 3;
+  gemm_tiles<KIND, true, true, false, E_PLAIN, 256, 256, 2, 4, 2>(w, wi, wj, wn, xcd_walk(wi * wj), lds);
+  TileWalk walk = xcd_walk(xi * xj);
+  const int heavy = (wi * wj + 7) / 8 % each, light = each - heavy;
+  if (extra) {
+    const int base = walk.t - lane;
+    walk.main = base + light * extra + lane;
+    if (lane >= heavy) {
+      walk.t = base + lane - heavy;
+      walk.pre = extra;
+      walk.pre_step = light;
+    } else {
+      walk.t = walk.main;
+    }
+  }
+  gemm_tiles<KIND, false, true, false, E_PLAIN, 256, 256, 2, 4, 2>(x, xi, xj, xn, walk, lds);
+}
+
+// How many tiles of x the light workgroups take first, or -1 where two launches take as
+// long: by the last workgroup's tiles, in stages and their rounds (a whole backward pass in us, two
+// launches / one: 8192 x 7168 x 4096 847 / 813, 4323 x 8456 x 1368 238 / 217, 3216 x 8960 x 4078
+// 479 / 433, 7431 x 8200 x 1362 367 / 351).
+int pair_extra(const Product& x, const Product& w) {
+  const TilePlan px = plan(x), pw = plan(w);
+  if (px.shape != G256X256 || pw.shape != G256X256 || px.splits > 1 || pw.splits > 1) return -1;
+  const int64_t nx = cdiv(cdiv(x.I, 256) * cdiv(x.J, 256), 8), nw = cdiv(cdiv(w.I, 256) * cdiv(w.J, 256), 8);
+  const double cx = kTiles[0].us * px.per + kTiles[0].round, cw = kTiles[0].us * pw.per + kTiles[0].round;
+  const int64_t heavy = nw % 32, light = 32 - heavy;
+  if (!heavy) return -1;
+  int64_t extra = static_cast<int64_t>(cw / cx + 0.5);
+  extra = extra < nx / light ? extra : nx / light;
+  const double first = nw / 32 * cw + (extra * cx > cw ? extra * cx : cw);
+  const double one = first + cdiv(nx - light * extra, 32) * cx;
+  return extra && one < 0.98 * (cdiv(nw, 32) * cw + cdiv(nx, 32) * cx) ? static_cast<int>(extra) : -1;
+}
+
+LinArgs args_of(const Product& p) {
+  LinArgs a{};
+  a.x_dtype = a.out_dtype = p.dtype;
+  a.activation = MI355MOE_LINEAR_NONE;
+  a.M = p.I;
+  a.N = p.J;
+  a.K = p.R;
+  a.x = p.q;
+  a.ldx = p.ldq;
+  a.weight = p.p;
+  a.ldw = p.ldp;
+  a.out = p.out;
+  a.ldo = p.ldo;
+  return a;
+}
+
 }  // namespace
+
+bool product_pair_supported(const Product& x, const Product& w) {
+  return !x.transposed && w.transposed && product_tile_supported(x) && product_tile_supported(w) &&
+         pair_extra(x, w) > 0;
+}
+int launch_product_pair(const Product& x, const Product& w, hipStream_t st) {
+  const int extra = pair_extra(x, w);
+  auto go = [&](auto kind) {
+    product_pair_kernel<decltype(kind)::value><<<dim3(256), dim3(512), 0, st>>>(
+        args_of(w), args_of(x), static_cast<int>(cdiv(w.I, 256)), static_cast<int>(cdiv(w.J, 256)), plan(w).per,
+        static_cast<int>(cdiv(x.I, 256)), static_cast<int>(cdiv(x.J, 256)), plan(x).per, extra);
+  };
+  if (x.dtype == MI355MOE_F16) go(std::integral_constant<int, K_F16>{});
+  else go(std::integral_constant<int, K_BF16>{});
+  MI_LAUNCH_CHECK();
+  return MI355MOE_OK;
+}
 
 bool product_tile_supported(const Product& p, bool padded) {
   const int64_t lim = int64_t(1) << 32;
@@ -46,18 +122,8 @@ bool product_tile_supported(const Product& p, bool padded) {
 int product_tile_splits(const Product& p) { return plan(p).splits; }
 int launch_product_tile(const Product& p, float* part, hipStream_t st) {
   const TilePlan n = plan(p);
-  LinArgs a{};
-  a.x_dtype = a.out_dtype = p.dtype;
-  a.activation = MI355MOE_LINEAR_NONE;
-  a.M = p.I;
-  a.N = p.J;
-  a.K = p.R;
-  a.x = p.q;
-  a.ldx = p.ldq;
-  a.weight = p.p;
-  a.ldw = p.ldp;
-  a.out = n.splits > 1 ? static_cast<void*>(part) : p.out;
-  a.ldo = p.ldo;
+  LinArgs a = args_of(p);
+  if (n.splits > 1) a.out = part;
   return p.dtype == MI355MOE_F16 ? launch<K_F16>(a, p.transposed, n, st)
                                  : launch<K_BF16>(a, p.transposed, n, st);
 }

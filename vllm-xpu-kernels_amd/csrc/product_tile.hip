@@ -32,6 +32,22 @@ int launch(const LinArgs& a, bool transposed, const TilePlan& n, hipStream_t st)
                     : launch_gemm_shape<KIND, false, true, false, E_PLAIN>(a, n, st);
 }
 
+// The workgroups' tiles of the second product: `pre` of them `pre_step` apart, then from `main` on.
+struct SecondWalk {
+  int t, end, step, pre, pre_step, main;
+  __device__ __forceinline__ int after() const { return pre > 1 ? t + pre_step : pre ? main : t + step; }
+  __device__ __forceinline__ bool more() const { return after() < end; }
+  __device__ __forceinline__ void next() {
+    t = after();
+    pre = pre ? pre - 1 : 0;
+  }
+};
+template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE, typename Walk,
+          int BYTES>
+__device__ __forceinline__ void gemm_tiles(const LinArgs& a, int tiles_i, int tiles_j, int stages_per_split,
+                                           Walk walk, uint8_t (&lds)[BYTES]) {
+#include "gemm_tile_body.h"
+}
 // Two products in one launch, 256 x 256 tiles on 256 workgroups: those of w, then those of x.
 // The workgroups of an XCD that get one tile of w less than the others (`light`, its last
 // ones) take `extra` tiles of x first.
@@ -40,20 +56,12 @@ __global__ __launch_bounds__(512, gemm_waves_per_simd(8, 256, 256, 2)) void prod
     const LinArgs w, const LinArgs x, int wi, int wj, int wn, int xi, int xj, int xn, int extra) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * 512 * GSB];
   const int each = static_cast<int>(gridDim.x) >> 3, lane = static_cast<int>(blockIdx.x) >> 3;
-  gemm_tiles<KIND, true, true, false, E_PLAIN, 256, 256, 2, 4, 2>(w, wi, wj, wn, xcd_walk(wi * wj), lds);
-  TileWalk walk = xcd_walk(xi * xj);
+  gemm_tiles<KIND, true, true, false, E_PLAIN, 256, 256, 2, 4, 2>(w, wi, wj, wn, XcdWalk(wi * wj), lds);
+  const XcdWalk all(xi * xj);
   const int heavy = (wi * wj + 7) / 8 % each, light = each - heavy;
-  if (extra) {
-    const int base = walk.t - lane;
-    walk.main = base + light * extra + lane;
-    if (lane >= heavy) {
-      walk.t = base + lane - heavy;
-      walk.pre = extra;
-      walk.pre_step = light;
-    } else {
-      walk.t = walk.main;
-    }
-  }
+  const int base = all.t - lane, main = base + light * extra + lane;
+  const bool first = lane >= heavy;
+  const SecondWalk walk{first ? base + lane - heavy : main, all.end, each, first ? extra : 0, light, main};
   gemm_tiles<KIND, false, true, false, E_PLAIN, 256, 256, 2, 4, 2>(x, xi, xj, xn, walk, lds);
 }
 
@@ -62,6 +70,8 @@ __global__ __launch_bounds__(512, gemm_waves_per_simd(8, 256, 256, 2)) void prod
 // launches / one: 8192 x 7168 x 4096 847 / 813, 4323 x 8456 x 1368 238 / 217, 3216 x 8960 x 4078
 // 479 / 433, 7431 x 8200 x 1362 367 / 351).
 int pair_extra(const Product& x, const Product& w) {
+  // (small ones have no such tiles: their plans, 0.4 us each, are not made again)
+  if (static_cast<double>(x.I) * x.J * x.R < 1e10) return -1;
   const TilePlan px = plan(x), pw = plan(w);
   if (px.shape != G256X256 || pw.shape != G256X256 || px.splits > 1 || pw.splits > 1) return -1;
   const int64_t nx = cdiv(cdiv(x.I, 256) * cdiv(x.J, 256), 8), nw = cdiv(cdiv(w.I, 256) * cdiv(w.J, 256), 8);

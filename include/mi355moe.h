@@ -468,7 +468,8 @@ typedef enum {
  * instruction's), with an F32 output it has fp32's precision.  x_dtype I8, or
  * BF16 / F16 with weight_dtype I8: weight int8 with a scale for each of its rows,
  * z[m, n] = (x_scale[m] * weight_scale[n]) * sum_k x[m, k] weight[n, k] + bias[n]
- * with exact sums (any code, -128 too; K < 131072); 16-bit x becomes codes and
+ * with exact sums (any code, -128 too; K < 131072), the scaled sum and the bias in
+ * one rounding, the same at every M; 16-bit x becomes codes and
  * x_scale in the call, as mi355moe_int8_quant makes them.
  * Row strides ld* and scale strides are in elements; columns of x, weight,
  * bias, residual and out are contiguous.  M may be 0; N and K are positive.

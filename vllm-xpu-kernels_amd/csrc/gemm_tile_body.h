@@ -389,7 +389,7 @@
               }
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
-                if constexpr (I8) o[k] = static_cast<float>(static_cast<int>(v[k])) * (xs * w[k]) + b[k];
+                if constexpr (I8) o[k] = scaled_sum(static_cast<int>(v[k]), xs, w[k], b[k]);
                 else o[k] = __uint_as_float(v[k]) + b[k];
               }
             };
@@ -405,18 +405,18 @@
             lin_act(a.activation, z);
             if constexpr (GATED) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) z[k] *= u[k];
+              for (int k = 0; k < 8; ++k) z[k] = times(z[k], u[k]);
             }
             if (early) {
               float r[8];
               const uint32_t(&rr)[4] = e ? r1 : r0;
               unpack8(make_uint4(rr[0], rr[1], rr[2], rr[3]), a.residual_dtype, r);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) z[k] += r[k];
+              for (int k = 0; k < 8; ++k) z[k] = plus(z[k], r[k]);
             } else if (a.residual) {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                if (on && n + k < a.N) z[k] += ld_any(a.residual, a.residual_dtype, m * a.ldr + n + k);
+                if (on && n + k < a.N) z[k] = plus(z[k], ld_any(a.residual, a.residual_dtype, m * a.ldr + n + k));
             }
           }
           const int64_t mx = ti + xrow + 32 * j, n = tj + prow(i) + xcol;

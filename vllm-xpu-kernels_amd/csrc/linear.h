@@ -24,8 +24,12 @@
 // alignment always convert.
 //
 // int8 products.  Sums of 8-bit products are int32 and exact (K < 2^17: 2^17 products
-// of -128 reach 2^31), so a result is the same whichever kernel, tile or split made
-// it:  z[m, n] = float(sum) * (x_scale[m] * weight_scale[n]) + bias[n].
+// of -128 reach 2^31), and every kernel takes the same fp32 steps from there, so a result is
+// the same whichever kernel, tile or split made it:
+//   z[m, n] = fma(float(sum), x_scale[m] * weight_scale[n], bias[n] or 0)  (scaled_sum),
+// then the activation, a product with the gated factor and a sum with the residual, each
+// rounded once (times, plus: the compiler would contract such a pair where both
+// meet in one block, in some kernels and not in others).
 #pragma once
 
 #include <type_traits>
@@ -96,6 +100,20 @@ __device__ __forceinline__ float w_scale_of(const LinArgs& a, int64_t n) {
   return a.weight_scale[n * a.weight_scale_row];
 }
 
+// ... and its sum, scaled and biased in one rounding (bias: 0 where there is none)
+__device__ __forceinline__ float scaled_sum(int sum, float x_scale, float weight_scale, float bias) {
+  return __builtin_fmaf(static_cast<float>(sum), x_scale * weight_scale, bias);
+}
+// the products and sums of an epilogue, never contracted
+__device__ __forceinline__ float times(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+__device__ __forceinline__ float plus(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
+
 // f of the activation (gated ones: f of the gate).  x sigmoid(k x) with the
 // hardware exp2 and reciprocal (about 1 ulp each): a finite x whose exp2
 // overflows gives x * rcp(inf) = -0, one whose exp2 vanishes gives x; x = inf
@@ -113,7 +131,7 @@ __device__ __forceinline__ float lin_f(float z) {
     return mul_sigmoid(z, 1.5957691216057308f * (z + 0.044715f * (z * z * z)));
   else if constexpr (ACT == MI355MOE_LINEAR_RELU2) {
     const float r = z < 0.f ? 0.f : z;  // keeps NaN
-    return r * r;
+    return times(r, r);
   } else return z;
 }
 // f of N values: one (uniform) branch for all
@@ -143,25 +161,33 @@ __device__ __forceinline__ void lin_act(int act, float (&y)[N]) {
   }
 }
 
-// One output: z and, for gated activations, the factor u, both without bias.
+// One output: z and, for gated activations, the factor u, both without bias (BIASED: with it).
 // KEEP: z and u with their biases are kept too (a.z).
-template <bool KEEP = false>
+template <bool KEEP = false, bool BIASED = false>
 __device__ __forceinline__ float lin_value(const LinArgs& a, int64_t m, int64_t n, float z,
                                            float u) {
-  if (a.bias) z += ld_any(a.bias, a.bias_dtype, n);
+  if (!BIASED && a.bias) z += ld_any(a.bias, a.bias_dtype, n);
   float v[1] = {z};
   lin_act(a.activation, v);
   float y = v[0];
   if (lin_gated(a.activation)) {
-    if (a.bias) u += ld_any(a.bias, a.bias_dtype, a.N + n);
-    y *= u;
+    if (!BIASED && a.bias) u += ld_any(a.bias, a.bias_dtype, a.N + n);
+    y = times(y, u);
   }
   if constexpr (KEEP) {
     a.z[m * 2 * a.N + n] = z;
     a.z[(m * 2 + 1) * a.N + n] = u;
   }
-  if (a.residual) y += ld_any(a.residual, a.residual_dtype, m * a.ldr + n);
+  if (a.residual) y = plus(y, ld_any(a.residual, a.residual_dtype, m * a.ldr + n));
   return y;
+}
+// The same of an int8 product's sums.
+__device__ __forceinline__ float lin_value_i32(const LinArgs& a, int64_t m, int64_t n, float x_scale,
+                                               int z, int u) {
+  auto scaled = [&](int sum, int64_t row) __attribute__((always_inline)) {
+    return scaled_sum(sum, x_scale, w_scale_of(a, row), a.bias ? ld_any(a.bias, a.bias_dtype, row) : 0.f);
+  };
+  return lin_value<false, true>(a, m, n, scaled(z, n), lin_gated(a.activation) ? scaled(u, a.N + n) : 0.f);
 }
 
 __device__ __forceinline__ void unpack8(uint4 v, int dtype, float (&f)[8]) {
@@ -206,22 +232,22 @@ __device__ __forceinline__ void st8_f32(float* p, const float (&y)[8], bool vec)
   }
 }
 // Outputs n .. n + 7 (those below N) of row m from their sums z and, for gated
-// activations, u.  vec: out's rows start at multiples of 16 bytes.  early: res
-// holds the 8 (16-bit) residuals, loaded before.
-template <bool KEEP = false>
+// activations, u (BIASED: with their biases).  vec: out's rows start at multiples of 16 bytes.
+// early: res holds the 8 (16-bit) residuals, loaded before.
+template <bool KEEP = false, bool BIASED = false>
 __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t n, const float* zp,
                                            const float* up, bool vec, bool early = false,
                                            uint4 res = uint4{}) {
   if (n + 8 > a.N) {
     for (int k = 0; k < 8 && n + k < a.N; ++k)
-      st_any(a.out, a.out_dtype, m * a.ldo + n + k, lin_value<KEEP>(a, m, n + k, zp[k], up[k]));
+      st_any(a.out, a.out_dtype, m * a.ldo + n + k, lin_value<KEEP, BIASED>(a, m, n + k, zp[k], up[k]));
     return;
   }
   const bool gated = lin_gated(a.activation);
   float y[8], t[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) y[k] = zp[k];
-  if (a.bias) {
+  if (!BIASED && a.bias) {
     ld8_any(a.bias, a.bias_dtype, n, t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] += t[k];
@@ -232,23 +258,23 @@ __device__ __forceinline__ void lin_store8(const LinArgs& a, int64_t m, int64_t 
     float u[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) u[k] = up[k];
-    if (a.bias) {
+    if (!BIASED && a.bias) {
       ld8_any(a.bias, a.bias_dtype, a.N + n, t);
 #pragma unroll
       for (int k = 0; k < 8; ++k) u[k] += t[k];
     }
     if constexpr (KEEP) st8_f32(a.z + (m * 2 + 1) * a.N + n, u, (a.N & 3) == 0);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] *= u[k];
+    for (int k = 0; k < 8; ++k) y[k] = times(y[k], u[k]);
   }
   if (early) {
     unpack8(res, a.residual_dtype, t);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] += t[k];
+    for (int k = 0; k < 8; ++k) y[k] = plus(y[k], t[k]);
   } else if (a.residual) {
     ld8_any(a.residual, a.residual_dtype, m * a.ldr + n, t);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] += t[k];
+    for (int k = 0; k < 8; ++k) y[k] = plus(y[k], t[k]);
   }
   if (!vec) {
 #pragma unroll
@@ -271,13 +297,26 @@ __device__ __forceinline__ void lin_store8_i32(const LinArgs& a, int64_t m, int6
                                                const int* up, bool vec) {
   const float xs = x_scale_of(a, m);
   float z[8], u[8];
+  auto scaled = [&](const int* sums, int64_t row, float (&o)[8]) __attribute__((always_inline)) {
+    float b[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t c = n + k < a.N ? n + k : a.N - 1;
-    z[k] = static_cast<float>(zp[k]) * (xs * w_scale_of(a, c));
-    u[k] = lin_gated(a.activation) ? static_cast<float>(up[k]) * (xs * w_scale_of(a, a.N + c)) : 0.f;
-  }
-  lin_store8(a, m, n, z, u, vec);
+    for (int k = 0; k < 8; ++k) b[k] = 0.f;
+    if (a.bias && n + 8 <= a.N) {
+      ld8_any(a.bias, a.bias_dtype, row, b);
+    } else if (a.bias) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (n + k < a.N) b[k] = ld_any(a.bias, a.bias_dtype, row + k);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      o[k] = scaled_sum(sums[k], xs, w_scale_of(a, n + k < a.N ? row + k : row), b[k]);
+  };
+  scaled(zp, n, z);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) u[k] = 0.f;
+  if (lin_gated(a.activation)) scaled(up, a.N + n, u);
+  lin_store8<false, true>(a, m, n, z, u, vec);
 }
 
 // 16 bytes from column byte c of a row of `bytes` bytes, from any address;

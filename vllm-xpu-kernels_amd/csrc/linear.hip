@@ -137,10 +137,8 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a, int pe
       if constexpr (RAW) {
         static_cast<int*>(a.out)[part + m * a.ldo + n] = acc[0][j][r];
       } else if constexpr (KIND == K_I8) {
-        const float xs = x_scale_of(a, m);
-        const float z = static_cast<float>(acc[0][j][r]) * (xs * w_scale_of(a, n));
-        const float u = GATED ? static_cast<float>(acc[NH - 1][j][r]) * (xs * w_scale_of(a, a.N + n)) : 0.f;
-        st_any(a.out, a.out_dtype, part + m * a.ldo + n, lin_value(a, m, n, z, u));
+        st_any(a.out, a.out_dtype, part + m * a.ldo + n,
+               lin_value_i32(a, m, n, x_scale_of(a, m), acc[0][j][r], acc[NH - 1][j][r]));
       } else {
         st_any(a.out, a.out_dtype, part + m * a.ldo + n,
                lin_value<KEEP>(a, m, n, acc[0][j][r], acc[NH - 1][j][r]));

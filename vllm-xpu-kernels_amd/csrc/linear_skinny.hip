@@ -304,13 +304,10 @@ __global__ __launch_bounds__(256) void linear_skinny_kernel(const LinArgs a) {
         z += p[0];
         if constexpr (GATED) u += p[MT * TILE];
       }
-    float zf = static_cast<float>(z), uf = static_cast<float>(u);
-    if constexpr (I8) {
-      const float xs = QUANT ? *s_row : x_scale_of(a, m);
-      zf *= xs * w_scale_of(a, n);
-      if constexpr (GATED) uf *= xs * w_scale_of(a, a.N + n);
-    }
-    st_any(a.out, a.out_dtype, m * a.ldo + n, lin_value(a, m, n, zf, uf));
+    float y;
+    if constexpr (I8) y = lin_value_i32(a, m, n, QUANT ? *s_row : x_scale_of(a, m), z, u);
+    else y = lin_value(a, m, n, z, u);
+    st_any(a.out, a.out_dtype, m * a.ldo + n, y);
   }
 }
 

@@ -530,8 +530,8 @@ int mi355moe_int8_quant(const void* x, int dtype, int64_t ldx, int8_t* q, int64_
  * one rounding); dbias sums its fp32 values.  Each gradient is optional, one at
  * least is asked for.  x, weight, dout, dx and dweight have `dtype`, row strides
  * in elements and contiguous columns; z is contiguous.  M may be 0: dweight and
- * dbias are then zeros.  No output overlaps an input or another output.  The
- * workspace is 16-byte aligned, of
+ * dbias are then zeros, and dx, which is empty, may be null.  No output overlaps
+ * an input or another output.  The workspace is 16-byte aligned, of
  * mi355moe_gated_linear_backward_workspace_size bytes, asked with the call's own
  * arguments (alignments take part).  M <= 4194240, N <= 2^20, K <= 2^24. */
 typedef struct {

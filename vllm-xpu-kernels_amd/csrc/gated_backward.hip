@@ -197,7 +197,8 @@ int check(const GradArgs& a) {
          "gated_linear_backward: negative stride");
   MI_ARG(!a.dx || a.M <= 1 || a.lddx >= a.K, "gated_linear_backward: rows of dx overlap");
   MI_ARG(!a.dweight || a.lddw >= a.K, "gated_linear_backward: rows of dweight overlap");
-  MI_ARG(a.dx || a.dweight || a.dbias, "gated_linear_backward: no gradient is asked for");
+  // (without rows dx has no elements, so it may have no address)
+  MI_ARG(a.M == 0 || a.dx || a.dweight || a.dbias, "gated_linear_backward: no gradient is asked for");
   return MI355MOE_OK;
 }
 

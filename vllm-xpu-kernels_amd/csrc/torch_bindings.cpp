@@ -943,6 +943,7 @@ std::vector<at::Tensor> rms_norm_new(const at::Tensor& input, const at::Tensor& 
 
 // [.., cols] as [rows, cols] with one row stride
 int64_t row_stride(const at::Tensor& t, const char* name) {
+  if (t.numel() == 0) return t.size(-1);  // (any strides: an expanded one counts as contiguous)
   TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
   int64_t ld = t.size(-1);
   bool set = false;

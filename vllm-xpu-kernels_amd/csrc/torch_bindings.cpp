@@ -14,6 +14,8 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <memory>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/mi355moe.h"
@@ -1292,21 +1294,40 @@ template <typename F>
 auto gated_op(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
-// A graph of a leaf that lives has the leaf's gradient accumulate on its own stream.  The
-// default stream can take no part in a capture, and the attempt would end the process in
-// autograd's thread: a captured step of such a leaf is refused before it records anything.
-void check_capture(const at::Tensor& t) {
-  if (!t.is_cuda() || t.unsafeGetTensorImpl()->is_python_dispatch() || !t.requires_grad() || !t.is_leaf())
-    return;
-  const auto base = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(t.device().index());
-  const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
-  if (here == base) return;
-  const auto sum = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!sum || sum->stream() != base.unwrap()) return;
+// A backward pass takes each node of the graph on the stream that the node was made on: a
+// leaf's accumulation on that of the first graph of the leaf that still lives.  The default stream
+// can take no part in a capture, and the attempt would end the process in autograd's thread: a
+// captured step whose inputs' graph reaches a node of the default stream, through whatever
+// operations, is refused before it records anything.
+void check_capture(const at::Tensor& input, const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
+  using torch::autograd::Node;
+  if (!input.is_cuda() || input.unsafeGetTensorImpl()->is_python_dispatch()) return;
+  const auto here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(input.device().index());
+  if (here == c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(input.device().index())) return;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   TORCH_CHECK(hipStreamIsCapturing(here.stream(), &status) == hipSuccess, "gated_linear: stream");
-  TORCH_CHECK(status == hipStreamCaptureStatusNone, "gated_linear: a graph of the same leaves, made on "
-              "the default stream, lives; drop its outputs before a step is captured");
+  if (status == hipStreamCaptureStatusNone) return;
+  std::vector<std::shared_ptr<Node>> roots;
+  for (const at::Tensor* t : {&input, &weight, bias ? &*bias : nullptr}) {
+    if (!t || !t->requires_grad()) continue;
+    roots.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+  }
+  std::vector<Node*> todo;
+  std::unordered_set<Node*> seen;
+  auto reach = [&](const std::shared_ptr<Node>& n) {
+    if (n && seen.insert(n.get()).second) todo.push_back(n.get());
+  };
+  for (const auto& n : roots) reach(n);
+  while (!todo.empty()) {
+    Node* n = todo.back();
+    todo.pop_back();
+    const auto s = n->stream();
+    TORCH_CHECK(!s || *s != c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(s->device_index()).unwrap(),
+                "gated_linear: the captured step's graph reaches nodes of the default stream: a graph of the "
+                "same leaves lives, or an input was made before the capture; drop the outputs of that graph, or "
+                "detach the input, before a step is captured");
+    for (const auto& e : n->next_edges()) reach(e.function);
+  }
 }
 class GatedLinear : public torch::autograd::Function<GatedLinear> {
  public:
@@ -1314,9 +1335,7 @@ class GatedLinear : public torch::autograd::Function<GatedLinear> {
                             const at::Tensor& weight, const std::optional<at::Tensor>& bias,
                             int64_t activation) {
     static const auto op = gated_op<decltype(gated_linear_keep)>("_mi355_C::gated_linear_keep");
-    check_capture(input);
-    check_capture(weight);
-    if (bias) check_capture(*bias);
+    check_capture(input, weight, bias);
     at::AutoDispatchBelowADInplaceOrView below;
     auto [out, z] = op.call(input, weight, bias, activation);
     // (what no asked gradient reads is not held)

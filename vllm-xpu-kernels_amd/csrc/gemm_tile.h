@@ -27,6 +27,7 @@
 #include "linear.h"
 #include "product.h"
 #include "tile.h"
+#include "tile_walk.h"
 
 namespace mi355 {
 
@@ -84,21 +85,6 @@ __device__ __forceinline__ void pair16(uint32_t (&a)[N], uint32_t (&b)[N]) {
 constexpr int gemm_waves_per_simd(int waves, int bi, int bj, int stages) {
   return (waves / 4) * (2 * (stages * (bi + bj) * GSB + 4 * (2 * bj + bi)) <= 160 * 1024 ? 2 : 1);
 }
-// The tiles that a workgroup takes: every step-th of [t, end).  Workgroups are dealt
-// round-robin to the 8 XCDs: XCD i takes a contiguous range of tiles, in bands of 4 tiles
-// of q, so that the tiles that run together on an XCD share rows of both operands in its L2.
-struct XcdWalk {
-  int t, end, step;
-  __device__ __forceinline__ explicit XcdWalk(int total) {
-    const int per = (total + 7) / 8;
-    const int xcd = static_cast<int>(blockIdx.x) & 7;
-    step = static_cast<int>(gridDim.x) >> 3;
-    end = (xcd + 1) * per < total ? (xcd + 1) * per : total;
-    t = xcd * per + (static_cast<int>(blockIdx.x) >> 3);
-  }
-  __device__ __forceinline__ bool more() const { return t + step < end; }
-  __device__ __forceinline__ void next() { t += step; }
-};
 // floats of biases and scales behind the ring
 constexpr int gemm_side(int kind, int epi, int bi, int bj) {
   return epi == E_LINEAR || epi == E_KEEP ? bj + (kind == K_I8 ? bi + bj : 0) : 0;
@@ -109,7 +95,7 @@ __global__ __launch_bounds__(64 * WI * WJ, gemm_waves_per_simd(WI * WJ, BI, BJ, 
   constexpr int BYTES = NSTAGE * (BI + BJ) * GSB + 4 * gemm_side(KIND, EPI, BI, BJ);
   static_assert(BYTES <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[BYTES];
-  XcdWalk walk(tiles_i * tiles_j * splits);
+  XcdWalk walk(tiles_i * tiles_j * splits, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
 #include "gemm_tile_body.h"
 }
 

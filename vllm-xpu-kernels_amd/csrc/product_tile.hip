@@ -32,37 +32,23 @@ int launch(const LinArgs& a, bool transposed, const TilePlan& n, hipStream_t st)
                     : launch_gemm_shape<KIND, false, true, false, E_PLAIN>(a, n, st);
 }
 
-// The workgroups' tiles of the second product: `pre` of them `pre_step` apart, then from `main` on.
-struct SecondWalk {
-  int t, end, step, pre, pre_step, main;
-  __device__ __forceinline__ int after() const { return pre > 1 ? t + pre_step : pre ? main : t + step; }
-  __device__ __forceinline__ bool more() const { return after() < end; }
-  __device__ __forceinline__ void next() {
-    t = after();
-    pre = pre ? pre - 1 : 0;
-  }
-};
 template <int KIND, bool TQ, bool TP, bool GATED, int EPI, int BI, int BJ, int WI, int WJ, int NSTAGE, typename Walk,
           int BYTES>
 __device__ __forceinline__ void gemm_tiles(const LinArgs& a, int tiles_i, int tiles_j, int stages_per_split,
                                            Walk walk, uint8_t (&lds)[BYTES]) {
 #include "gemm_tile_body.h"
 }
-// Two products in one launch, 256 x 256 tiles on 256 workgroups: those of w, then those of x.
-// The workgroups of an XCD that get one tile of w less than the others (`light`, its last
-// ones) take `extra` tiles of x first.
+// Two products in one launch, 256 x 256 tiles on 256 workgroups: those of w, then those of x
+// (tile_walk.h).
 template <int KIND>
 __global__ __launch_bounds__(512, gemm_waves_per_simd(8, 256, 256, 2)) void product_pair_kernel(
     const LinArgs w, const LinArgs x, int wi, int wj, int wn, int xi, int xj, int xn, int extra) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * 512 * GSB];
-  const int each = static_cast<int>(gridDim.x) >> 3, lane = static_cast<int>(blockIdx.x) >> 3;
-  gemm_tiles<KIND, true, true, false, E_PLAIN, 256, 256, 2, 4, 2>(w, wi, wj, wn, XcdWalk(wi * wj), lds);
-  const XcdWalk all(xi * xj);
-  const int heavy = (wi * wj + 7) / 8 % each, light = each - heavy;
-  const int base = all.t - lane, main = base + light * extra + lane;
-  const bool first = lane >= heavy;
-  const SecondWalk walk{first ? base + lane - heavy : main, all.end, each, first ? extra : 0, light, main};
-  gemm_tiles<KIND, false, true, false, E_PLAIN, 256, 256, 2, 4, 2>(x, xi, xj, xn, walk, lds);
+  const int block = static_cast<int>(blockIdx.x), blocks = static_cast<int>(gridDim.x);
+  gemm_tiles<KIND, true, true, false, E_PLAIN, 256, 256, 2, 4, 2>(w, wi, wj, wn, XcdWalk(wi * wj, block, blocks),
+                                                                  lds);
+  gemm_tiles<KIND, false, true, false, E_PLAIN, 256, 256, 2, 4, 2>(
+      x, xi, xj, xn, SecondWalk(wi * wj, xi * xj, extra, block, blocks), lds);
 }
 
 // How many tiles of x the light workgroups take first, or -1 where two launches take as

@@ -17,7 +17,6 @@ namespace mi355 {
 namespace {
 
 typedef mi355moe_gated_linear_backward_args GradArgs;
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // f(z) and f'(z) of the gate.
 //   SiLU, s = sigmoid(z):  f = z s,  f' = s (1 + z (1 - s))

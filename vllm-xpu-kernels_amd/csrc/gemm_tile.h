@@ -18,8 +18,8 @@
 // stored; the last stage's r past R are cleared in LDS.
 //
 // The epilogue takes the sums from the registers: a swap of half waves gives each lane 8
-// consecutive columns, stored 16 bytes (32 rows x 32 bytes) at a time; the scales of int8
-// and the biases wait in LDS, residuals are loaded one row of tiles ahead.  No LDS
+// consecutive columns, one of 16-lane groups makes a wave's 16-byte stores 16 rows x 64 bytes
+// (of 16-bit outputs); the scales of int8 and the biases wait in LDS, residuals are loaded one row of tiles ahead.  No LDS
 // of the ring is needed for that, so a workgroup takes tile after tile, and the next one's
 // first stages are on their way meanwhile.
 #pragma once
@@ -174,13 +174,17 @@ int launch_gemm(const LinArgs& a, const TilePlan& p, int per_cu, hipStream_t st)
   MI_LAUNCH_CHECK();
   return MI355MOE_OK;
 }
-// Waves and stages.  8 waves hide each other's latency where a CU holds one workgroup: 256 x 256 in
-// 8 waves of 128 x 64 against 4 of 128 x 128, which read a third less from LDS (in turn, us: int8
-// 8192 x 7168 x 4096 gated 214 / 232, kept 421 / 447, dx 8192 x 4096 x 7168 412 / 433, dW 4096 x
-// 8192 x 7168 405 / 413); 128 x 128 in 8 and 4 (int8 1003 x 2880 x 2880 21.0 / 23.9).  Small
-// tiles share a CU: 64 x 128 with two workgroups of three stages against one of four (dW 2048 x 512 x
-// 4096 16.6 / 21.9, int8 1003 x 2880 x 2880 22.9 / 28.9), 64 x 64 three of three, two of four and
-// one of eight (dx 512 x 2048 x 4096 16.5 / 17.0 / 25.7).
+// Waves and stages.  Where a CU holds one workgroup, tiles with sides of 128 and 256 have 8 waves,
+// which hide each other's latency; those with a side of 96 or 192, for the fill of the CUs, have 4
+// (more were not measured).  256 x 256 in 8 waves of 128 x 64 against 4 of 128 x 128, which read a
+// third less from LDS (in turn, us: int8 8192 x 7168 x 4096 gated 214 / 232, kept 421 / 447, dx 8192
+// x 4096 x 7168 412 / 433, dW 4096 x 8192 x 7168 405 / 413); 128 x 128 in 8 and 4 (int8 1003 x 2880
+// x 2880 21.0 / 23.9).  Small tiles share a CU: 64 x 128 with two workgroups of three stages against
+// one of four (dW 2048 x 512 x 4096 16.6 / 21.9, int8 1003 x 2880 x 2880 22.9 / 28.9), 64 x 64 three
+// of three, two of four and one of eight (dx 512 x 2048 x 4096 16.5 / 17.0 / 25.7).  The gated 256 x
+// 256 epilogues, int8 and kept, hold more than the 256 registers and spill 78 and 43 of them around
+// a tile (220 and 176 bytes of scratch a lane, none on the way through full stages); a stage still
+// takes 1.78 us where two of 128 x 256, which do not spill, take 1.96.  No other tile spills.
 template <int KIND, bool TQ, bool TP, bool GATED, int EPI>
 int launch_gemm_shape(const LinArgs& a, const TilePlan& p, hipStream_t st) {
   switch (p.shape) {

@@ -320,7 +320,9 @@ __device__ __forceinline__ void lin_store8_i32(const LinArgs& a, int64_t m, int6
 }
 
 // 16 bytes from column byte c of a row of `bytes` bytes, from any address;
-// zeros past its end and for rows that do not exist.
+// zeros past its end and for rows that do not exist.  (A piece that the row's end cuts is
+// loaded byte by byte, each load waited for: that chain, not the way through registers, is
+// what kernels on such rows spend most of their time on.)
 typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
 __device__ __forceinline__ uint4 row16(const uint8_t* row, bool ok, int64_t c, int64_t bytes) {
   if (!ok || c >= bytes) return make_uint4(0, 0, 0, 0);

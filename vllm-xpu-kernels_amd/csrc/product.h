@@ -42,6 +42,6 @@ int launch_product_pair(const Product& x, const Product& w, hipStream_t st);
 
 // bytes of workspace (copied rows, partial sums; 0: neither), 16-byte aligned, that launch_product wants
 size_t product_workspace(const Product& p);
-int launch_product(const Product& p, void* sums, hipStream_t st);
+int launch_product(const Product& p, void* workspace, hipStream_t st);
 
 }  // namespace mi355

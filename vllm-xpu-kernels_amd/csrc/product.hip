@@ -98,10 +98,6 @@ size_t partials(const Product& p, int splits) {
   return splits == 1 ? 0 : static_cast<size_t>(splits) * p.I * p.J * sizeof(float);
 }
 
-}  // namespace
-
-namespace {
-
 // What runs: the product on p's rows, or on a copy of them (launch_pack_rows) in the workspace,
 // before the partial sums.
 struct Run {

@@ -1350,8 +1350,9 @@ class GatedLinear : public torch::autograd::Function<GatedLinear> {
                                                  torch::autograd::variable_list grads) {
     static const auto op = gated_op<decltype(gated_linear_backward)>("_mi355_C::gated_linear_backward");
     TORCH_CHECK(!at::GradMode::is_enabled(), "gated_linear has no gradient of its gradient");
-    at::AutoDispatchBelowADInplaceOrView below;
+    // (before the guard: a hook of saved tensors may run a forward pass, as checkpointing does)
     const auto saved = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
     // (this pass may ask for less than requires a gradient; inputs 0 to 2: input, weight, bias)
     auto given = [&](const at::Tensor& t, size_t of) {
       return t.defined() && ctx->needs_input_grad(of) ? std::optional<at::Tensor>(t) : std::nullopt;
